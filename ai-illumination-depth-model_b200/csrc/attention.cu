@@ -1,0 +1,489 @@
+// Attention and its backward pass on the CUDA cores: the path of 32-bit
+// storage, and of bf16 tensors whose addresses or head sizes the tensor-core
+// kernels (attention_tc.cu) do not take.
+//
+//   S = scale Q K', masked; P = softmax(S); O = P V; lse = log sum exp S
+//   dV = P' dO; dP = dO V'; dS = P (dP - rowsum(dO O)); dQ = scale dS K; dK = scale dS' Q
+//
+// All three kernels have one shape: a tile of kFix rows stays in shared memory
+// (queries; in the key pass keys), tiles of STR rows of the other side stream
+// past it, products run as outer products from transposed tiles ([d][row]),
+// 4 x STR/16 results a thread. The probabilities are never stored: the backward
+// recomputes them from lse. It has two passes, one over key tiles for every
+// query tile (dQ) and one over query tiles for every key tile (dK, dV, summed
+// over the query heads that share a key head), so no result needs an atomic
+// and the order of every sum is fixed. Bound by the FP32 pipe.
+#include "attention.cuh"
+#include "kernels.h"
+#include "token_common.cuh"
+
+namespace illumina {
+namespace gpu {
+namespace {
+
+using namespace tok;
+
+constexpr int kThreads = 128;
+constexpr int kFix = 32;
+constexpr int kFixLd = kFix + 4;
+
+// Rows [row0, row0 + ROWS) of one head into dst[d][row] as floats; rows from
+// `end` on and columns from head_dim on are zeros.
+template <typename T, int ROWS, int DP>
+__device__ __forceinline__ void load_tile(float *dst, const AttnTensor &t, long long base, int row0, int end, int d,
+                                          bool vec) {
+  constexpr int ld = ROWS + 4;
+  const T *p = (const T *)t.p + base;
+  for (int i = threadIdx.x; i < ROWS * (DP / 4); i += kThreads) {
+    const int r = i % ROWS, c = i / ROWS * 4;
+    float v[4] = {0, 0, 0, 0};
+    if (row0 + r < end) {
+      const T *q = p + (long long)(row0 + r) * t.s[1] + c;
+      if (vec && c + 4 <= d) {
+        Pack<T, 4>::load(q, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (c + j < d) v[j] = to_f32(q[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) dst[(c + j) * ld + r] = v[j];
+  }
+}
+
+// acc[i][j] += sum over d of a[d][4 ty + i] * b[d][n tx + j].
+template <int STR, int DP>
+__device__ __forceinline__ void outer(float (&acc)[4][STR / 16], const float *a, const float *b, int ty, int tx) {
+  constexpr int N = STR / 16;
+#pragma unroll 4
+  for (int d = 0; d < DP; d++) {
+    const float4 x = *reinterpret_cast<const float4 *>(a + d * kFixLd + 4 * ty);
+    float y[N];
+    if constexpr (N == 4) {
+      const float4 w = *reinterpret_cast<const float4 *>(b + d * (STR + 4) + 4 * tx);
+      y[0] = w.x, y[1] = w.y, y[2] = w.z, y[3] = w.w;
+    } else {
+      const float2 w = *reinterpret_cast<const float2 *>(b + d * (STR + 4) + 2 * tx);
+      y[0] = w.x, y[1] = w.y;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      acc[0][j] += x.x * y[j];
+      acc[1][j] += x.y * y[j];
+      acc[2][j] += x.z * y[j];
+      acc[3][j] += x.w * y[j];
+    }
+  }
+}
+
+// acc[i][c] += sum over n of p[n][4 ty + i] * b[tx + 16 c][n].
+template <int STR, int DP>
+__device__ __forceinline__ void inner(float (&acc)[4][DP / 16], const float *p, const float *b, int ty, int tx) {
+  for (int n = 0; n < STR; n += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) x[k] = *reinterpret_cast<const float4 *>(p + (n + k) * kFixLd + 4 * ty);
+#pragma unroll
+    for (int c = 0; c < DP / 16; c++) {
+      const float4 y = *reinterpret_cast<const float4 *>(b + (tx + 16 * c) * (STR + 4) + n);
+      acc[0][c] += x[0].x * y.x + x[1].x * y.y + x[2].x * y.z + x[3].x * y.w;
+      acc[1][c] += x[0].y * y.x + x[1].y * y.y + x[2].y * y.z + x[3].y * y.w;
+      acc[2][c] += x[0].z * y.x + x[1].z * y.y + x[2].z * y.z + x[3].z * y.w;
+      acc[3][c] += x[0].w * y.x + x[1].w * y.y + x[2].w * y.z + x[3].w * y.w;
+    }
+  }
+}
+
+__device__ __forceinline__ float half_warp_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float half_warp_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The sum a row's probabilities divide by, in the exponent; a row whose logits
+// are all -inf (lse -inf) has probabilities of zero.
+__device__ __forceinline__ float row_lse(float v) { return v == -INFINITY ? INFINITY : v; }
+
+struct Vecs {
+  bool q, k, v, dout;
+};
+
+// Writes rows of a fixed tile: out[row][tx + 16 c] = acc * factor[i].
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(const AttnTensor &t, long long base, int row0, int end, int d, int ty, int tx,
+                                           const float (&acc)[4][DP / 16], const float (&f)[4]) {
+  T *p = (T *)t.p + base;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = row0 + 4 * ty + i;
+    if (r >= end) continue;
+#pragma unroll
+    for (int c = 0; c < DP / 16; c++)
+      if (tx + 16 * c < d) from_f32(p[(long long)r * t.s[1] + tx + 16 * c], acc[i][c] * f[i]);
+  }
+}
+
+// One CTA: kFix queries of one head, key tiles [split * per, ...) of `splits`
+// shares. With splits > 1 the share's output and lse go to the workspace.
+template <typename T, int DP, int STR>
+__global__ void __launch_bounds__(kThreads) k_attn(const AttnParams p, int q_tiles, int splits, Vecs vec) {
+  extern __shared__ __align__(16) float sm[];
+  float *sq = sm, *sk = sq + DP * kFixLd, *sp = sk + DP * (STR + 4);
+  constexpr int N = STR / 16;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  long long id = blockIdx.x;
+  const int split = (int)(id % splits);
+  id /= splits;
+  const int qt = q_tiles - 1 - (int)(id % q_tiles);  // long rows first
+  id /= q_tiles;
+  const int h = (int)(id % p.heads), n = (int)(id / p.heads);
+  const AttnMask mask(p, n);
+  const int row0 = qt * kFix, hk = h / (p.heads / p.kv_heads);
+  int end[4], most = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) end[i] = mask.key_end(row0 + 4 * ty + i);
+  most = mask.key_end(min(row0 + kFix, mask.q_len) - 1);
+  if (row0 >= mask.q_len) most = 0;
+  const int tiles = (most + STR - 1) / STR, per = (tiles + splits - 1) / splits;
+  const int t0 = split * per, t1 = min(tiles, t0 + per);
+  load_tile<T, kFix, DP>(sq, p.q, n * p.q.s[0] + h * p.q.s[2], row0, mask.q_len, p.head_dim, vec.q);
+  float acc[4][DP / 16], top[4], sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    top[i] = -INFINITY, sum[i] = 0;
+#pragma unroll
+    for (int c = 0; c < DP / 16; c++) acc[i][c] = 0;
+  }
+  for (int t = t0; t < t1; t++) {
+    __syncthreads();
+    load_tile<T, STR, DP>(sk, p.k, n * p.k.s[0] + hk * p.k.s[2], t * STR, mask.k_len, p.head_dim, vec.k);
+    __syncthreads();
+    float s[4][N];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) s[i][j] = 0;
+    outer<STR, DP>(s, sq, sk, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float m = top[i];
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        s[i][j] = t * STR + N * tx + j < end[i] ? s[i][j] * p.scale : -INFINITY;
+        m = fmaxf(m, s[i][j]);
+      }
+      m = half_warp_max(m);
+      const float base = m == -INFINITY ? 0.0f : m;  // a row that has seen no key yet
+      const float f = expf(top[i] - base);
+      top[i] = m;
+      float add = 0;
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        s[i][j] = expf(s[i][j] - base);
+        add += s[i][j];
+      }
+      sum[i] = sum[i] * f + half_warp_sum(add);
+#pragma unroll
+      for (int c = 0; c < DP / 16; c++) acc[i][c] *= f;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      *reinterpret_cast<float4 *>(sp + (N * tx + j) * kFixLd + 4 * ty) =
+          make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+    __syncthreads();
+    load_tile<T, STR, DP>(sk, p.v, n * p.v.s[0] + hk * p.v.s[2], t * STR, mask.k_len, p.head_dim, vec.v);
+    __syncthreads();
+    inner<STR, DP>(acc, sp, sk, ty, tx);
+  }
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    f[i] = sum[i] > 0 ? 1.0f / sum[i] : (sum[i] == 0 ? 0.0f : NAN);
+    sum[i] = sum[i] == 0 ? -INFINITY : top[i] + logf(sum[i]);
+  }
+  const long long row = ((long long)n * p.heads + h) * p.q_tokens + row0;
+  if (splits == 1) {
+    store_rows<T, DP>(p.out, n * p.out.s[0] + h * p.out.s[2], row0, p.q_tokens, p.head_dim, ty, tx, acc, f);
+    if (tx == 0)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (row0 + 4 * ty + i < p.q_tokens) p.lse[row + 4 * ty + i] = sum[i];
+    return;
+  }
+  const long long rows = (long long)p.batch * p.heads * p.q_tokens;
+  AttnTensor part;
+  part.p = p.ws + split * rows * p.head_dim;
+  part.s[1] = p.head_dim;
+  store_rows<float, DP>(part, (row - row0) * p.head_dim, row0, p.q_tokens, p.head_dim, ty, tx, acc, f);
+  if (tx == 0)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (row0 + 4 * ty + i < p.q_tokens) p.ws[splits * rows * p.head_dim + split * rows + row + 4 * ty + i] = sum[i];
+}
+
+// Joins the shares of a split forward: a warp takes one row.
+//   lse = log sum_s exp(lse_s),  out = sum_s exp(lse_s - lse) out_s
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_join(const AttnParams p, int splits) {
+  const long long rows = (long long)p.batch * p.heads * p.q_tokens;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  const float *sums = p.ws + splits * rows * p.head_dim + row;
+  float top = -INFINITY;
+  for (int s = 0; s < splits; s++) {
+    const float v = sums[s * rows];
+    top = v != v ? v : fmaxf(top, v);
+  }
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0;
+  for (int s = 0; s < splits; s++) total += expf(sums[s * rows] - base);
+  const float inv = total == 0 ? 0.0f : 1.0f / total;
+  const long long i = row % p.q_tokens, bh = row / p.q_tokens;
+  T *out = (T *)p.out.p + bh / p.heads * p.out.s[0] + i * p.out.s[1] + bh % p.heads * p.out.s[2];
+  for (int d = lane; d < p.head_dim; d += 32) {
+    float o = 0;
+    for (int s = 0; s < splits; s++) {
+      const float f = expf(sums[s * rows] - base) * inv;
+      if (f != 0) o += f * p.ws[(s * rows + row) * p.head_dim + d];
+    }
+    from_f32(out[d], o);
+  }
+  if (lane == 0) p.lse[row] = total == 0 ? -INFINITY : top + logf(total);
+}
+
+// delta[row] = sum over d of dout * out; a warp takes one row.
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_delta(const AttnParams p) {
+  const long long rows = (long long)p.batch * p.heads * p.q_tokens;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  const long long i = row % p.q_tokens, bh = row / p.q_tokens, n = bh / p.heads, h = bh % p.heads;
+  const AttnMask mask(p, (int)n);
+  float s = 0;
+  if (i < mask.q_len) {
+    const T *a = (const T *)p.dout.p + n * p.dout.s[0] + i * p.dout.s[1] + h * p.dout.s[2];
+    const T *b = (const T *)p.out.p + n * p.out.s[0] + i * p.out.s[1] + h * p.out.s[2];
+    for (int d = lane; d < p.head_dim; d += 32) s += to_f32(a[d]) * to_f32(b[d]);
+  }
+  s = warp_sum(s);
+  if (lane == 0) p.ws[row] = s;
+}
+
+// dQ: one CTA takes kFix queries of one head past the keys they see.
+template <typename T, int DP, int STR>
+__global__ void __launch_bounds__(kThreads) k_attn_dq(const AttnParams p, int q_tiles, Vecs vec) {
+  extern __shared__ __align__(16) float sm[];
+  float *sq = sm, *sg = sq + DP * kFixLd, *sk = sg + DP * kFixLd, *sv = sk + DP * (STR + 4),
+        *sp = sv + DP * (STR + 4);
+  constexpr int N = STR / 16;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  long long id = blockIdx.x;
+  const int qt = q_tiles - 1 - (int)(id % q_tiles);
+  id /= q_tiles;
+  const int h = (int)(id % p.heads), n = (int)(id / p.heads);
+  const AttnMask mask(p, n);
+  const int row0 = qt * kFix, hk = h / (p.heads / p.kv_heads);
+  const int most = row0 < mask.q_len ? mask.key_end(min(row0 + kFix, mask.q_len) - 1) : 0;
+  load_tile<T, kFix, DP>(sq, p.q, n * p.q.s[0] + h * p.q.s[2], row0, mask.q_len, p.head_dim, vec.q);
+  load_tile<T, kFix, DP>(sg, p.dout, n * p.dout.s[0] + h * p.dout.s[2], row0, mask.q_len, p.head_dim, vec.dout);
+  float acc[4][DP / 16], lse[4], delta[4], f[4];
+  int end[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = row0 + 4 * ty + i;
+    const long long row = ((long long)n * p.heads + h) * p.q_tokens + r;
+    end[i] = mask.key_end(r);
+    lse[i] = end[i] ? row_lse(p.lse[row]) : 0.0f;
+    delta[i] = end[i] ? p.ws[row] : 0.0f;
+    f[i] = p.scale;
+#pragma unroll
+    for (int c = 0; c < DP / 16; c++) acc[i][c] = 0;
+  }
+  for (int k0 = 0; k0 < most; k0 += STR) {
+    __syncthreads();
+    load_tile<T, STR, DP>(sk, p.k, n * p.k.s[0] + hk * p.k.s[2], k0, mask.k_len, p.head_dim, vec.k);
+    load_tile<T, STR, DP>(sv, p.v, n * p.v.s[0] + hk * p.v.s[2], k0, mask.k_len, p.head_dim, vec.v);
+    __syncthreads();
+    float s[4][N], g[4][N];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) s[i][j] = g[i][j] = 0;
+    outer<STR, DP>(s, sq, sk, ty, tx);
+    outer<STR, DP>(g, sg, sv, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        s[i][j] = k0 + N * tx + j < end[i] ? expf(s[i][j] * p.scale - lse[i]) * (g[i][j] - delta[i]) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      *reinterpret_cast<float4 *>(sp + (N * tx + j) * kFixLd + 4 * ty) =
+          make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+    __syncthreads();
+    inner<STR, DP>(acc, sp, sk, ty, tx);
+  }
+  store_rows<T, DP>(p.dq, n * p.dq.s[0] + h * p.dq.s[2], row0, p.q_tokens, p.head_dim, ty, tx, acc, f);
+}
+
+// dK, dV: one CTA takes kFix keys of one key head past the queries that see
+// them, of every query head that shares it.
+template <typename T, int DP, int STR>
+__global__ void __launch_bounds__(kThreads) k_attn_dkv(const AttnParams p, int k_tiles, Vecs vec) {
+  extern __shared__ __align__(16) float sm[];
+  float *sk = sm, *sv = sk + DP * kFixLd, *sq = sv + DP * kFixLd, *sg = sq + DP * (STR + 4),
+        *sp = sg + DP * (STR + 4), *ss = sp + STR * kFixLd;
+  constexpr int N = STR / 16;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  long long id = blockIdx.x;
+  const int kt = (int)(id % k_tiles);
+  id /= k_tiles;
+  const int hk = (int)(id % p.kv_heads), n = (int)(id / p.kv_heads), group = p.heads / p.kv_heads;
+  const AttnMask mask(p, n);
+  const int key0 = kt * kFix;
+  load_tile<T, kFix, DP>(sk, p.k, n * p.k.s[0] + hk * p.k.s[2], key0, mask.k_len, p.head_dim, vec.k);
+  load_tile<T, kFix, DP>(sv, p.v, n * p.v.s[0] + hk * p.v.s[2], key0, mask.k_len, p.head_dim, vec.v);
+  float dk[4][DP / 16], dv[4][DP / 16];
+  int begin[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int key = key0 + 4 * ty + i;
+    begin[i] = key < mask.k_len ? mask.row_begin(key) : mask.q_len;
+#pragma unroll
+    for (int c = 0; c < DP / 16; c++) dk[i][c] = dv[i][c] = 0;
+  }
+  const int first = key0 < mask.k_len ? mask.row_begin(key0) / STR * STR : mask.q_len;
+  for (int h = hk * group; h < (hk + 1) * group; h++)
+    for (int q0 = first; q0 < mask.q_len; q0 += STR) {
+      __syncthreads();
+      load_tile<T, STR, DP>(sq, p.q, n * p.q.s[0] + h * p.q.s[2], q0, mask.q_len, p.head_dim, vec.q);
+      load_tile<T, STR, DP>(sg, p.dout, n * p.dout.s[0] + h * p.dout.s[2], q0, mask.q_len, p.head_dim, vec.dout);
+      float lse[N], delta[N];
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const int r = q0 + N * tx + j;
+        const long long row = ((long long)n * p.heads + h) * p.q_tokens + r;
+        lse[j] = r < mask.q_len ? row_lse(p.lse[row]) : 0.0f;
+        delta[j] = r < mask.q_len ? p.ws[row] : 0.0f;
+      }
+      __syncthreads();
+      float s[4][N], g[4][N];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < N; j++) s[i][j] = g[i][j] = 0;
+      outer<STR, DP>(s, sk, sq, ty, tx);
+      outer<STR, DP>(g, sv, sg, ty, tx);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+          const int r = q0 + N * tx + j;
+          const float pr = r >= begin[i] && r < mask.q_len ? expf(s[i][j] * p.scale - lse[j]) : 0.0f;
+          s[i][j] = pr;
+          g[i][j] = r >= begin[i] && r < mask.q_len ? pr * (g[i][j] - delta[j]) : 0.0f;
+        }
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        *reinterpret_cast<float4 *>(sp + (N * tx + j) * kFixLd + 4 * ty) =
+            make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+        *reinterpret_cast<float4 *>(ss + (N * tx + j) * kFixLd + 4 * ty) =
+            make_float4(g[0][j], g[1][j], g[2][j], g[3][j]);
+      }
+      __syncthreads();
+      inner<STR, DP>(dv, sp, sg, ty, tx);
+      inner<STR, DP>(dk, ss, sq, ty, tx);
+    }
+  const float one[4] = {1, 1, 1, 1}, sc[4] = {p.scale, p.scale, p.scale, p.scale};
+  store_rows<T, DP>(p.dk, n * p.dk.s[0] + hk * p.dk.s[2], key0, p.k_tokens, p.head_dim, ty, tx, dk, sc);
+  store_rows<T, DP>(p.dv, n * p.dv.s[0] + hk * p.dv.s[2], key0, p.k_tokens, p.head_dim, ty, tx, dv, one);
+}
+
+// A tensor whose rows can be read four elements at a time.
+template <typename T>
+bool vec_rows(const AttnTensor &t) {
+  return reinterpret_cast<uintptr_t>(t.p) % (4 * sizeof(T)) == 0 && t.s[0] % 4 == 0 && t.s[1] % 4 == 0 && t.s[2] % 4 == 0;
+}
+
+int ceil_div(long long a, int b) { return (int)((a + b - 1) / b); }
+
+// Shares of the keys in the forward: as many as give every SM a CTA, while a
+// share keeps at least four key tiles (joining costs another launch).
+template <int STR>
+int simt_splits(const AttnParams &p) {
+  const long long ctas = (long long)p.batch * p.heads * ceil_div(p.q_tokens, kFix);
+  const int tiles = ceil_div(p.k_tokens, STR);
+  if (ctas == 0 || ctas >= 148 || tiles < 8) return 1;
+  const int want = (int)((2 * 148 + ctas - 1) / ctas), most = tiles / 4;
+  return want < most ? want : most;
+}
+
+template <typename T, int DP, int STR>
+cudaError_t run_simt(const AttnParams &p, bool bwd, cudaStream_t st) {
+  const Vecs vec{vec_rows<T>(p.q), vec_rows<T>(p.k), vec_rows<T>(p.v), bwd && vec_rows<T>(p.dout)};
+  const int q_tiles = ceil_div(p.q_tokens, kFix), k_tiles = ceil_div(p.k_tokens, kFix);
+  const long long rows = (long long)p.batch * p.heads * p.q_tokens;
+  constexpr size_t fix = sizeof(float) * DP * kFixLd, str = sizeof(float) * DP * (STR + 4),
+                   prob = sizeof(float) * STR * kFixLd;
+  auto big = [](const void *f, size_t bytes) {
+    return bytes > 48 * 1024 ? cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+  };
+  cudaError_t e;
+  if (!bwd) {
+    const int splits = simt_splits<STR>(p);
+    const size_t sm = fix + str + prob;
+    if ((e = big((const void *)k_attn<T, DP, STR>, sm)) != cudaSuccess) return e;
+    const long long grid = (long long)p.batch * p.heads * q_tiles * splits;
+    if (grid > 0) k_attn<T, DP, STR><<<(unsigned)grid, kThreads, sm, st>>>(p, q_tiles, splits, vec);
+    if (splits > 1) k_attn_join<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, splits);
+    return cudaGetLastError();
+  }
+  if (rows > 0) {
+    k_attn_delta<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
+    const size_t sm = 2 * fix + 2 * str + prob;
+    if ((e = big((const void *)k_attn_dq<T, DP, STR>, sm)) != cudaSuccess) return e;
+    k_attn_dq<T, DP, STR><<<(unsigned)((long long)p.batch * p.heads * q_tiles), kThreads, sm, st>>>(p, q_tiles, vec);
+  }
+  const long long grid = (long long)p.batch * p.kv_heads * k_tiles;
+  if (grid > 0) {
+    const size_t sm = 2 * fix + 2 * str + 2 * prob;
+    if ((e = big((const void *)k_attn_dkv<T, DP, STR>, sm)) != cudaSuccess) return e;
+    k_attn_dkv<T, DP, STR><<<(unsigned)grid, kThreads, sm, st>>>(p, k_tiles, vec);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_simt(const AttnParams &p, bool bwd, cudaStream_t st) {
+  if (p.head_dim <= 32) return run_simt<T, 32, 64>(p, bwd, st);
+  if (p.head_dim <= 64) return run_simt<T, 64, 64>(p, bwd, st);
+  return run_simt<T, 128, 32>(p, bwd, st);
+}
+
+}  // namespace
+
+size_t attention_workspace(int T, const AttnParams &p, bool backward) {
+  const size_t rows = (size_t)p.batch * p.heads * p.q_tokens;
+  if (backward) return rows * sizeof(float);
+  const int splits = p.head_dim <= 64 ? simt_splits<64>(p) : simt_splits<32>(p);
+  return splits == 1 ? 0 : splits * rows * (p.head_dim + 1) * sizeof(float);
+}
+
+cudaError_t attention(int T, const AttnParams &p, cudaStream_t st) {
+  return T == F32 ? run_simt<float>(p, false, st) : run_simt<bf16>(p, false, st);
+}
+
+cudaError_t attention_backward(int T, const AttnParams &p, cudaStream_t st) {
+  return T == F32 ? run_simt<float>(p, true, st) : run_simt<bf16>(p, true, st);
+}
+
+}  // namespace gpu
+}  // namespace illumina

@@ -1,0 +1,368 @@
+// Layer norm over the last dimension, forward and backward.
+//
+//   y  = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(var + eps)
+//   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)),  g = w * dy
+//   dw = sum over rows of dy * xhat,  db = sum over rows of dy
+//
+// Bound by HBM: the forward reads x and writes y, the backward reads x and dy
+// and writes dx. A row's elements stay in registers between the statistics
+// (two passes over the registers: the mean, then the squared distances from
+// it) and the output. One warp takes a row of up to 1024 elements (no block
+// barrier), a CTA of 256 threads one of up to 4096, and rows beyond that are
+// re-read. In the backward a thread owns the same columns in every row it
+// sees, so dw and db accumulate in registers; one partial row per CTA goes to
+// the workspace and a second launch adds the partials in a fixed order, so
+// that results do not depend on scheduling.
+#include "token_common.cuh"
+#include "token_ops.h"
+
+namespace illumina {
+namespace gpu {
+namespace {
+
+using namespace tok;
+
+constexpr int kThreads = 256;
+
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float *red) {
+  v = warp_sum(v);
+  if constexpr (LANES > 32) {
+    const int w = threadIdx.x >> 5;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[w] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < LANES / 32; i++) v += red[i];
+  }
+  return v;
+}
+
+template <typename T, int VW, int VPT, int LANES>
+__global__ void __launch_bounds__(kThreads) k_norm(const T *__restrict__ x, long long xs, long long rows, int c,
+                                                   const float *__restrict__ w, const float *__restrict__ b, float eps,
+                                                   T *__restrict__ y, long long ys, float *mean, float *rstd) {
+  __shared__ float red[kThreads / 32];
+  const int lane = threadIdx.x % LANES;
+  const long long row = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  if (row >= rows) return;  // uniform over the threads of a row
+  const T *xr = x + row * xs;
+  float v[VPT][VW];
+  float s = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    const int col = (i * LANES + lane) * VW;
+    if (col < c) {
+      Pack<T, VW>::load(xr + col, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VW; j++) v[i][j] = 0;
+    }
+#pragma unroll
+    for (int j = 0; j < VW; j++) s += v[i][j];
+  }
+  const float mu = row_sum<LANES>(s, red) / c;
+  float q = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    const int col = (i * LANES + lane) * VW;
+#pragma unroll
+    for (int j = 0; j < VW; j++) {
+      v[i][j] -= mu;
+      if (col < c) q += v[i][j] * v[i][j];
+    }
+  }
+  const float r = 1.0f / sqrtf(row_sum<LANES>(q, red) / c + eps);
+  if (lane == 0) {
+    if (mean) mean[row] = mu;
+    if (rstd) rstd[row] = r;
+  }
+  T *yr = y + row * ys;
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    const int col = (i * LANES + lane) * VW;
+    if (col >= c) break;
+    float o[VW];
+#pragma unroll
+    for (int j = 0; j < VW; j++) {
+      o[j] = v[i][j] * r;
+      if (w) o[j] *= w[col + j];
+      if (b) o[j] += b[col + j];
+    }
+    Pack<T, VW>::store(yr + col, o);
+  }
+}
+
+// Rows longer than the registers hold: three readings of x.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_norm_long(const T *__restrict__ x, long long xs, int c,
+                                                        const float *__restrict__ w, const float *__restrict__ b,
+                                                        float eps, T *__restrict__ y, long long ys, float *mean,
+                                                        float *rstd) {
+  __shared__ float red[kThreads / 32];
+  const long long row = blockIdx.x;
+  const T *xr = x + row * xs;
+  float s = 0;
+  for (int i = threadIdx.x; i < c; i += kThreads) s += to_f32(xr[i]);
+  const float mu = row_sum<kThreads>(s, red) / c;
+  float q = 0;
+  for (int i = threadIdx.x; i < c; i += kThreads) {
+    const float d = to_f32(xr[i]) - mu;
+    q += d * d;
+  }
+  const float r = 1.0f / sqrtf(row_sum<kThreads>(q, red) / c + eps);
+  if (threadIdx.x == 0) {
+    if (mean) mean[row] = mu;
+    if (rstd) rstd[row] = r;
+  }
+  for (int i = threadIdx.x; i < c; i += kThreads) {
+    float o = (to_f32(xr[i]) - mu) * r;
+    if (w) o *= w[i];
+    if (b) o += b[i];
+    from_f32(y[row * ys + i], o);
+  }
+}
+
+// part: [gridDim.x][2][c], or null when neither dw nor db is wanted.
+template <typename T, int VW, int VPT, int LANES>
+__global__ void __launch_bounds__(kThreads) k_norm_bwd(const T *__restrict__ dy, long long dys,
+                                                       const T *__restrict__ x, long long xs, long long rows, int c,
+                                                       const float *__restrict__ w, const float *__restrict__ mean,
+                                                       const float *__restrict__ rstd, T *__restrict__ dx,
+                                                       long long dxs, float *__restrict__ part) {
+  extern __shared__ float sums[];  // [rows per CTA][c] when a warp takes a row
+  __shared__ float red[kThreads / 32];
+  constexpr int kRows = kThreads / LANES;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  float aw[VPT][VW], ab[VPT][VW];
+#pragma unroll
+  for (int i = 0; i < VPT; i++)
+#pragma unroll
+    for (int j = 0; j < VW; j++) aw[i][j] = ab[i][j] = 0;
+  for (long long row = (long long)blockIdx.x * kRows + group; row < rows; row += (long long)gridDim.x * kRows) {
+    const T *xr = x + row * xs, *gr = dy + row * dys;
+    const float mu = mean[row], r = rstd[row];
+    float h[VPT][VW], g[VPT][VW];
+    float s0 = 0, s1 = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+      const int col = (i * LANES + lane) * VW;
+      if (col < c) {
+        Pack<T, VW>::load(xr + col, h[i]);
+        Pack<T, VW>::load(gr + col, g[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+      const int col = (i * LANES + lane) * VW;
+      if (col >= c) break;
+#pragma unroll
+      for (int j = 0; j < VW; j++) {
+        h[i][j] = (h[i][j] - mu) * r;
+        aw[i][j] += g[i][j] * h[i][j];
+        ab[i][j] += g[i][j];
+        if (w) g[i][j] *= __ldg(w + col + j);
+        s0 += g[i][j];
+        s1 += g[i][j] * h[i][j];
+      }
+    }
+    s0 = row_sum<LANES>(s0, red) / c;
+    s1 = row_sum<LANES>(s1, red) / c;
+    if (dx) {
+      T *dr = dx + row * dxs;
+#pragma unroll
+      for (int i = 0; i < VPT; i++) {
+        const int col = (i * LANES + lane) * VW;
+        if (col >= c) break;
+        float o[VW];
+#pragma unroll
+        for (int j = 0; j < VW; j++) o[j] = r * (g[i][j] - s0 - h[i][j] * s1);
+        Pack<T, VW>::store(dr + col, o);
+      }
+    }
+  }
+  if (!part) return;
+  float *out = part + (size_t)blockIdx.x * 2 * c;
+  if constexpr (LANES == kThreads) {
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+      const int col = (i * LANES + lane) * VW;
+      if (col >= c) break;
+#pragma unroll
+      for (int j = 0; j < VW; j++) out[col + j] = aw[i][j], out[c + col + j] = ab[i][j];
+    }
+  } else {
+    for (int which = 0; which < 2; which++) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < VPT; i++) {
+        const int col = (i * LANES + lane) * VW;
+        if (col >= c) break;
+#pragma unroll
+        for (int j = 0; j < VW; j++) sums[group * c + col + j] = which ? ab[i][j] : aw[i][j];
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < c; i += kThreads) {
+        float t = 0;
+#pragma unroll
+        for (int k = 0; k < kRows; k++) t += sums[k * c + i];
+        out[which * c + i] = t;
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_norm_bwd_long(const T *__restrict__ dy, long long dys,
+                                                            const T *__restrict__ x, long long xs, long long rows,
+                                                            int c, const float *__restrict__ w,
+                                                            const float *__restrict__ mean,
+                                                            const float *__restrict__ rstd, T *__restrict__ dx,
+                                                            long long dxs, float *__restrict__ part) {
+  __shared__ float red[kThreads / 32];
+  float *out = part ? part + (size_t)blockIdx.x * 2 * c : nullptr;
+  if (out)
+    for (int i = threadIdx.x; i < 2 * c; i += kThreads) out[i] = 0;  // each thread adds to its own columns only
+  __syncthreads();
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T *xr = x + row * xs, *gr = dy + row * dys;
+    const float mu = mean[row], r = rstd[row];
+    float s0 = 0, s1 = 0;
+    for (int i = threadIdx.x; i < c; i += kThreads) {
+      const float h = (to_f32(xr[i]) - mu) * r, d = to_f32(gr[i]);
+      if (out) out[i] += d * h, out[c + i] += d;
+      const float g = w ? d * w[i] : d;
+      s0 += g;
+      s1 += g * h;
+    }
+    s0 = row_sum<kThreads>(s0, red) / c;
+    s1 = row_sum<kThreads>(s1, red) / c;
+    if (dx)
+      for (int i = threadIdx.x; i < c; i += kThreads) {
+        const float h = (to_f32(xr[i]) - mu) * r, d = to_f32(gr[i]);
+        const float g = w ? d * w[i] : d;
+        from_f32(dx[row * dxs + i], r * (g - s0 - h * s1));
+      }
+  }
+}
+
+// Column sums of part ([n][2c]) in a fixed order: 32 columns a CTA, its 32
+// warps take every 32nd row, then the warps' sums are added.
+__global__ void __launch_bounds__(1024) k_norm_reduce(const float *__restrict__ part, int n, int c, float *dw,
+                                                      float *db) {
+  __shared__ float s[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + tx;
+  float t = 0;
+  if (col < 2 * c)
+    for (int i = ty; i < n; i += 32) t += part[(size_t)i * 2 * c + col];
+  s[ty][tx] = t;
+  __syncthreads();
+  t = warp_sum(s[tx][ty]);
+  const int o = blockIdx.x * 32 + ty;
+  if (tx == 0 && o < 2 * c) {
+    if (o < c) {
+      if (dw) dw[o] = t;
+    } else if (db) {
+      db[o - c] = t;
+    }
+  }
+}
+
+struct NormArgs {
+  const void *x, *dy;
+  long long xs, dys, rows;
+  int c;
+  const float *w, *b;
+  float eps;
+  void *y;
+  long long ys;
+  float *mean, *rstd;
+  float *part;
+  int blocks;
+  cudaStream_t st;
+};
+
+template <typename T, int VW, int VPT, int LANES>
+void launch(const NormArgs &a, bool bwd) {
+  constexpr int kRows = kThreads / LANES;
+  const T *x = (const T *)a.x;
+  if (!bwd) {
+    k_norm<T, VW, VPT, LANES><<<(unsigned)((a.rows + kRows - 1) / kRows), kThreads, 0, a.st>>>(
+        x, a.xs, a.rows, a.c, a.w, a.b, a.eps, (T *)a.y, a.ys, a.mean, a.rstd);
+  } else {
+    const size_t sm = LANES == kThreads || !a.part ? 0 : (size_t)kRows * a.c * sizeof(float);
+    k_norm_bwd<T, VW, VPT, LANES><<<a.blocks, kThreads, sm, a.st>>>((const T *)a.dy, a.dys, x, a.xs, a.rows, a.c, a.w,
+                                                                  a.mean, a.rstd, (T *)a.y, a.ys, a.part);
+  }
+}
+
+// Smallest register tile that holds a row.
+template <typename T, int VW>
+bool pick(const NormArgs &a, bool bwd) {
+  constexpr int e = VW == 1 ? 4 : VW;  // elements a thread holds at least
+  constexpr int u = e / VW;
+  if (a.c <= 32 * e) launch<T, VW, u, 32>(a, bwd);
+  else if (a.c <= 64 * e) launch<T, VW, 2 * u, 32>(a, bwd);
+  else if (a.c <= 128 * e) launch<T, VW, 4 * u, 32>(a, bwd);
+  else if (a.c <= 256 * e && e <= 4) launch<T, VW, (e <= 4 ? 8 * u : u), 32>(a, bwd);
+  else if (a.c <= 256 * e) launch<T, VW, u, 256>(a, bwd);
+  else if (a.c <= 512 * e) launch<T, VW, 2 * u, 256>(a, bwd);
+  else if (a.c <= 1024 * e && e <= 4) launch<T, VW, (e <= 4 ? 4 * u : u), 256>(a, bwd);
+  else return false;
+  return true;
+}
+
+template <typename T>
+void dispatch(const NormArgs &a, bool bwd) {
+  constexpr int V = 16 / sizeof(T);
+  bool vec = a.c % V == 0 && a.xs % V == 0 && a.ys % V == 0 && aligned16(a.x) && aligned16(a.y);
+  if (bwd) vec = vec && a.dys % V == 0 && aligned16(a.dy);
+  if (vec ? pick<T, V>(a, bwd) : pick<T, 1>(a, bwd)) return;
+  if (!bwd)
+    k_norm_long<T><<<(unsigned)a.rows, kThreads, 0, a.st>>>((const T *)a.x, a.xs, a.c, a.w, a.b, a.eps, (T *)a.y, a.ys,
+                                                            a.mean, a.rstd);
+  else
+    k_norm_bwd_long<T><<<a.blocks, kThreads, 0, a.st>>>((const T *)a.dy, a.dys, (const T *)a.x, a.xs, a.rows, a.c, a.w,
+                                                        a.mean, a.rstd, (T *)a.y, a.ys, a.part);
+}
+
+}  // namespace
+
+cudaError_t layer_norm(int T, const void *x, long long xs, long long rows, int c, const float *w, const float *b,
+                       float eps, void *y, long long ys, float *mean, float *rstd, cudaStream_t st) {
+  if (rows == 0) return cudaSuccess;
+  NormArgs a{};
+  a.x = x, a.xs = xs, a.rows = rows, a.c = c, a.w = w, a.b = b, a.eps = eps, a.y = y, a.ys = ys, a.mean = mean;
+  a.rstd = rstd, a.st = st;
+  if (T == 0) dispatch<float>(a, false);
+  else dispatch<bf16>(a, false);
+  return cudaGetLastError();
+}
+
+int layer_norm_blocks(long long rows, int c) {
+  // two waves of resident CTAs at most: every CTA leaves one partial row
+  const long long per = c <= 1024 ? kThreads / 32 : 1;
+  const long long want = (rows + per - 1) / per;
+  return (int)(want < 2 * 148 ? want : 2 * 148);
+}
+
+cudaError_t layer_norm_backward(int T, const void *dy, long long dys, const void *x, long long xs, long long rows,
+                                int c, const float *w, const float *mean, const float *rstd, void *dx, long long dxs,
+                                float *dw, float *db, float *ws, cudaStream_t st) {
+  NormArgs a{};
+  a.dy = dy, a.dys = dys, a.x = x, a.xs = xs, a.rows = rows, a.c = c, a.w = w, a.mean = const_cast<float *>(mean);
+  a.rstd = const_cast<float *>(rstd), a.y = dx, a.ys = dxs, a.st = st;
+  a.part = dw || db ? ws : nullptr;
+  a.blocks = layer_norm_blocks(rows, c);
+  if (rows > 0) {
+    if (T == 0) dispatch<float>(a, true);
+    else dispatch<bf16>(a, true);
+  }
+  if (dw || db) k_norm_reduce<<<(2 * c + 31) / 32, 1024, 0, st>>>(ws, a.blocks, c, dw, db);
+  return cudaGetLastError();
+}
+
+}  // namespace gpu
+}  // namespace illumina

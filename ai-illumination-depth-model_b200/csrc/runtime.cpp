@@ -18,6 +18,7 @@
 #include <fstream>
 #include <mutex>
 
+#include "api.h"
 #include "host.h"
 #include "illumina.h"
 #include "kernels.h"
@@ -32,22 +33,6 @@ thread_local std::string g_last_error;
 void set_last_error(const std::string &msg) { g_last_error = msg; }
 }  // namespace illumina
 
-#define ILL_TRY try {
-#define ILL_CATCH                                          \
-  }                                                        \
-  catch (const Error &e) {                                 \
-    set_last_error(e.what());                              \
-    return e.status;                                       \
-  }                                                        \
-  catch (const std::bad_alloc &) {                         \
-    set_last_error("out of host memory");                  \
-    return ILLUMINA_INVALID_ARG;                           \
-  }                                                        \
-  catch (const std::exception &e) {                        \
-    set_last_error(e.what());                              \
-    return ILLUMINA_INVALID_ARG;                           \
-  }
-
 namespace {
 
 // Split-K workspace of the tensor-core kernels: a model holds 16 MiB of fp32
@@ -57,11 +42,6 @@ constexpr size_t kSplitKBytes = 16u << 20;
 constexpr size_t kSplitKOpBytes = 8u << 20;
 // Largest batch whose forward uses programmatic dependent launch.
 constexpr int kPdlMaxBatch = 16;
-
-void cuda_check(cudaError_t e, const char *what) {
-  if (e != cudaSuccess)
-    throw Error(ILLUMINA_CUDA_ERROR, std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")");
-}
 
 bool is_device_ptr(const void *p) {
   if (!p) return false;
@@ -1098,10 +1078,6 @@ struct Scratch {
     if (p) cudaFreeAsync(p, st);
   }
 };
-
-void require(bool ok, const std::string &msg) {
-  if (!ok) throw Error(ILLUMINA_INVALID_ARG, msg);
-}
 
 thread_local int g_op_engine = ILLUMINA_ENGINE_SIMT;
 

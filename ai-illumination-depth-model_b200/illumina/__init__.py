@@ -12,6 +12,8 @@ The names mirror the reference's TypeScript API surface for the hot path:
   frame     renderFrame -> FrameResult                               (src/engine/frame.ts)
   scene     createProceduralScene, renderScenes, evaluateDepth       (src/scene/procedural.ts, metrics.ts)
   ops       per-kernel entry points                                  (src/model/kernels/*.ts)
+            layerNorm, rotary (createRotary), attention and their gradients  (no counterpart)
+  optimizer createOptimizer -> AdamW                                 (no counterpart)
   bundle    readBundle, writeBundle, dumpForward (ntb/1)             (scripts/ref-forward.ts)
   ref_forward  the ref-forward CLI on the CUDA path: python -m illumina.ref_forward
 
@@ -24,6 +26,8 @@ from .bundle import dumpForward, readBundle, writeBundle  # noqa: F401
 from .frame import FrameResult, renderFrame  # noqa: F401
 from .lighting import (DEFAULT_SETTINGS, MAX_LIGHTS, LightDescription, LightKind, Renderer,  # noqa: F401
                        ShadingSettings, createRenderer, packLights)
+from .ops import RotaryPlan, createRotary  # noqa: F401
+from .optimizer import AdamW, createOptimizer  # noqa: F401
 from .runner import DepthModel, createDepthModel, cropTransform  # noqa: F401
 from .scene import (DepthMetrics, ProceduralScene, createProceduralScene, evaluateDepth,  # noqa: F401
                     renderScenes, sceneParams)

@@ -78,6 +78,44 @@ class ShadeSteps(C.Structure):
     _fields_ = [("contact", C.c_int), ("ao_dirs", C.c_int), ("ao_steps", C.c_int), ("volumetric", C.c_int)]
 
 
+class RotaryTensor(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("heads", C.c_int), ("x_stride", C.c_longlong * 3),
+                ("y_stride", C.c_longlong * 3)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("precision", C.c_int), ("batch", C.c_longlong), ("tokens", C.c_longlong), ("head_dim", C.c_int),
+                ("pairs", C.c_int), ("axes", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int),
+                ("first", RotaryTensor), ("second", RotaryTensor), ("positions", C.c_void_p),
+                ("positions_float", C.c_int), ("position_stride", C.c_longlong * 3), ("turns", C.c_void_p),
+                ("axis", C.c_void_p)]
+
+
+class AttentionTensor(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_longlong * 3)]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [("precision", C.c_int), ("batch", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("q_tokens", C.c_int), ("k_tokens", C.c_int), ("causal_block", C.c_int),
+                ("scale", C.c_float), ("q", AttentionTensor), ("k", AttentionTensor), ("v", AttentionTensor),
+                ("out", AttentionTensor), ("q_lens", C.c_void_p), ("k_lens", C.c_void_p), ("lse", C.c_void_p),
+                ("dout", AttentionTensor), ("dq", AttentionTensor), ("dk", AttentionTensor), ("dv", AttentionTensor),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class AdamwOptions(C.Structure):
+    _fields_ = [("device", C.c_int), ("tensors", C.c_int), ("params", C.POINTER(C.c_void_p)),
+                ("counts", C.POINTER(C.c_longlong)), ("decay", C.POINTER(C.c_int)), ("moment_bits", C.c_int),
+                ("grad_precision", C.c_int), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p),
+                ("v_scale", C.c_void_p)]
+
+
+class AdamwHyper(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("lr_device", C.c_void_p)]
+
+
 _F = C.POINTER(C.c_float)
 _V = C.c_void_p
 _S = C.c_int  # status
@@ -131,6 +169,22 @@ SIGNATURES = {
     "illumina_op_head": (_S, [_V, C.c_long, C.c_int, _V, C.c_float, _V, _V]),
     "illumina_op_preprocess": (_S, [_V, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _V, _V, _V]),
     "illumina_op_bilateral": (_S, [_V, C.c_int, C.c_int, C.c_int, _V, C.c_int, C.c_float, _V, _V]),
+    "illumina_op_layer_norm": (_S, [C.c_int, _V, C.c_longlong, C.c_longlong, C.c_int, _V, _V, C.c_float, _V,
+                                    C.c_longlong, _V, _V, _V]),
+    "illumina_op_layer_norm_backward": (_S, [C.c_int, _V, C.c_longlong, _V, C.c_longlong, C.c_longlong, C.c_int, _V, _V,
+                                             _V, _V, C.c_longlong, _V, _V, _V, C.c_size_t, _V]),
+    "illumina_op_layer_norm_workspace": (_S, [C.c_longlong, C.c_int, C.POINTER(C.c_size_t)]),
+    "illumina_op_rotary": (_S, [C.POINTER(RotaryArgs), _V]),
+    "illumina_op_attention_workspace": (_S, [C.POINTER(AttentionArgs), C.c_int, C.POINTER(C.c_size_t)]),
+    "illumina_op_attention": (_S, [C.POINTER(AttentionArgs), _V]),
+    "illumina_op_attention_backward": (_S, [C.POINTER(AttentionArgs), _V]),
+    "illumina_adamw_blocks": (_S, [C.POINTER(C.c_longlong), C.c_int, C.POINTER(C.c_longlong)]),
+    "illumina_adamw_create": (_S, [C.POINTER(AdamwOptions), C.POINTER(C.c_void_p)]),
+    "illumina_adamw_destroy": (_S, [_V]),
+    "illumina_adamw_step": (_S, [_V, C.POINTER(C.c_void_p), C.POINTER(AdamwHyper), _V]),
+    "illumina_adamw_get_steps": (_S, [_V, C.POINTER(C.c_longlong), _V]),
+    "illumina_adamw_set_steps": (_S, [_V, C.c_longlong, _V]),
+    "illumina_adamw_moments": (_S, [_V, _V, _V, _V]),
     "illumina_shading_settings_default": (None, [C.POINTER(ShadingSettingsC)]),
     "illumina_shade": (_S, [_V, C.c_int, C.c_int, C.c_int, _V, C.c_int, C.c_int, C.POINTER(Light),
                             C.POINTER(ShadingSettingsC), C.c_uint32, C.POINTER(ShadeSteps), C.c_int,

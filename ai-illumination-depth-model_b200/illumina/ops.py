@@ -3,10 +3,24 @@
 makePreprocess, makeDepthUpsample under src/model/kernels/). Arguments are
 torch CUDA tensors in the reference's logical layouts; each call launches the
 same CUDA kernel the model uses.
+
+The token operators at the end (layerNorm, rotary, attention and their
+gradients) have no counterpart in the reference: a transformer stage over the
+network's feature maps, or over the frames of a clip. They take shaped torch
+CUDA tensors of one device, float32 or bfloat16, with any strides over a
+contiguous last dimension, and run on `stream` (a torch stream or handle; by
+default torch's current stream of that device), where their results are
+allocated too. Inputs must stay alive until the work is done. Errors are
+IlluminaError with status INVALID_ARG.
 """
 from __future__ import annotations
 
-from ._lib import ACT, ENGINE, check, lib, ptr, stream_handle
+import ctypes as C
+import math
+from dataclasses import dataclass
+
+from ._lib import (ACT, ENGINE, INVALID_ARG, PRECISION_BF16, PRECISION_F32, AttentionArgs, IlluminaError, RotaryArgs,
+                   check, lib, ptr, stream_handle)
 
 
 def set_engine(engine: str) -> None:
@@ -79,3 +93,278 @@ def bilateral(low, lh, lw, low_c, guide, guide_c, range_sigma=0.12, dst=None, st
     check(lib().illumina_op_bilateral(ptr(low), lh, lw, low_c, ptr(guide), guide_c, float(range_sigma), ptr(dst),
                                       stream_handle(stream)))
     return dst
+
+
+# ---------------------------------------------------------------------------
+# Token operators
+# ---------------------------------------------------------------------------
+
+def _require(ok, message):
+    if not ok:
+        raise IlluminaError(INVALID_ARG, message)
+
+
+class _On:
+    """Makes a tensor's device and the call's stream current for a scope; `handle` is the stream's cudaStream_t."""
+
+    def __init__(self, torch, device, stream):
+        self._scopes = []
+        if device.index != torch.cuda.current_device():
+            self._scopes.append(torch.cuda.device(device))
+        if stream is None:
+            self.handle = torch.cuda.current_stream(device).cuda_stream
+        else:
+            if isinstance(stream, int):
+                stream = torch.cuda.ExternalStream(stream, device=device)
+            self._scopes.append(torch.cuda.stream(stream))
+            self.handle = stream.cuda_stream
+
+    def __enter__(self):
+        for s in self._scopes:
+            s.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        for s in reversed(self._scopes):
+            s.__exit__(*exc)
+
+
+def _precision(torch, name, x):
+    if x.dtype == torch.float32:
+        return PRECISION_F32
+    _require(x.dtype == torch.bfloat16, f"{name} must be float32 or bfloat16")
+    return PRECISION_BF16
+
+
+def _tensor(torch, name, x, like=None, dims=None):
+    """Checks a storage tensor: on a CUDA device, contiguous in its last dimension, of `like`'s type and device."""
+    _require(isinstance(x, torch.Tensor) and x.is_cuda, f"{name} must be a CUDA tensor")
+    _require(dims is None or x.dim() == dims, f"{name} must have {dims} dimensions")
+    _require(x.dim() > 0 and (x.shape[-1] <= 1 or x.stride(-1) == 1), f"{name} must be contiguous in its last dimension")
+    if like is not None:
+        _require(x.dtype == like.dtype and x.device == like.device, f"{name} must have the type and device of the others")
+    return x
+
+
+def _vector(torch, name, x, n, device, dtype=None):
+    """Checks a contiguous vector of n elements (float32 by default); None passes."""
+    if x is None:
+        return
+    _require(isinstance(x, torch.Tensor) and x.dtype == (dtype or torch.float32) and x.device == device and
+             x.numel() == n and x.is_contiguous(),
+             f"{name} must be {n} contiguous {str(dtype or torch.float32)[6:]} values on the device of the others")
+
+
+def _rows(torch, name, x):
+    """(rows, width, row stride) of a tensor whose leading dimensions are evenly spaced rows."""
+    shape, strides = x.shape, x.stride()
+    if len(shape) == 2:
+        return shape[0], shape[1], strides[0]
+    rows, stride = 1, None
+    for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n != 1:
+            if stride is None:
+                stride = s
+            _require(rows == 0 or s == stride * rows, f"{name} must have evenly spaced rows (reshape it to two dimensions)")
+        rows *= n
+    return rows, shape[-1], shape[-1] if stride is None else stride
+
+
+def layerNorm(x, weight=None, bias=None, eps=1e-6, out=None, stream=None):
+    """Layer norm over the last dimension: (y, mean, rstd), the float32 statistics [rows] being what layerNormBackward
+    needs. weight, bias: float32 [width] or None. out may be x."""
+    import torch
+    _tensor(torch, "x", x)
+    precision = _precision(torch, "x", x)
+    rows, c, stride = _rows(torch, "x", x)
+    _require(c > 0, "x must not have a width of zero")
+    _vector(torch, "weight", weight, c, x.device)
+    _vector(torch, "bias", bias, c, x.device)
+    with _On(torch, x.device, stream) as on:
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        else:
+            _tensor(torch, "out", out, x)
+            _require(out.shape == x.shape, "out must have the shape of x")
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean, rstd = stats.unbind()
+        check(lib().illumina_op_layer_norm(precision, x.data_ptr(), stride, rows, c, ptr(weight), ptr(bias), eps,
+                                           out.data_ptr(), _rows(torch, "out", out)[2], mean.data_ptr(),
+                                           rstd.data_ptr(), on.handle))
+    return out, mean, rstd
+
+
+def layerNormBackward(dy, x, mean, rstd, weight=None, needWeight=True, stream=None):
+    """Gradients of layerNorm: (dx, dw, db); dw and db are float32 [width], None unless needWeight."""
+    import torch
+    _tensor(torch, "x", x)
+    _tensor(torch, "dy", dy, x)
+    _require(dy.shape == x.shape, "dy must have the shape of x")
+    precision = _precision(torch, "x", x)
+    rows, c, stride = _rows(torch, "x", x)
+    _, _, dy_stride = _rows(torch, "dy", dy)
+    _require(c > 0, "x must not have a width of zero")
+    _vector(torch, "weight", weight, c, x.device)
+    _require(mean is not None and rstd is not None, "mean and rstd of the forward pass are needed")
+    _vector(torch, "mean", mean, rows, x.device)
+    _vector(torch, "rstd", rstd, rows, x.device)
+    with _On(torch, x.device, stream) as on:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = db = workspace = None
+        size = C.c_size_t(0)
+        if needWeight:
+            check(lib().illumina_op_layer_norm_workspace(rows, c, C.byref(size)))
+            dw, db = torch.empty(c, dtype=torch.float32, device=x.device), torch.empty(c, dtype=torch.float32, device=x.device)
+            workspace = torch.empty(size.value, dtype=torch.uint8, device=x.device)
+        check(lib().illumina_op_layer_norm_backward(precision, dy.data_ptr(), dy_stride, x.data_ptr(), stride, rows, c,
+                                                    ptr(weight), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), c,
+                                                    ptr(dw), ptr(db), ptr(workspace), size.value, on.handle))
+    return dx, dw, db
+
+
+@dataclass(frozen=True)
+class RotaryPlan:
+    """The frequencies of a rotation, made once by createRotary: turns (float64) and axis (int32) of every pair."""
+    headDim: int
+    axes: int
+    interleaved: bool
+    turns: object
+    axis: object
+
+
+def createRotary(headDim, sections, base=10000.0, interleaved=False, spectrum="axis", device="cuda"):
+    """Rotary positions with len(sections) axes (time, row, column; any number). Axis a has sections[a] consecutive
+    pairs. spectrum "axis": its j-th pair turns by position * base**(-j / sections[a]), every axis covers all
+    frequencies; "shared": pair i of all P turns by position[axis] * base**(-i / P), the axes share one spectrum.
+    Pairs are elements (i, i + P), or neighbours (2i, 2i + 1) when interleaved; elements from 2P on stay."""
+    import torch
+    sections = [int(n) for n in sections]
+    pairs = sum(sections)
+    _require(len(sections) > 0 and all(n >= 0 for n in sections), "sections must be counts of pairs")
+    _require(pairs >= 1 and 2 * pairs <= headDim, "sections must hold between 1 and headDim / 2 pairs")
+    _require(base > 0, "base must be positive")
+    _require(spectrum in ("axis", "shared"), 'spectrum must be "axis" or "shared"')
+    turns, axis = [], []
+    for a, n in enumerate(sections):
+        for j in range(n):
+            power = j / n if spectrum == "axis" else len(turns) / pairs
+            turns.append(base ** -power / (2 * math.pi))
+            axis.append(a)
+    return RotaryPlan(int(headDim), len(sections), bool(interleaved),
+                      torch.tensor(turns, dtype=torch.float64, device=device),
+                      torch.tensor(axis, dtype=torch.int32, device=device))
+
+
+def rotary(q, positions, plan, k=None, inverse=False, outQ=None, outK=None, stream=None):
+    """Rotates q [batch, tokens, heads, headDim], and k with its own head count, by positions [axes, tokens] or [axes,
+    batch, tokens] (int32 or float32). inverse turns back: the gradient. Returns q's result, or both with k. outQ and
+    outK may be q and k."""
+    import torch
+    _tensor(torch, "q", q, dims=4)
+    precision = _precision(torch, "q", q)
+    b, t, h, d = q.shape
+    _require(d == plan.headDim, f"q must have the plan's {plan.headDim} elements a head")
+    _require(plan.turns.device == q.device, "the plan must be on the device of q")
+    _require(isinstance(positions, torch.Tensor) and positions.device == q.device and
+             positions.dtype in (torch.int32, torch.float32), "positions must be int32 or float32 on the device of q")
+    _require(tuple(positions.shape) in ((plan.axes, t), (plan.axes, b, t)),
+             "positions must be [axes, tokens] or [axes, batch, tokens]")
+    if k is not None:
+        _tensor(torch, "k", k, q, 4)
+        _require((k.shape[0], k.shape[1], k.shape[3]) == (b, t, d), "k must have the batch, tokens and head size of q")
+    args = RotaryArgs(precision=precision, batch=b, tokens=t, head_dim=d, pairs=plan.turns.numel(), axes=plan.axes,
+                      interleaved=plan.interleaved, inverse=bool(inverse), positions=positions.data_ptr(),
+                      positions_float=positions.dtype == torch.float32, turns=plan.turns.data_ptr(),
+                      axis=plan.axis.data_ptr())
+    ps = positions.stride()
+    args.position_stride[:] = (ps[0], ps[1], ps[2]) if len(ps) == 3 else (ps[0], 0, ps[1])
+    with _On(torch, q.device, stream) as on:
+        results = []
+        for slot, x, out, name in ((args.first, q, outQ, "outQ"), (args.second, k, outK, "outK")):
+            if x is None:
+                continue
+            if out is None:
+                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            else:
+                _tensor(torch, name, out, x, 4)
+                _require(out.shape == x.shape, f"{name} must have the shape of its input")
+            slot.x, slot.y, slot.heads = x.data_ptr(), out.data_ptr(), x.shape[2]
+            slot.x_stride[:], slot.y_stride[:] = x.stride()[:3], out.stride()[:3]
+            results.append(out)
+        check(lib().illumina_op_rotary(C.byref(args), on.handle))
+    return results[0] if k is None else tuple(results)
+
+
+def _set(slot, x):
+    slot.data = x.data_ptr()
+    slot.stride[:] = x.stride()[:3]
+
+
+def _attention_args(torch, q, k, v, scale, causalBlock, qLens, kLens):
+    _tensor(torch, "q", q, dims=4)
+    _tensor(torch, "k", k, q, 4)
+    _tensor(torch, "v", v, q, 4)
+    (b, tq, h, d), (_, tk, hk, _) = q.shape, k.shape
+    _require(k.shape == v.shape and k.shape[0] == b and k.shape[3] == d, "k and v must have q's batch and head size, and one shape")
+    _require(hk > 0 and h % hk == 0, "q's heads must be a multiple of the key heads")
+    _require(1 <= d <= 128, "head sizes from 1 to 128 are supported")
+    _require(max(b, h, tq, tk) < 2 ** 30, "attention: size beyond 2^30")
+    _require(isinstance(causalBlock, int) and 0 <= causalBlock < 2 ** 31, "causalBlock must be a token count, 0 for none")
+    _vector(torch, "qLens", qLens, b, q.device, torch.int32)
+    _vector(torch, "kLens", kLens, b, q.device, torch.int32)
+    args = AttentionArgs(precision=_precision(torch, "q", q), batch=b, heads=h, kv_heads=hk, head_dim=d, q_tokens=tq,
+                         k_tokens=tk, causal_block=causalBlock, scale=d ** -0.5 if scale is None else scale,
+                         q_lens=ptr(qLens), k_lens=ptr(kLens))
+    _set(args.q, q)
+    _set(args.k, k)
+    _set(args.v, v)
+    return args
+
+
+def _workspace(torch, args, backward, device):
+    size = C.c_size_t(0)
+    check(lib().illumina_op_attention_workspace(C.byref(args), backward, C.byref(size)))
+    if not size.value:
+        return None
+    workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = workspace.data_ptr(), size.value
+    return workspace
+
+
+def attention(q, k, v, scale=None, causalBlock=0, qLens=None, kLens=None, stream=None):
+    """softmax(scale q k') v: (out [batch, tokens, heads, headDim], lse float32 [batch, heads, tokens]).
+
+    q [batch, queries, heads, headDim]; k, v [batch, keys, keyHeads, headDim], heads a multiple of keyHeads, headDim at
+    most 128; scale defaults to headDim**-0.5. qLens, kLens (int32 [batch]): lengths of a padded batch; padding may
+    hold anything and its rows come back as zeros. causalBlock n: the last query stands at the last key, and a query
+    sees its own block of n keys and those before it (1: causal tokens; the tokens of a frame: causal frames). Rows
+    that see no key are zeros with lse -inf."""
+    import torch
+    args = _attention_args(torch, q, k, v, scale, causalBlock, qLens, kLens)
+    with _On(torch, q.device, stream) as on:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+        _set(args.out, out)
+        args.lse = lse.data_ptr()
+        workspace = _workspace(torch, args, 0, q.device)  # noqa: F841 - alive until the launch is queued
+        check(lib().illumina_op_attention(C.byref(args), on.handle))
+    return out, lse
+
+
+def attentionBackward(dOut, q, k, v, out, lse, scale=None, causalBlock=0, qLens=None, kLens=None, stream=None):
+    """Gradients (dq, dk, dv) of attention, from its results out and lse and the same masks."""
+    import torch
+    args = _attention_args(torch, q, k, v, scale, causalBlock, qLens, kLens)
+    for name, x in (("dOut", dOut), ("out", out)):
+        _tensor(torch, name, x, q, 4)
+        _require(x.shape == q.shape, f"{name} must have the shape of q")
+    _require(lse is not None, "lse of the forward pass is needed")
+    _vector(torch, "lse", lse, q.shape[0] * q.shape[2] * q.shape[1], q.device)
+    with _On(torch, q.device, stream) as on:
+        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+        args.lse = lse.data_ptr()
+        for slot, x in ((args.dout, dOut), (args.out, out), (args.dq, dq), (args.dk, dk), (args.dv, dv)):
+            _set(slot, x)
+        workspace = _workspace(torch, args, 1, q.device)  # noqa: F841 - alive until the launch is queued
+        check(lib().illumina_op_attention_backward(C.byref(args), on.handle))
+    return dq, dk, dv

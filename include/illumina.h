@@ -363,6 +363,162 @@ illumina_status illumina_op_bilateral(const float *low, int lh, int lw, int low_
                                       int guide_c, float range_sigma, float *dst, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Token operators: a transformer stage over the network's feature maps (a
+ * token is a pixel of a channels-last map) or over the frames of a clip,
+ * forward and backward. No counterpart in the reference.
+ *
+ * Storage is ILLUMINA_PRECISION_F32 or ILLUMINA_PRECISION_BF16; sums,
+ * statistics and softmax are held in 32 bits. All pointers are device pointers
+ * of the current device, strides are in elements, the last dimension is
+ * contiguous. The calls queue their kernels on `stream` and return; they
+ * allocate nothing and can be captured. A workspace belongs to the call until
+ * its kernels are done: calls that may overlap (two streams, two graphs) need
+ * one each. Outputs must not overlap inputs unless an entry point says so.
+ * ------------------------------------------------------------------------- */
+
+/* Layer norm over the last dimension: y = (x - mean) * rstd * w + b with
+ * rstd = 1 / sqrt(var + eps), of `rows` rows of c elements, `x_stride` apart.
+ * w, b ([c], nullable). mean, rstd ([rows], nullable) keep the statistics for
+ * the backward pass. y may be x. */
+illumina_status illumina_op_layer_norm(int precision, const void *x, long long x_stride, long long rows, int c,
+                                       const float *w, const float *b, float eps, void *y, long long y_stride,
+                                       float *mean, float *rstd, void *stream);
+
+/* Gradients of illumina_op_layer_norm: dx (nullable; may be dy), and dw and db
+ * ([c], nullable), the sums over all rows, written and not added to. The order
+ * of the sums is fixed: the same inputs give the same bits. `workspace` (16-byte
+ * aligned) holds illumina_op_layer_norm_workspace bytes; it may be NULL when
+ * neither dw nor db is wanted. */
+illumina_status illumina_op_layer_norm_backward(int precision, const void *dy, long long dy_stride, const void *x,
+                                                long long x_stride, long long rows, int c, const float *w,
+                                                const float *mean, const float *rstd, void *dx, long long dx_stride,
+                                                float *dw, float *db, void *workspace, size_t workspace_bytes,
+                                                void *stream);
+illumina_status illumina_op_layer_norm_workspace(long long rows, int c, size_t *bytes);
+
+/* One tensor of a rotation: [batch][tokens][heads][head_dim] read at `x`,
+ * written at `y` (y may be x), strides of batch, token and head. */
+typedef struct illumina_rotary_tensor {
+  const void *x;
+  void *y;
+  int heads;
+  long long x_stride[3], y_stride[3];
+} illumina_rotary_tensor;
+
+/* Rotary positions with several axes (time, row, column; any number): pair j
+ * belongs to axis `axis[j]` and turns by position * turns[j] whole turns
+ * (frequency / 2 pi). Pairs are elements (j, j + pairs), or neighbours
+ * (2j, 2j + 1) when `interleaved`; elements from 2 * pairs on are copied.
+ * `inverse` turns back: the gradient of the rotation. Queries and keys share
+ * the angles of one launch: second.heads may be 0. */
+typedef struct illumina_rotary_args {
+  int precision;
+  long long batch, tokens;
+  int head_dim, pairs, axes;
+  int interleaved, inverse;
+  illumina_rotary_tensor first, second;
+  const void *positions;           /* int32, or float32 when positions_float */
+  int positions_float;
+  long long position_stride[3];    /* axis, batch, token */
+  const double *turns;             /* [pairs] */
+  const int *axis;                 /* [pairs], 0 <= axis[j] < axes */
+} illumina_rotary_args;
+illumina_status illumina_op_rotary(const illumina_rotary_args *args, void *stream);
+
+/* A tensor of an attention call: [batch][tokens][heads][head_dim], strides of
+ * batch, token and head (0 is allowed for inputs that are broadcast). */
+typedef struct illumina_attention_tensor {
+  void *data;
+  long long stride[3];
+} illumina_attention_tensor;
+
+/* out = softmax(scale q k' masked) v for `heads` query heads, `heads / kv_heads`
+ * of which share a key head; head_dim at most 128.
+ * q_lens, k_lens ([batch] int32, nullable) are the lengths of a padded batch
+ * (clamped to the token counts): padding may hold anything, and the rows of
+ * padding in out, dq, dk and dv are written as zeros. causal_block 0: a query
+ * sees every key. causal_block n > 0: the last query stands at the last key, a
+ * query sees its own block of n keys and those before it (1: causal tokens; the
+ * tokens of a frame: causal frames). A row that sees no key gives zeros and lse
+ * -inf. Keys that only the causal mask hides must be finite.
+ * lse: [batch][heads][q_tokens] log of the softmax's sum, for the backward. */
+typedef struct illumina_attention_args {
+  int precision;
+  int batch, heads, kv_heads, head_dim;
+  int q_tokens, k_tokens;
+  int causal_block;
+  float scale;
+  illumina_attention_tensor q, k, v, out;
+  const int *q_lens, *k_lens;
+  float *lse;
+  /* backward: read dout, out and lse, write dq, dk, dv */
+  illumina_attention_tensor dout, dq, dk, dv;
+  void *workspace;                 /* 16-byte aligned */
+  size_t workspace_bytes;
+} illumina_attention_args;
+illumina_status illumina_op_attention_workspace(const illumina_attention_args *args, int backward, size_t *bytes);
+illumina_status illumina_op_attention(const illumina_attention_args *args, void *stream);
+/* Recomputes the probabilities from lse. Every sum has a fixed order, over the
+ * query heads that share a key head too: the same inputs give the same bits.
+ * ILLUMINA_TIMEOUT from either call: a tensor-core kernel of an earlier call
+ * gave up a bounded wait (that call's outputs are undefined). */
+illumina_status illumina_op_attention_backward(const illumina_attention_args *args, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * AdamW over many tensors (the weights of a model, illumina_weights_* order or
+ * any other). No counterpart in the reference.
+ *
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+ *   p = p (1 - lr decay) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+ *
+ * Parameters are float32. The caller owns the moments: flat arrays m and v in
+ * which every tensor begins at a multiple of ILLUMINA_ADAMW_BLOCK elements
+ * (illumina_adamw_blocks blocks in all), zeros before the first step. With 32
+ * bits they are float32. With 8 bits m holds int8 codes and v uint8 codes of
+ * the second moment's root, with one float32 scale a block in m_scale and
+ * v_scale: m = code * scale, v = (code * scale)^2; codes are rounded up where
+ * their fraction passes a threshold that sweeps [0, 1) evenly from step to
+ * step. A gradient that is not finite spoils its element, and with 8 bits its
+ * block.
+ * ------------------------------------------------------------------------- */
+
+#define ILLUMINA_ADAMW_BLOCK 256
+
+typedef struct illumina_adamw illumina_adamw;
+typedef struct illumina_adamw_options {
+  int device;
+  int tensors;
+  float *const *params;            /* [tensors] device pointers */
+  const long long *counts;         /* [tensors] elements, 0 allowed */
+  const int *decay;                /* [tensors] 1: weight decay applies; NULL: to all */
+  int moment_bits;                 /* 32 or 8 */
+  int grad_precision;              /* ILLUMINA_PRECISION_* of the gradients */
+  void *m, *v;                     /* device, 16-byte aligned */
+  float *m_scale, *v_scale;        /* device, 8 bits only */
+} illumina_adamw_options;
+typedef struct illumina_adamw_hyper {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float *lr_device;          /* nullable: a device scalar read in place of lr (a captured step's schedule) */
+} illumina_adamw_hyper;
+
+/* Blocks of the flat moments of tensors with these counts. */
+illumina_status illumina_adamw_blocks(const long long *counts, int tensors, long long *blocks);
+/* Uploads the tensor table; no step has been taken. The tensors and moments
+ * must outlive the optimiser. */
+illumina_status illumina_adamw_create(const illumina_adamw_options *opts, illumina_adamw **out);
+illumina_status illumina_adamw_destroy(illumina_adamw *opt);
+/* One step: grads is a host array of device pointers, one a tensor (ignored for
+ * empty tensors). The step count is kept on the device, so that a captured
+ * step counts on when it is replayed. Steps of one optimiser must not overlap. */
+illumina_status illumina_adamw_step(illumina_adamw *opt, const void *const *grads, const illumina_adamw_hyper *hyper,
+                                    void *stream);
+/* Reads or sets the steps taken, after the work queued on `stream`; both wait for it. */
+illumina_status illumina_adamw_get_steps(illumina_adamw *opt, long long *steps, void *stream);
+illumina_status illumina_adamw_set_steps(illumina_adamw *opt, long long steps, void *stream);
+/* The float32 values of 8-bit moments, [blocks * ILLUMINA_ADAMW_BLOCK] each. */
+illumina_status illumina_adamw_moments(illumina_adamw *opt, float *m, float *v, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Lighting (src/lighting/)
  * ------------------------------------------------------------------------- */
 
