@@ -15,6 +15,7 @@
 // and the order of every sum is fixed. Bound by the FP32 pipe.
 #include "attention.cuh"
 #include "kernels.h"
+#include <algorithm>
 #include "token_common.cuh"
 
 namespace illumina {
@@ -470,19 +471,34 @@ cudaError_t run_simt(const AttnParams &p, bool bwd, cudaStream_t st) {
 
 }  // namespace
 
+// By sizes alone, so that it does not depend on which path the tensors'
+// addresses and strides allow.
 size_t attention_workspace(int T, const AttnParams &p, bool backward) {
   const size_t rows = (size_t)p.batch * p.heads * p.q_tokens;
   if (backward) return rows * sizeof(float);
-  const int splits = p.head_dim <= 64 ? simt_splits<64>(p) : simt_splits<32>(p);
+  int splits = p.head_dim <= 64 ? simt_splits<64>(p) : simt_splits<32>(p);
+  if (T == BF16) splits = std::max(splits, attention_tc_splits(p));
   return splits == 1 ? 0 : splits * rows * (p.head_dim + 1) * sizeof(float);
 }
 
 cudaError_t attention(int T, const AttnParams &p, cudaStream_t st) {
-  return T == F32 ? run_simt<float>(p, false, st) : run_simt<bf16>(p, false, st);
+  if (T == F32) return run_simt<float>(p, false, st);
+  if (!attention_tc_takes(p, false)) return run_simt<bf16>(p, false, st);
+  const cudaError_t e = attention_tc(p, false, st);
+  const int splits = attention_tc_splits(p);
+  if (e != cudaSuccess || splits == 1) return e;
+  const long long rows = (long long)p.batch * p.heads * p.q_tokens;
+  k_attn_join<bf16><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, splits);
+  return cudaGetLastError();
 }
 
 cudaError_t attention_backward(int T, const AttnParams &p, cudaStream_t st) {
-  return T == F32 ? run_simt<float>(p, true, st) : run_simt<bf16>(p, true, st);
+  if (T == F32) return run_simt<float>(p, true, st);
+  if (!attention_tc_takes(p, true)) return run_simt<bf16>(p, true, st);
+  const long long rows = (long long)p.batch * p.heads * p.q_tokens;
+  k_attn_delta<bf16><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess ? e : attention_tc(p, true, st);
 }
 
 }  // namespace gpu

@@ -1,0 +1,1020 @@
+// Attention and its backward pass on the tensor cores, for bf16 storage.
+//
+//   S = scale Q K', masked; P = softmax(S); O = P V; lse = log sum exp S
+//   dV = P' dO; dP = dO V'; dS = P (dP - rowsum(dO O)); dQ = scale dS K; dK = scale dS' Q
+//
+// Every product is a tcgen05.mma of 128 rows with its accumulator in TMEM.
+// Operand tiles come by TMA into 128-byte swizzled images (128 rows x 64
+// columns; two for head sizes over 64, the columns past head_dim filled with
+// zeros by the copy) and serve both as K-major and, transposed by the matrix
+// descriptor, as MN-major operands. Probabilities and their gradients go from
+// registers to TMEM as bf16 and are the A operand of the following product
+// from there, so that they never pass through shared memory.
+//
+// A query tile holds the G query heads that share a key head for 128 / G
+// consecutive tokens (row r: token r / G, head r % G): key and value tiles are
+// read once for all of them, and a single token's heads fill one tile.
+//
+// Warps: two warpgroups compute (one TMEM lane, that is one row, a thread, so
+// a row's maximum and sum need no shuffles), one warp issues the copies, one
+// the products. All waits are on mbarriers and bounded.
+//
+// Rows of padding inside the last tile may hold NaN: where such rows are a
+// contraction index (V; K in dQ; Q and dO in dK, dV), 0 * NaN would spoil the
+// sum, so the product warp clears them in shared memory first.
+#include "attention.cuh"
+#include "kernels.h"
+#include "tc_common.cuh"
+#include "token_common.cuh"
+
+#include <cudaTypedefs.h>
+
+namespace illumina {
+namespace gpu {
+
+int sm_count();
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
+
+namespace {
+
+using namespace tcx;
+using tok::bf16;
+
+constexpr int kTcThreads = 384;
+constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr uint32_t kImage = 128 * 128;  // 128 rows x 64 bf16 columns
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct TcArgs {
+  int group, tpt;        // query heads a key head has; tokens of a query tile
+  int q_tiles, k_tiles;  // per (batch, key head)
+  int splits;
+  int n16;               // head_dim rounded up to the MMA's 16 columns
+  int qh, qb, kh, kb, vh, vb, gh, gb;  // 0: that dimension of the tensor is broadcast (stride 0)
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(a));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t *r) {
+  tmem_st16(a, r);
+  tmem_st16(a + 16, r + 16);
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Operand descriptors of an image: K-major (smem_desc, K = the 64 columns) and
+// MN-major: the 64 columns are the N index, 8-row groups of K are 1024 bytes
+// apart, the next 64 columns are in the next image.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(kImage >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+constexpr uint32_t kBMnMajor = 1u << 16;
+
+// d[128][n] (+)= a(image rows)[128][nk * 16] * b(image rows)[n][nk * 16]'
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, int nk, uint32_t idesc) {
+  for (int k = 0; k < nk; k++) {
+    const uint32_t o = (k >> 2) * kImage + (k & 3) * 32;
+    mma_f16(d, smem_desc(a + o), smem_desc(b + o), idesc, k > 0);
+  }
+}
+// d[128][n] (+)= a(TMEM, bf16 pairs)[128][128] * b(image)[128][n]; the second
+// half of a's columns begins `half` TMEM columns after the first.
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t half, uint32_t b, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const uint32_t at = a + (k >> 2) * half + (k & 3) * 8;
+    const uint32_t acc = first && k == 0 ? 0u : 1u;
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(at), "l"(desc_mn(b + k * 2048)), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&b);
+}
+
+// A wait that ends when another role of the CTA has given up, too.
+struct Waiter {
+  volatile int *fail;
+  __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity) const {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+      if (*fail || clock64() - t0 > kWaitCycles) {
+        *fail = 1;
+        return false;
+      }
+    }
+    return true;
+  }
+  // The same for a whole warp: all of its threads go on, or none.
+  __device__ __forceinline__ bool warp(uint64_t *bar, uint32_t parity) const {
+    return __all_sync(0xffffffffu, (*this)(bar, parity));
+  }
+};
+
+// Loads `boxes` 64-column images of a tile.
+__device__ __forceinline__ void load_images(uint32_t dst, const CUtensorMap *map, int boxes, int head, int token, int b,
+                                            uint64_t *bar) {
+  for (int i = 0; i < boxes; i++) tma_load_4d(dst + i * kImage, map, i * 64, head, token, b, bar);
+}
+
+// Clears rows [from, 128) of a tile's images; one warp.
+__device__ __forceinline__ void clear_rows(uint8_t *tile, int boxes, int from) {
+  const int lane = threadIdx.x & 31;
+  for (int i = 0; i < boxes; i++)
+    for (int o = from * 128 + lane * 16; o < (int)kImage; o += 512)
+      *reinterpret_cast<uint4 *>(tile + i * kImage + o) = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+  __syncwarp();
+}
+
+// Writes n (a multiple of 8, at most 32) values as bf16, times f.
+__device__ __forceinline__ void store_bf16(bf16 *dst, const uint32_t *r, int n, float f) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 8)
+    if (c < n) {
+      uint4 u;
+      u.x = pack2(__uint_as_float(r[c]) * f, __uint_as_float(r[c + 1]) * f);
+      u.y = pack2(__uint_as_float(r[c + 2]) * f, __uint_as_float(r[c + 3]) * f);
+      u.z = pack2(__uint_as_float(r[c + 4]) * f, __uint_as_float(r[c + 5]) * f);
+      u.w = pack2(__uint_as_float(r[c + 6]) * f, __uint_as_float(r[c + 7]) * f);
+      *reinterpret_cast<uint4 *>(dst + c) = u;
+    }
+}
+__device__ __forceinline__ void store_zeros(bf16 *dst, int n) {
+  for (int c = 0; c < n; c += 8) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0, 0, 0, 0);
+}
+
+// The end of every kernel: copies and products of a CTA that gave up are
+// drained, then TMEM is freed.
+__device__ __forceinline__ void leave(uint32_t tmem, int warp, volatile int *fail, uint64_t *drain, int *err) {
+  if (warp == kMmaWarp && (threadIdx.x & 31) == 0) {
+    mma_commit(drain);
+    mbar_wait(drain, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *fail) report_gave_up(err);
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+__device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
+  return p + ((1024u - (smem_u32(p) & 1023u)) & 1023u);
+}
+
+// ---------------------------------------------------------------------------
+// Forward: two query tiles past one stream of key and value tiles. The two
+// warpgroups alternate on the tensor cores: while one turns its S into P, the
+// other's products run. The output accumulator is rescaled only when a row's
+// maximum has grown by more than 2^8 since the exponent's base was chosen
+// (the probabilities stay exact in relation to the sum).
+// ---------------------------------------------------------------------------
+
+template <int DP>
+struct FwdSmem {
+  static constexpr int kBoxes = DP / 64, kStages = DP == 64 ? 3 : 2;
+  static constexpr uint32_t kTile = kBoxes * kImage;
+  static constexpr size_t kBytes = 1024 + (2 + 2 * kStages) * kTile + 256;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_attn_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+              const __grid_constant__ CUtensorMap mv, const AttnParams p, const TcArgs a) {
+  using L = FwdSmem<DP>;
+  extern __shared__ uint8_t raw[];
+  uint8_t *base = align1024(raw);
+  uint8_t *sq = base, *sk = sq + 2 * L::kTile, *sv = sk + L::kStages * L::kTile;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile);
+  uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 4, *o_full = bars + 6, *drain = bars + 8,
+           *k_full = bars + 9, *k_empty = k_full + L::kStages, *v_full = k_empty + L::kStages,
+           *v_empty = v_full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 9 + 4 * L::kStages);
+  volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
+  const int warp = threadIdx.x >> 5;
+
+  long long id = blockIdx.x;
+  const int pairs = (a.q_tiles + 1) / 2;
+  const int split = (int)(id % a.splits);
+  id /= a.splits;
+  const int pair = pairs - 1 - (int)(id % pairs);  // the longest causal rows first
+  id /= pairs;
+  const int hk = (int)(id % p.kv_heads), n = (int)(id / p.kv_heads);
+  const AttnMask mask(p, n);
+  // key tiles [t0, t1[i]) of query tile i
+  int t0, t1[2], most = 0;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int first = (2 * pair + i) * a.tpt;
+    const int end = 2 * pair + i < a.q_tiles && first < mask.q_len
+                        ? mask.key_end(min(first + a.tpt, mask.q_len) - 1)
+                        : 0;
+    t1[i] = (end + 127) / 128;
+    most = max(most, t1[i]);
+  }
+  const int per = (most + a.splits - 1) / a.splits;
+  t0 = split * per;
+#pragma unroll
+  for (int i = 0; i < 2; i++) t1[i] = min(t1[i], t0 + per);
+  most = max(t1[0], t1[1]);
+
+  if (threadIdx.x == 0) {
+    *fail = 0;
+    for (int i = 0; i < 2; i++) mbar_init(q_full + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1);
+    mbar_init(drain, 1);
+    for (int i = 0; i < L::kStages; i++)
+      mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(tmem_ptr, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  const Waiter wait{fail};
+
+  if (warp >= kProducerWarp) {
+    reg_dealloc<88>();
+    if (warp == kProducerWarp && (threadIdx.x & 31) == 0 && t0 < most) {
+      int queries = 0;
+      for (int i = 0; i < 2; i++)
+        if (t0 < t1[i]) {
+          mbar_expect_tx(q_full + i, L::kBoxes * a.group * a.tpt * 128);
+          load_images(smem_u32(sq + i * L::kTile), &mq, L::kBoxes, a.qh * hk * a.group, (2 * pair + i) * a.tpt, a.qb * n,
+                      q_full + i);
+          queries |= 1 << i;
+        }
+      int issued_k = 0, issued_v = 0;
+      for (int j = t0; j < most; j++) {
+        const int s = (j - t0) % L::kStages, use = (j - t0) / L::kStages;
+        if (use > 0 && !wait(k_empty + s, (use - 1) & 1)) break;
+        mbar_expect_tx(k_full + s, L::kTile);
+        load_images(smem_u32(sk + s * L::kTile), &mk, L::kBoxes, a.kh * hk, j * 128, a.kb * n, k_full + s);
+        issued_k++;
+        if (use > 0 && !wait(v_empty + s, (use - 1) & 1)) break;
+        mbar_expect_tx(v_full + s, L::kTile);
+        load_images(smem_u32(sv + s * L::kTile), &mv, L::kBoxes, a.vh * hk, j * 128, a.vb * n, v_full + s);
+        issued_v++;
+      }
+      // every copy has landed before the CTA leaves
+      for (int i = 0; i < 2; i++)
+        if (queries >> i & 1) mbar_wait(q_full + i, 0);
+      for (int i = max(0, issued_k - L::kStages); i < issued_k; i++) mbar_wait(k_full + i % L::kStages, (i / L::kStages) & 1);
+      for (int i = max(0, issued_v - L::kStages); i < issued_v; i++) mbar_wait(v_full + i % L::kStages, (i / L::kStages) & 1);
+    } else if (warp == kMmaWarp && t0 < most) {
+      const bool lead = (threadIdx.x & 31) == 0;
+      const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
+      const int nk = a.n16 / 16;
+      bool ok = true;
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (ok && t0 < t1[i]) ok = wait.warp(q_full + i, 0);
+      ok = ok && wait.warp(k_full, 0);
+      tc_fence_after();
+      if (ok && lead) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          if (t0 < t1[i]) {
+            mma_rows(tmem + i * 128, smem_u32(sq + i * L::kTile), smem_u32(sk), nk, id_s);
+            mma_commit(s_full + i);
+          }
+        mma_commit(k_empty);
+      }
+      for (int j = t0; j < most && ok; j++) {
+        const int it = j - t0, s = it % L::kStages, s1 = (it + 1) % L::kStages;
+        ok = wait.warp(v_full + s, (it / L::kStages) & 1);
+        if (!ok) break;
+        if ((j + 1) * 128 > mask.k_len) clear_rows(sv + s * L::kTile, L::kBoxes, mask.k_len - j * 128);
+        const bool more = j + 1 < most;
+        bool have_k = false;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          if (j >= t1[i] || !ok) continue;
+          ok = wait.warp(p_full + i, it & 1);
+          if (!ok) continue;
+          tc_fence_after();
+          if (lead) {
+            mma_tmem(tmem + 256 + i * DP, tmem + i * 128, 32, smem_u32(sv + s * L::kTile), id_o, j == t0);
+            mma_commit(o_full + i);
+          }
+          if (j + 1 < t1[i]) {
+            if (!have_k) ok = wait.warp(k_full + s1, ((it + 1) / L::kStages) & 1);
+            if (!ok) continue;
+            have_k = true;
+            if (lead) {
+              mma_rows(tmem + i * 128, smem_u32(sq + i * L::kTile), smem_u32(sk + s1 * L::kTile), nk, id_s);
+              mma_commit(s_full + i);
+            }
+          }
+        }
+        if (!ok) break;
+        if (lead) {
+          mma_commit(v_empty + s);
+          if (more) mma_commit(k_empty + s1);
+        }
+        __syncwarp();
+      }
+    }
+    __syncwarp();
+  } else {
+    reg_alloc<208>();
+    const int i = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // 32 TMEM lanes a warp
+    const uint32_t ts = tmem + lane_base + i * 128, to = tmem + lane_base + 256 + i * DP;
+    const int tile = 2 * pair + i;
+    const int token = tile * a.tpt + row / a.group, h = hk * a.group + row % a.group;
+    const bool mine = tile < a.q_tiles && row < a.group * a.tpt && token < p.q_tokens;
+    const int end = mine ? mask.key_end(token) : 0;
+    const float sl2 = p.scale * kLog2e;
+    float top = -INFINITY, sum = 0;  // the exponent's base (scaled logits, base 2)
+    bool ok = true;
+    for (int j = t0; j < t1[i]; j++) {
+      const int it = j - t0;
+      ok = wait.warp(s_full + i, it & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t r[128];
+#pragma unroll
+      for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, r + 32 * c);
+      tmem_wait_ld();
+      const int left = end - j * 128;
+      if (__any_sync(0xffffffffu, left < 128)) {
+#pragma unroll
+        for (int c = 0; c < 128; c++)
+          if (c >= left) r[c] = 0xff800000u;
+      }
+      float m4[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) m4[c] = __uint_as_float(r[c]);
+#pragma unroll
+      for (int c = 4; c < 128; c++) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(r[c]));
+      const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
+      bool grow = false;
+      float f = 1.0f;
+      if (top == -INFINITY) {
+        top = m;  // nothing summed yet
+      } else if (m > top + 8.0f) {
+        f = ex2(top - m);
+        top = m;
+        sum *= f;
+        grow = true;
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+        ok = wait.warp(o_full + i, (it - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(to + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          tmem_st32(to + c, o);
+        }
+      }
+      const float shift = top == -INFINITY ? 0.0f : -top;
+      float s4[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t q[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const float x = ex2(fmaf(__uint_as_float(r[c + k]), sl2, shift));
+          const float y = ex2(fmaf(__uint_as_float(r[c + k + 1]), sl2, shift));
+          s4[k & 2] += x;
+          s4[(k & 2) + 1] += y;
+          q[k / 2] = pack2(x, y);
+        }
+        tmem_st16(ts + c / 2, q);
+      }
+      sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(p_full + i);
+    }
+    // output
+    const long long rows = (long long)p.batch * p.heads * p.q_tokens;
+    const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
+    const float f = sum > 0 ? 1.0f / sum : (sum == 0 ? 0.0f : NAN);
+    const float lse = sum == 0 ? -INFINITY : (top + log2f(sum)) * kLn2;
+    const bool some = ok && t0 < t1[i];
+    if (some) ok = wait.warp(o_full + i, (t1[i] - 1 - t0) & 1);
+    tc_fence_after();
+    const bool have = some && ok && end > 0;
+    if (a.splits == 1) {
+      bf16 *dst = (bf16 *)p.out.p + n * p.out.s[0] + token * p.out.s[1] + h * p.out.s[2];
+      if (some && ok) {
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(to + c, o);
+          tmem_wait_ld();
+          if (mine && have) store_bf16(dst + c, o, p.head_dim - c, f);
+        }
+      }
+      if (mine && !have) store_zeros(dst, p.head_dim);
+      if (mine) p.lse[at] = lse;
+    } else if (mine || some) {
+      float *dst = p.ws + (split * rows + at) * p.head_dim;
+      if (some && ok) {
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(to + c, o);
+          tmem_wait_ld();
+          if (mine && have)
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              if (c + k < p.head_dim)
+                *reinterpret_cast<float4 *>(dst + c + k) =
+                    make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f, __uint_as_float(o[k + 2]) * f,
+                                __uint_as_float(o[k + 3]) * f);
+        }
+      }
+      // a share without keys has lse -inf: its output is not read
+      if (mine) p.ws[a.splits * rows * p.head_dim + split * rows + at] = lse;
+    }
+  }
+  leave(tmem, warp, fail, drain, p.err);
+}
+
+// ---------------------------------------------------------------------------
+// Backward, dK and dV: one key tile (its rows are the TMEM lanes) past the
+// query tiles that see it. Per query tile: S' = K Q', dP' = V dO', and from
+// TMEM dV += P' dO, dK += dS' Q. The products of one tile run while the other
+// phase's arithmetic does: dP' under the exponentials, dV and the next S'
+// under dS, dK under the next exponentials. The two warpgroups take 64 query
+// columns each.
+// ---------------------------------------------------------------------------
+
+template <int DP>
+struct BwdSmem {
+  static constexpr int kBoxes = DP / 64, kStages = DP == 64 ? 3 : 2;
+  static constexpr uint32_t kTile = kBoxes * kImage;
+  static constexpr uint32_t kRowSums = 8 * 128 * 4;  // a warp's copy of 64 lse and 64 delta
+  static constexpr size_t kBytes = 1024 + (2 + 2 * kStages) * kTile + kRowSums + 256;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_attn_dkv_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                  const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg, const AttnParams p,
+                  const TcArgs a) {
+  using L = BwdSmem<DP>;
+  extern __shared__ uint8_t raw[];
+  uint8_t *base = align1024(raw);
+  uint8_t *sk = base, *sv = sk + L::kTile, *sq = sv + L::kTile, *sg = sq + L::kStages * L::kTile;
+  float *row_sums = reinterpret_cast<float *>(sg + L::kStages * L::kTile);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sg + L::kStages * L::kTile + L::kRowSums);
+  uint64_t *kv_full = bars, *s_full = bars + 1, *g_full = bars + 2, *p_full = bars + 3, *d_full = bars + 4,
+           *done = bars + 5, *drain = bars + 6, *full = bars + 7, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 7 + 2 * L::kStages);
+  volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
+  const int warp = threadIdx.x >> 5;
+
+  long long id = blockIdx.x;
+  const int kt = (int)(id % a.k_tiles);  // the keys that most queries see first
+  id /= a.k_tiles;
+  const int hk = (int)(id % p.kv_heads), n = (int)(id / p.kv_heads);
+  const AttnMask mask(p, n);
+  const int key0 = kt * 128;
+  const int t0 = key0 < mask.k_len ? mask.row_begin(key0) / a.tpt : 0;
+  const int t1 = key0 < mask.k_len ? (mask.q_len + a.tpt - 1) / a.tpt : 0;
+  const bool some = t0 < t1;
+
+  if (threadIdx.x == 0) {
+    *fail = 0;
+    for (uint64_t *b = bars; b < bars + 7; b++) mbar_init(b, b == p_full || b == d_full ? 8 : 1);
+    for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    fence_barrier_init();
+  }
+  // rows of the query images past group * tpt are never written by the copies
+  if (a.group * a.tpt < 128)
+    for (int t = warp; t < 2 * L::kStages; t += kTcThreads / 32) clear_rows(sq + t * L::kTile, L::kBoxes, a.group * a.tpt);
+  if (warp == kMmaWarp) tmem_alloc(tmem_ptr, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  const uint32_t t_s = tmem, t_g = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
+  const Waiter wait{fail};
+
+  if (warp == kProducerWarp && (threadIdx.x & 31) == 0 && some) {
+    mbar_expect_tx(kv_full, 2 * L::kTile);
+    load_images(smem_u32(sk), &mk, L::kBoxes, a.kh * hk, key0, a.kb * n, kv_full);
+    load_images(smem_u32(sv), &mv, L::kBoxes, a.vh * hk, key0, a.vb * n, kv_full);
+    int issued = 0;
+    for (int j = t0; j < t1; j++) {
+      const int s = (j - t0) % L::kStages, use = (j - t0) / L::kStages;
+      if (use > 0 && !wait(empty + s, (use - 1) & 1)) break;
+      mbar_expect_tx(full + s, 2 * L::kBoxes * a.group * a.tpt * 128);
+      load_images(smem_u32(sq + s * L::kTile), &mq, L::kBoxes, a.qh * hk * a.group, j * a.tpt, a.qb * n, full + s);
+      load_images(smem_u32(sg + s * L::kTile), &mg, L::kBoxes, a.gh * hk * a.group, j * a.tpt, a.gb * n, full + s);
+      issued++;
+    }
+    mbar_wait(kv_full, 0);
+    for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
+  } else if (warp == kMmaWarp && some) {
+    const bool lead = (threadIdx.x & 31) == 0;
+    const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
+    const int nk = a.n16 / 16;
+    // query tile j is in shared memory, its padding cleared
+    auto ready = [&](int j) {
+      const int it = j - t0, s = it % L::kStages;
+      if (!wait.warp(full + s, (it / L::kStages) & 1)) return false;
+      const int from = (mask.q_len - j * a.tpt) * a.group;
+      if (from < a.group * a.tpt) {
+        clear_rows(sq + s * L::kTile, L::kBoxes, from);
+        clear_rows(sg + s * L::kTile, L::kBoxes, from);
+      }
+      tc_fence_after();
+      return true;
+    };
+    bool ok = wait.warp(kv_full, 0) && ready(t0);
+    if (ok && lead) {
+      mma_rows(t_s, smem_u32(sk), smem_u32(sq), nk, id_s);
+      mma_commit(s_full);
+      mma_rows(t_g, smem_u32(sv), smem_u32(sg), nk, id_s);
+      mma_commit(g_full);
+    }
+    __syncwarp();
+    for (int j = t0; j < t1 && ok; j++) {
+      const int it = j - t0, s = it % L::kStages, s1 = (it + 1) % L::kStages;
+      const bool more = j + 1 < t1;
+      ok = wait.warp(p_full, it & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (lead) mma_tmem(t_dv, t_s, 64, smem_u32(sg + s * L::kTile), id_o, it == 0);
+      __syncwarp();
+      if (more) {
+        ok = ready(j + 1);
+        if (!ok) break;
+        if (lead) {
+          mma_rows(t_s, smem_u32(sk), smem_u32(sq + s1 * L::kTile), nk, id_s);
+          mma_commit(s_full);
+        }
+        __syncwarp();
+      }
+      ok = wait.warp(d_full, it & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (lead) {
+        mma_tmem(t_dk, t_g, 64, smem_u32(sq + s * L::kTile), id_o, it == 0);
+        mma_commit(empty + s);
+        if (more) {
+          mma_rows(t_g, smem_u32(sv), smem_u32(sg + s1 * L::kTile), nk, id_s);
+          mma_commit(g_full);
+        } else {
+          mma_commit(done);
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp < kProducerWarp) {
+    const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
+    const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
+    const uint32_t ts = t_s + lane_base + wg * 64, tg = t_g + lane_base + wg * 64;
+    const int key = key0 + row;
+    const int begin = key < mask.k_len ? mask.row_begin(key) : INT_MAX / 2;
+    const float sl2 = p.scale * kLog2e;
+    float *mine_lse = row_sums + warp * 128, *mine_delta = mine_lse + 64;
+    // lse (base 2; +inf where the row has no probabilities) and delta of the
+    // two columns this lane fetches of query tile j
+    float nl[2], nd[2];
+    auto fetch = [&](int j) {
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int r = wg * 64 + k * 32 + lane;
+        const int token = j * a.tpt + r / a.group, h = hk * a.group + r % a.group;
+        nl[k] = INFINITY, nd[k] = 0;
+        if (r < a.group * a.tpt && token < mask.q_len) {
+          const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
+          const float v = p.lse[at];
+          nl[k] = v == -INFINITY ? INFINITY : v * kLog2e;
+          nd[k] = p.ws[at];
+        }
+      }
+    };
+    bool ok = true;
+    if (some) fetch(t0);
+    for (int j = t0; j < t1; j++) {
+      const int it = j - t0;
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 2; k++) mine_lse[k * 32 + lane] = nl[k], mine_delta[k * 32 + lane] = nd[k];
+      __syncwarp();
+      if (j + 1 < t1) fetch(j + 1);
+      // columns below `skip` are queries that do not see this key
+      const long long skip_ll = ((long long)begin - (long long)j * a.tpt) * a.group - wg * 64;
+      const int skip = (int)min(max(skip_ll, 0ll), 64ll);
+      const bool masked = __any_sync(0xffffffffu, skip > 0);
+      ok = wait.warp(s_full, it & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t r[64];
+      tmem_ld32(ts, r);
+      tmem_ld32(ts + 32, r + 32);
+      tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 l = *reinterpret_cast<const float4 *>(mine_lse + c);
+        r[c] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c]), sl2, -l.x)));
+        r[c + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c + 1]), sl2, -l.y)));
+        r[c + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c + 2]), sl2, -l.z)));
+        r[c + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c + 3]), sl2, -l.w)));
+      }
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 64; c++)
+          if (c < skip) r[c] = 0;
+      }
+      uint32_t q[32];
+#pragma unroll
+      for (int c = 0; c < 32; c++) q[c] = pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      tmem_st32(ts, q);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+      ok = wait.warp(g_full, it & 1);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        uint32_t g[32];
+        tmem_ld32(tg + 32 * half, g);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 d = *reinterpret_cast<const float4 *>(mine_delta + 32 * half + c);
+          const float *pr = reinterpret_cast<const float *>(r) + 32 * half + c;
+          float v[4] = {pr[0] * (__uint_as_float(g[c]) - d.x), pr[1] * (__uint_as_float(g[c + 1]) - d.y),
+                        pr[2] * (__uint_as_float(g[c + 2]) - d.z), pr[3] * (__uint_as_float(g[c + 3]) - d.w)};
+          if (masked) {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              if (32 * half + c + k < skip) v[k] = 0;
+          }
+          q[16 * half + c / 2] = pack2(v[0], v[1]);
+          q[16 * half + c / 2 + 1] = pack2(v[2], v[3]);
+        }
+      }
+      tmem_st32(tg, q);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(d_full);
+    }
+    if (some && ok) ok = wait.warp(done, 0);
+    tc_fence_after();
+    const bool inside = key < p.k_tokens, have = some && ok && key < mask.k_len;
+    // warpgroup 0 writes dV, warpgroup 1 dK
+    const AttnTensor &t = wg ? p.dk : p.dv;
+    bf16 *dst = (bf16 *)t.p + n * t.s[0] + (long long)key * t.s[1] + hk * t.s[2];
+    if (some && ok) {
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        tmem_ld32((wg ? t_dk : t_dv) + lane_base + c, o);
+        tmem_wait_ld();
+        if (inside && have) store_bf16(dst + c, o, p.head_dim - c, wg ? p.scale : 1.0f);
+      }
+    }
+    if (inside && !have) store_zeros(dst, p.head_dim);
+  }
+  leave(tmem, warp, fail, drain, p.err);
+}
+
+// ---------------------------------------------------------------------------
+// Backward, dQ: one query tile past the key tiles it sees. S = Q K' and
+// dP = dO V' are recomputed, dQ += dS K from TMEM. The warpgroups take 64 key
+// columns each; a thread's lse and delta stay in registers.
+// ---------------------------------------------------------------------------
+
+template <int DP>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_attn_dq_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg, const AttnParams p,
+                 const TcArgs a) {
+  using L = BwdSmem<DP>;
+  extern __shared__ uint8_t raw[];
+  uint8_t *base = align1024(raw);
+  uint8_t *sq = base, *sg = sq + L::kTile, *sk = sg + L::kTile, *sv = sk + L::kStages * L::kTile;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile);
+  uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 2, *s_free = bars + 3, *d_full = bars + 4,
+           *done = bars + 5, *drain = bars + 6, *full = bars + 7, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 7 + 2 * L::kStages);
+  volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
+  const int warp = threadIdx.x >> 5;
+
+  long long id = blockIdx.x;
+  const int qt = a.q_tiles - 1 - (int)(id % a.q_tiles);  // the longest causal rows first
+  id /= a.q_tiles;
+  const int hk = (int)(id % p.kv_heads), n = (int)(id / p.kv_heads);
+  const AttnMask mask(p, n);
+  const int first = qt * a.tpt;
+  const int t1 = first < mask.q_len ? (mask.key_end(min(first + a.tpt, mask.q_len) - 1) + 127) / 128 : 0;
+
+  if (threadIdx.x == 0) {
+    *fail = 0;
+    for (uint64_t *b = bars; b < bars + 7; b++) mbar_init(b, b == s_free || b == d_full ? 8 : 1);
+    for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(tmem_ptr, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  const uint32_t t_s = tmem, t_g = tmem + 128, t_dq = tmem + 256;
+  const Waiter wait{fail};
+
+  if (warp == kProducerWarp && (threadIdx.x & 31) == 0 && t1 > 0) {
+    mbar_expect_tx(q_full, 2 * L::kBoxes * a.group * a.tpt * 128);
+    load_images(smem_u32(sq), &mq, L::kBoxes, a.qh * hk * a.group, first, a.qb * n, q_full);
+    load_images(smem_u32(sg), &mg, L::kBoxes, a.gh * hk * a.group, first, a.gb * n, q_full);
+    int issued = 0;
+    for (int j = 0; j < t1; j++) {
+      const int s = j % L::kStages, use = j / L::kStages;
+      if (use > 0 && !wait(empty + s, (use - 1) & 1)) break;
+      mbar_expect_tx(full + s, 2 * L::kTile);
+      load_images(smem_u32(sk + s * L::kTile), &mk, L::kBoxes, a.kh * hk, j * 128, a.kb * n, full + s);
+      load_images(smem_u32(sv + s * L::kTile), &mv, L::kBoxes, a.vh * hk, j * 128, a.vb * n, full + s);
+      issued++;
+    }
+    mbar_wait(q_full, 0);
+    for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
+  } else if (warp == kMmaWarp && t1 > 0) {
+    const bool lead = (threadIdx.x & 31) == 0;
+    const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
+    const int nk = a.n16 / 16;
+    auto ready = [&](int j) {
+      const int s = j % L::kStages;
+      if (!wait.warp(full + s, (j / L::kStages) & 1)) return false;
+      if ((j + 1) * 128 > mask.k_len) clear_rows(sk + s * L::kTile, L::kBoxes, mask.k_len - j * 128);
+      tc_fence_after();
+      return true;
+    };
+    bool ok = wait.warp(q_full, 0) && ready(0);
+    if (ok && lead) {
+      mma_rows(t_s, smem_u32(sq), smem_u32(sk), nk, id_s);
+      mma_commit(s_full);
+      mma_rows(t_g, smem_u32(sg), smem_u32(sv), nk, id_s);
+      mma_commit(g_full);
+    }
+    __syncwarp();
+    for (int j = 0; j < t1 && ok; j++) {
+      const int s = j % L::kStages, s1 = (j + 1) % L::kStages;
+      const bool more = j + 1 < t1;
+      if (more) {
+        ok = wait.warp(s_free, j & 1) && ready(j + 1);
+        if (!ok) break;
+        if (lead) {
+          mma_rows(t_s, smem_u32(sq), smem_u32(sk + s1 * L::kTile), nk, id_s);
+          mma_commit(s_full);
+        }
+        __syncwarp();
+      }
+      ok = wait.warp(d_full, j & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (lead) {
+        mma_tmem(t_dq, t_g, 64, smem_u32(sk + s * L::kTile), id_o, j == 0);
+        mma_commit(empty + s);
+        if (more) {
+          mma_rows(t_g, smem_u32(sg), smem_u32(sv + s1 * L::kTile), nk, id_s);
+          mma_commit(g_full);
+        } else {
+          mma_commit(done);
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp < kProducerWarp) {
+    const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
+    const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
+    const uint32_t ts = t_s + lane_base + wg * 64, tg = t_g + lane_base + wg * 64;
+    const int token = first + row / a.group, h = hk * a.group + row % a.group;
+    const bool mine = row < a.group * a.tpt && token < p.q_tokens;
+    const int end = mine ? mask.key_end(token) : 0;
+    const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
+    const float v = end ? p.lse[at] : -INFINITY;
+    const float lse = v == -INFINITY ? INFINITY : v * kLog2e, delta = end ? p.ws[at] : 0.0f;
+    const float sl2 = p.scale * kLog2e;
+    bool ok = true;
+    for (int j = 0; j < t1; j++) {
+      const int left = end - j * 128 - wg * 64;
+      const bool masked = __any_sync(0xffffffffu, left < 64);
+      ok = wait.warp(s_full, j & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t r[64];
+      tmem_ld32(ts, r);
+      tmem_ld32(ts + 32, r + 32);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free);
+#pragma unroll
+      for (int c = 0; c < 64; c++) r[c] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c]), sl2, -lse)));
+      ok = wait.warp(g_full, j & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t q[32];
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        uint32_t g[32];
+        tmem_ld32(tg + 32 * half, g);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float x = __uint_as_float(r[32 * half + c]) * (__uint_as_float(g[c]) - delta);
+          float y = __uint_as_float(r[32 * half + c + 1]) * (__uint_as_float(g[c + 1]) - delta);
+          if (masked) {
+            if (32 * half + c >= left) x = 0;
+            if (32 * half + c + 1 >= left) y = 0;
+          }
+          q[16 * half + c / 2] = pack2(x, y);
+        }
+      }
+      tmem_st32(tg, q);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(d_full);
+    }
+    if (t1 > 0 && ok) ok = wait.warp(done, 0);
+    tc_fence_after();
+    const bool have = t1 > 0 && ok && end > 0;
+    bf16 *dst = (bf16 *)p.dq.p + n * p.dq.s[0] + token * p.dq.s[1] + h * p.dq.s[2];
+    // a warpgroup writes half of the columns
+    constexpr int kHalf = DP / 2;
+    if (t1 > 0 && ok) {
+#pragma unroll
+      for (int c = 0; c < kHalf; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(t_dq + lane_base + wg * kHalf + c, o);
+        tmem_wait_ld();
+        if (mine && have) store_bf16(dst + wg * kHalf + c, o, p.head_dim - wg * kHalf - c, p.scale);
+      }
+    }
+    if (mine && !have && wg == 0) store_zeros(dst, p.head_dim);
+  }
+  leave(tmem, warp, fail, drain, p.err);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+bool tma_tensor(const AttnTensor &t, int tokens, int heads, int batch) {
+  if (reinterpret_cast<uintptr_t>(t.p) & 15) return false;
+  const int extent[3] = {batch, tokens, heads};
+  for (int i = 0; i < 3; i++) {
+    if (extent[i] == 1) continue;
+    if (t.s[i] % 8 || t.s[i] < 0 || t.s[i] >= (1ll << 38) || (t.s[i] == 0 && i == 1)) return false;
+  }
+  return true;
+}
+bool wide_rows(const AttnTensor &t) {
+  return (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && t.s[0] % 8 == 0 && t.s[1] % 8 == 0 && t.s[2] % 8 == 0;
+}
+
+// [batch][tokens][heads][d] as a 4-D map (d, head, token, batch) with boxes of
+// 64 columns x `heads_box` heads x `rows_box` tokens. A broadcast dimension has
+// extent 1.
+bool encode(CUtensorMap *m, const AttnTensor &t, int d, int heads, int tokens, int batch, int heads_box, int rows_box,
+            bool &has_heads, bool &has_batch) {
+  has_heads = t.s[2] != 0 || heads == 1;
+  has_batch = t.s[0] != 0 || batch == 1;
+  if (!has_heads && heads_box > 1) return false;
+  cuuint64_t dim[4] = {(cuuint64_t)d, (cuuint64_t)(has_heads ? heads : 1), (cuuint64_t)tokens, (cuuint64_t)(has_batch ? batch : 1)};
+  // strides of dimensions of extent 1 are never used: any valid one will do
+  cuuint64_t stride[3] = {(cuuint64_t)t.s[2] * 2, (cuuint64_t)t.s[1] * 2, (cuuint64_t)t.s[0] * 2};
+  for (int i = 0; i < 3; i++)
+    if (dim[i + 1] == 1) stride[i] = (cuuint64_t)((d * 2 + 15) / 16 * 16);
+  cuuint32_t box[4] = {64, (cuuint32_t)heads_box, (cuuint32_t)rows_box, 1}, step[4] = {1, 1, 1, 1};
+  auto fn = tensor_map_encoder();
+  return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(t.p), dim, stride, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+TcArgs shape_of(const AttnParams &p) {
+  TcArgs a{};
+  a.group = p.heads / p.kv_heads;
+  a.tpt = 128 / a.group;
+  a.q_tiles = (p.q_tokens + a.tpt - 1) / a.tpt;
+  a.k_tiles = (p.k_tokens + 127) / 128;
+  a.n16 = (p.head_dim + 15) / 16 * 16;
+  a.splits = 1;
+  return a;
+}
+
+// Shares of the keys in the forward: enough for a CTA on every SM, while a
+// share keeps at least two key tiles.
+int tc_splits(const AttnParams &p, const TcArgs &a) {
+  const long long ctas = (long long)p.batch * p.kv_heads * ((a.q_tiles + 1) / 2);
+  const int sms = 148, most = a.k_tiles / 2;
+  if (ctas == 0 || ctas * 2 > sms || most < 2) return 1;
+  const int want = (int)(sms / ctas);
+  return want < most ? want : most;
+}
+
+cudaError_t big(const void *f, size_t bytes) {
+  return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <int DP>
+cudaError_t forward_tc(const AttnParams &p, const TcArgs &a, const CUtensorMap &mq, const CUtensorMap &mk,
+                       const CUtensorMap &mv, cudaStream_t st) {
+  constexpr size_t sm = FwdSmem<DP>::kBytes;
+  const cudaError_t e = big((const void *)k_attn_tc<DP>, sm);
+  if (e != cudaSuccess) return e;
+  const long long grid = (long long)p.batch * p.kv_heads * ((a.q_tiles + 1) / 2) * a.splits;
+  k_attn_tc<DP><<<(unsigned)grid, kTcThreads, sm, st>>>(mq, mk, mv, p, a);
+  return cudaGetLastError();
+}
+
+template <int DP>
+cudaError_t backward_tc(const AttnParams &p, const TcArgs &a, const CUtensorMap &mq, const CUtensorMap &mk,
+                        const CUtensorMap &mv, const CUtensorMap &mg, cudaStream_t st) {
+  constexpr size_t sm = BwdSmem<DP>::kBytes;
+  cudaError_t e = big((const void *)k_attn_dq_tc<DP>, sm);
+  if (e == cudaSuccess) e = big((const void *)k_attn_dkv_tc<DP>, sm);
+  if (e != cudaSuccess) return e;
+  const long long heads = (long long)p.batch * p.kv_heads;
+  k_attn_dkv_tc<DP><<<(unsigned)(heads * a.k_tiles), kTcThreads, sm, st>>>(mq, mk, mv, mg, p, a);
+  k_attn_dq_tc<DP><<<(unsigned)(heads * a.q_tiles), kTcThreads, sm, st>>>(mq, mk, mv, mg, p, a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+bool attention_tc_takes(const AttnParams &p, bool backward) {
+  if (p.head_dim % 8 || !(p.scale > 0) || p.scale > 1e30f) return false;
+  if (!p.batch || !p.heads || !p.q_tokens || !p.k_tokens || p.heads / p.kv_heads > 128) return false;
+  const bool grouped = p.heads > p.kv_heads;
+  if (!tma_tensor(p.q, p.q_tokens, p.heads, p.batch) || !tma_tensor(p.k, p.k_tokens, p.kv_heads, p.batch) ||
+      !tma_tensor(p.v, p.k_tokens, p.kv_heads, p.batch) || (grouped && p.q.s[2] == 0))
+    return false;
+  if (!backward) return wide_rows(p.out);
+  return tma_tensor(p.dout, p.q_tokens, p.heads, p.batch) && !(grouped && p.dout.s[2] == 0) && wide_rows(p.dq) &&
+         wide_rows(p.dk) && wide_rows(p.dv);
+}
+
+int attention_tc_splits(const AttnParams &p) {
+  if (!p.batch || !p.heads || !p.q_tokens || !p.k_tokens || p.heads / p.kv_heads > 128) return 1;
+  return tc_splits(p, shape_of(p));
+}
+
+cudaError_t attention_tc(const AttnParams &p, bool backward, cudaStream_t st) {
+  TcArgs a = shape_of(p);
+  CUtensorMap mq, mk, mv, mg;
+  bool h, b;
+  if (!encode(&mq, p.q, p.head_dim, p.heads, p.q_tokens, p.batch, a.group, a.tpt, h, b)) return cudaErrorInvalidValue;
+  a.qh = h, a.qb = b;
+  if (!encode(&mk, p.k, p.head_dim, p.kv_heads, p.k_tokens, p.batch, 1, 128, h, b)) return cudaErrorInvalidValue;
+  a.kh = h, a.kb = b;
+  if (!encode(&mv, p.v, p.head_dim, p.kv_heads, p.k_tokens, p.batch, 1, 128, h, b)) return cudaErrorInvalidValue;
+  a.vh = h, a.vb = b;
+  if (!backward) {
+    a.splits = tc_splits(p, a);
+    return p.head_dim <= 64 ? forward_tc<64>(p, a, mq, mk, mv, st) : forward_tc<128>(p, a, mq, mk, mv, st);
+  }
+  if (!encode(&mg, p.dout, p.head_dim, p.heads, p.q_tokens, p.batch, a.group, a.tpt, h, b)) return cudaErrorInvalidValue;
+  a.gh = h, a.gb = b;
+  return p.head_dim <= 64 ? backward_tc<64>(p, a, mq, mk, mv, mg, st) : backward_tc<128>(p, a, mq, mk, mv, mg, st);
+}
+
+}  // namespace gpu
+}  // namespace illumina

@@ -84,6 +84,27 @@ gpu::AttnParams attn_params(const illumina_attention_args *a, bool backward, boo
   return p;
 }
 
+// The word that attention kernels set when they give up a bounded wait: host
+// memory that every device can write, allocated on first use (a call that is
+// being captured included). A later call reports and clears it.
+int *attention_error() {
+  static int *const word = [] {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "attention: capture mode");
+    void *p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cuda_check(e, "attention: cudaHostAlloc");
+    *(int *)p = 0;
+    return (int *)p;
+  }();
+  if (*(volatile int *)word) {
+    *(volatile int *)word = 0;
+    throw Error(ILLUMINA_TIMEOUT, "attention: a kernel of an earlier call gave up a bounded wait");
+  }
+  return word;
+}
+
 }  // namespace
 
 struct illumina_adamw {
@@ -207,7 +228,8 @@ illumina_status illumina_op_attention_workspace(const illumina_attention_args *a
 
 illumina_status illumina_op_attention(const illumina_attention_args *a, void *stream) {
   ILL_TRY
-  const gpu::AttnParams p = attn_params(a, false, true);
+  gpu::AttnParams p = attn_params(a, false, true);
+  p.err = attention_error();
   cuda_check(gpu::attention(a->precision, p, (cudaStream_t)stream), "attention");
   return ILLUMINA_OK;
   ILL_CATCH
@@ -215,7 +237,8 @@ illumina_status illumina_op_attention(const illumina_attention_args *a, void *st
 
 illumina_status illumina_op_attention_backward(const illumina_attention_args *a, void *stream) {
   ILL_TRY
-  const gpu::AttnParams p = attn_params(a, true, true);
+  gpu::AttnParams p = attn_params(a, true, true);
+  p.err = attention_error();
   cuda_check(gpu::attention_backward(a->precision, p, (cudaStream_t)stream), "attention_backward");
   return ILLUMINA_OK;
   ILL_CATCH

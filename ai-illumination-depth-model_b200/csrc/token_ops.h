@@ -69,6 +69,13 @@ struct AttnParams {
 size_t attention_workspace(int T, const AttnParams &p, bool backward);
 cudaError_t attention(int T, const AttnParams &p, cudaStream_t st);
 cudaError_t attention_backward(int T, const AttnParams &p, cudaStream_t st);
+// The tensor-core kernels (bf16): whether they take these tensors (head sizes
+// that are multiples of 8, 16-byte aligned rows, a positive scale), the shares
+// the forward splits the keys into, and the kernels without the joining or the
+// row sums that surround them.
+bool attention_tc_takes(const AttnParams &p, bool backward);
+int attention_tc_splits(const AttnParams &p);
+cudaError_t attention_tc(const AttnParams &p, bool backward, cudaStream_t st);
 
 // ---- AdamW (adamw.cu) -----------------------------------------------------------
 
