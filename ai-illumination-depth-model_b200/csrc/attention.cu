@@ -230,31 +230,46 @@ __global__ void __launch_bounds__(kThreads) k_attn(const AttnParams p, int q_til
 
 // Joins the shares of a split forward: a warp takes one row.
 //   lse = log sum_s exp(lse_s),  out = sum_s exp(lse_s - lse) out_s
+constexpr int kMostSplits = 2 * 148;
 template <typename T>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnParams p, int splits) {
+  __shared__ float weights[8][kMostSplits];
   const long long rows = (long long)p.batch * p.heads * p.q_tokens;
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int lane = threadIdx.x & 31;
+  float *w = weights[threadIdx.x >> 5];
   const float *sums = p.ws + splits * rows * p.head_dim + row;
   float top = -INFINITY;
-  for (int s = 0; s < splits; s++) {
+  bool nan = false;
+  for (int s = lane; s < splits; s += 32) {
     const float v = sums[s * rows];
-    top = v != v ? v : fmaxf(top, v);
+    w[s] = v;
+    top = fmaxf(top, v);
+    nan = nan || v != v;
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (__any_sync(0xffffffffu, nan)) top = NAN;
   const float base = top == -INFINITY ? 0.0f : top;
   float total = 0;
-  for (int s = 0; s < splits; s++) total += expf(sums[s * rows] - base);
+  for (int s = lane; s < splits; s += 32) {
+    w[s] = expf(w[s] - base);
+    total += w[s];
+  }
+  total = warp_sum(total);
+  __syncwarp();
   const float inv = total == 0 ? 0.0f : 1.0f / total;
   const long long i = row % p.q_tokens, bh = row / p.q_tokens;
   T *out = (T *)p.out.p + bh / p.heads * p.out.s[0] + i * p.out.s[1] + bh % p.heads * p.out.s[2];
+  const float *part = p.ws + row * p.head_dim;
+  const long long step = rows * p.head_dim;
   for (int d = lane; d < p.head_dim; d += 32) {
     float o = 0;
-    for (int s = 0; s < splits; s++) {
-      const float f = expf(sums[s * rows] - base) * inv;
-      if (f != 0) o += f * p.ws[(s * rows + row) * p.head_dim + d];
-    }
-    from_f32(out[d], o);
+#pragma unroll 8
+    for (int s = 0; s < splits; s++)  // a share without keys (weight 0) has no output
+      if (w[s] != 0) o = fmaf(w[s], __ldcg(part + s * step + d), o);
+    from_f32(out[d], o * inv);
   }
   if (lane == 0) p.lse[row] = total == 0 ? -INFINITY : top + logf(total);
 }
@@ -423,7 +438,7 @@ int simt_splits(const AttnParams &p) {
   const long long ctas = (long long)p.batch * p.heads * ceil_div(p.q_tokens, kFix);
   const int tiles = ceil_div(p.k_tokens, STR);
   if (ctas == 0 || ctas >= 148 || tiles < 8) return 1;
-  const int want = (int)((2 * 148 + ctas - 1) / ctas), most = tiles / 4;
+  const int want = (int)(kMostSplits / ctas), most = tiles / 4;
   return want < most ? want : most;
 }
 
@@ -434,14 +449,11 @@ cudaError_t run_simt(const AttnParams &p, bool bwd, cudaStream_t st) {
   const long long rows = (long long)p.batch * p.heads * p.q_tokens;
   constexpr size_t fix = sizeof(float) * DP * kFixLd, str = sizeof(float) * DP * (STR + 4),
                    prob = sizeof(float) * STR * kFixLd;
-  auto big = [](const void *f, size_t bytes) {
-    return bytes > 48 * 1024 ? cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
-  };
   cudaError_t e;
   if (!bwd) {
     const int splits = simt_splits<STR>(p);
     const size_t sm = fix + str + prob;
-    if ((e = big((const void *)k_attn<T, DP, STR>, sm)) != cudaSuccess) return e;
+    if ((e = allow_smem<k_attn<T, DP, STR>>(sm)) != cudaSuccess) return e;
     const long long grid = (long long)p.batch * p.heads * q_tiles * splits;
     if (grid > 0) k_attn<T, DP, STR><<<(unsigned)grid, kThreads, sm, st>>>(p, q_tiles, splits, vec);
     if (splits > 1) k_attn_join<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, splits);
@@ -450,13 +462,13 @@ cudaError_t run_simt(const AttnParams &p, bool bwd, cudaStream_t st) {
   if (rows > 0) {
     k_attn_delta<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
     const size_t sm = 2 * fix + 2 * str + prob;
-    if ((e = big((const void *)k_attn_dq<T, DP, STR>, sm)) != cudaSuccess) return e;
+    if ((e = allow_smem<k_attn_dq<T, DP, STR>>(sm)) != cudaSuccess) return e;
     k_attn_dq<T, DP, STR><<<(unsigned)((long long)p.batch * p.heads * q_tiles), kThreads, sm, st>>>(p, q_tiles, vec);
   }
   const long long grid = (long long)p.batch * p.kv_heads * k_tiles;
   if (grid > 0) {
     const size_t sm = 2 * fix + 2 * str + 2 * prob;
-    if ((e = big((const void *)k_attn_dkv<T, DP, STR>, sm)) != cudaSuccess) return e;
+    if ((e = allow_smem<k_attn_dkv<T, DP, STR>>(sm)) != cudaSuccess) return e;
     k_attn_dkv<T, DP, STR><<<(unsigned)grid, kThreads, sm, st>>>(p, k_tiles, vec);
   }
   return cudaGetLastError();
@@ -494,11 +506,7 @@ cudaError_t attention(int T, const AttnParams &p, cudaStream_t st) {
 
 cudaError_t attention_backward(int T, const AttnParams &p, cudaStream_t st) {
   if (T == F32) return run_simt<float>(p, true, st);
-  if (!attention_tc_takes(p, true)) return run_simt<bf16>(p, true, st);
-  const long long rows = (long long)p.batch * p.heads * p.q_tokens;
-  k_attn_delta<bf16><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
-  const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess ? e : attention_tc(p, true, st);
+  return attention_tc_takes(p, true) ? attention_tc(p, true, st) : run_simt<bf16>(p, true, st);
 }
 
 }  // namespace gpu

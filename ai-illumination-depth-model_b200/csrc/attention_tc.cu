@@ -38,6 +38,7 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 namespace {
 
 using namespace tcx;
+using tok::allow_smem;
 using tok::bf16;
 
 constexpr int kTcThreads = 384;
@@ -114,6 +115,18 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&b);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two finite values >= 0 as bf16, rounded to the nearest (ties away from
+// zero). The conversion instruction shares the pipe of the exponentials, which
+// bounds these kernels; two integer additions and a byte permutation do not.
+__device__ __forceinline__ uint32_t pack2_finite(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
 }
 
 // A wait that ends when another role of the CTA has given up, too.
@@ -224,9 +237,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int pairs = (a.q_tiles + 1) / 2;
   const int split = (int)(id % a.splits);
   id /= a.splits;
-  const int pair = pairs - 1 - (int)(id % pairs);  // the longest causal rows first
-  id /= pairs;
-  const int hk = (int)(id % p.kv_heads), n = (int)(id / p.kv_heads);
+  const int hk = (int)(id % p.kv_heads);
+  id /= p.kv_heads;
+  const int n = (int)(id % p.batch);
+  const int pair = pairs - 1 - (int)(id / p.batch);  // the longest causal rows of all heads first
   const AttnMask mask(p, n);
   // key tiles [t0, t1[i]) of query tile i
   int t0, t1[2], most = 0;
@@ -374,7 +388,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
       for (int c = 0; c < 4; c++) m4[c] = __uint_as_float(r[c]);
 #pragma unroll
-      for (int c = 4; c < 128; c++) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(r[c]));
+      for (int c = 4; c < 124; c += 8)
+#pragma unroll
+        for (int k = 0; k < 4; k++) m4[k] = max3(m4[k], __uint_as_float(r[c + k]), __uint_as_float(r[c + 4 + k]));
+#pragma unroll
+      for (int c = 0; c < 4; c++) m4[c] = fmaxf(m4[c], __uint_as_float(r[124 + c]));
       const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
       bool grow = false;
       float f = 1.0f;
@@ -401,21 +419,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       const float shift = top == -INFINITY ? 0.0f : -top;
-      float s4[4] = {0, 0, 0, 0};
+      const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(shift, shift);
+      float2 s2[2] = {make_float2(0, 0), make_float2(0, 0)};
 #pragma unroll
       for (int c = 0; c < 128; c += 32) {
         uint32_t q[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          const float x = ex2(fmaf(__uint_as_float(r[c + k]), sl2, shift));
-          const float y = ex2(fmaf(__uint_as_float(r[c + k + 1]), sl2, shift));
-          s4[k & 2] += x;
-          s4[(k & 2) + 1] += y;
-          q[k / 2] = pack2(x, y);
+          float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c + k]), __uint_as_float(r[c + k + 1])), scale2, shift2);
+          x = make_float2(ex2(x.x), ex2(x.y));
+          s2[k / 2 & 1] = __fadd2_rn(s2[k / 2 & 1], x);
+          // a NaN goes missing here, and shows in the sum
+          q[k / 2] = pack2_finite(x.x, x.y);
         }
         tmem_st16(ts + c / 2, q);
       }
-      sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      sum += (s2[0].x + s2[0].y) + (s2[1].x + s2[1].y);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -502,9 +521,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int warp = threadIdx.x >> 5;
 
   long long id = blockIdx.x;
-  const int kt = (int)(id % a.k_tiles);  // the keys that most queries see first
-  id /= a.k_tiles;
-  const int hk = (int)(id % p.kv_heads), n = (int)(id / p.kv_heads);
+  const int hk = (int)(id % p.kv_heads);
+  id /= p.kv_heads;
+  const int n = (int)(id % p.batch), kt = (int)(id / p.batch);  // the keys that most queries see first
   const AttnMask mask(p, n);
   const int key0 = kt * 128;
   const int t0 = key0 < mask.k_len ? mask.row_begin(key0) / a.tpt : 0;
@@ -607,7 +626,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int begin = key < mask.k_len ? mask.row_begin(key) : INT_MAX / 2;
     const float sl2 = p.scale * kLog2e;
     float *mine_lse = row_sums + warp * 128, *mine_delta = mine_lse + 64;
-    // lse (base 2; +inf where the row has no probabilities) and delta of the
+    const float2 scale2 = make_float2(sl2, sl2);
+    // -lse (base 2; -inf where the row has no probabilities) and delta of the
     // two columns this lane fetches of query tile j
     float nl[2], nd[2];
     auto fetch = [&](int j) {
@@ -615,11 +635,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int k = 0; k < 2; k++) {
         const int r = wg * 64 + k * 32 + lane;
         const int token = j * a.tpt + r / a.group, h = hk * a.group + r % a.group;
-        nl[k] = INFINITY, nd[k] = 0;
+        nl[k] = -INFINITY, nd[k] = 0;
         if (r < a.group * a.tpt && token < mask.q_len) {
           const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
           const float v = p.lse[at];
-          nl[k] = v == -INFINITY ? INFINITY : v * kLog2e;
+          nl[k] = v == -INFINITY ? -INFINITY : -v * kLog2e;
           nd[k] = p.ws[at];
         }
       }
@@ -630,8 +650,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int it = j - t0;
       __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 2; k++) mine_lse[k * 32 + lane] = nl[k], mine_delta[k * 32 + lane] = nd[k];
+      for (int k = 0; k < 2; k++) mine_lse[k * 32 + lane] = nl[k], mine_delta[k * 32 + lane] = -nd[k];
       __syncwarp();
+      // probabilities are NaN where a row's lse is, and nowhere else
+      const bool spoiled = __any_sync(0xffffffffu, nl[0] != nl[0] || nl[1] != nl[1]);
       if (j + 1 < t1) fetch(j + 1);
       // columns below `skip` are queries that do not see this key
       const long long skip_ll = ((long long)begin - (long long)j * a.tpt) * a.group - wg * 64;
@@ -647,10 +669,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
       for (int c = 0; c < 64; c += 4) {
         const float4 l = *reinterpret_cast<const float4 *>(mine_lse + c);
-        r[c] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c]), sl2, -l.x)));
-        r[c + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c + 1]), sl2, -l.y)));
-        r[c + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c + 2]), sl2, -l.z)));
-        r[c + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c + 3]), sl2, -l.w)));
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, make_float2(l.x, l.y));
+        const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, make_float2(l.z, l.w));
+        r[c] = __float_as_uint(ex2(x.x)), r[c + 1] = __float_as_uint(ex2(x.y));
+        r[c + 2] = __float_as_uint(ex2(y.x)), r[c + 3] = __float_as_uint(ex2(y.y));
       }
       if (masked) {
 #pragma unroll
@@ -658,8 +680,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (c < skip) r[c] = 0;
       }
       uint32_t q[32];
+      if (!spoiled) {
 #pragma unroll
-      for (int c = 0; c < 32; c++) q[c] = pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+        for (int c = 0; c < 32; c++) q[c] = pack2_finite(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; c++) q[c] = pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      }
       tmem_st32(ts, q);
       tmem_wait_st();
       tc_fence_before();
@@ -676,9 +703,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
           const float4 d = *reinterpret_cast<const float4 *>(mine_delta + 32 * half + c);
-          const float *pr = reinterpret_cast<const float *>(r) + 32 * half + c;
-          float v[4] = {pr[0] * (__uint_as_float(g[c]) - d.x), pr[1] * (__uint_as_float(g[c + 1]) - d.y),
-                        pr[2] * (__uint_as_float(g[c + 2]) - d.z), pr[3] * (__uint_as_float(g[c + 3]) - d.w)};
+          const uint32_t *pr = r + 32 * half + c;
+          const float2 x = __fmul2_rn(make_float2(__uint_as_float(pr[0]), __uint_as_float(pr[1])),
+                                      __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), make_float2(d.x, d.y)));
+          const float2 y = __fmul2_rn(make_float2(__uint_as_float(pr[2]), __uint_as_float(pr[3])),
+                                      __fadd2_rn(make_float2(__uint_as_float(g[c + 2]), __uint_as_float(g[c + 3])), make_float2(d.z, d.w)));
+          float v[4] = {x.x, x.y, y.x, y.y};
           if (masked) {
 #pragma unroll
             for (int k = 0; k < 4; k++)
@@ -717,7 +747,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // ---------------------------------------------------------------------------
 // Backward, dQ: one query tile past the key tiles it sees. S = Q K' and
 // dP = dO V' are recomputed, dQ += dS K from TMEM. The warpgroups take 64 key
-// columns each; a thread's lse and delta stay in registers.
+// columns each; a thread's lse and delta stay in registers. This pass runs
+// first and leaves the row sums delta in the workspace for the other.
 // ---------------------------------------------------------------------------
 
 template <int DP>
@@ -729,7 +760,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   extern __shared__ uint8_t raw[];
   uint8_t *base = align1024(raw);
   uint8_t *sq = base, *sg = sq + L::kTile, *sk = sg + L::kTile, *sv = sk + L::kStages * L::kTile;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile);
+  float *row_sums = reinterpret_cast<float *>(sv + L::kStages * L::kTile);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile + L::kRowSums);
   uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 2, *s_free = bars + 3, *d_full = bars + 4,
            *done = bars + 5, *drain = bars + 6, *full = bars + 7, *empty = full + L::kStages;
   uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 7 + 2 * L::kStages);
@@ -737,9 +769,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int warp = threadIdx.x >> 5;
 
   long long id = blockIdx.x;
-  const int qt = a.q_tiles - 1 - (int)(id % a.q_tiles);  // the longest causal rows first
-  id /= a.q_tiles;
-  const int hk = (int)(id % p.kv_heads), n = (int)(id / p.kv_heads);
+  const int hk = (int)(id % p.kv_heads);
+  id /= p.kv_heads;
+  const int n = (int)(id % p.batch);
+  const int qt = a.q_tiles - 1 - (int)(id / p.batch);  // the longest causal rows first
   const AttnMask mask(p, n);
   const int first = qt * a.tpt;
   const int t1 = first < mask.q_len ? (mask.key_end(min(first + a.tpt, mask.q_len) - 1) + 127) / 128 : 0;
@@ -828,8 +861,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int end = mine ? mask.key_end(token) : 0;
     const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
     const float v = end ? p.lse[at] : -INFINITY;
-    const float lse = v == -INFINITY ? INFINITY : v * kLog2e, delta = end ? p.ws[at] : 0.0f;
+    const float shift = v == -INFINITY ? -INFINITY : -v * kLog2e;
+    // delta = rowsum(dO O): a warpgroup adds every second 8 columns
+    float part = 0;
+    if (end > 0) {
+      const bf16 *x = (const bf16 *)p.dout.p + n * p.dout.s[0] + token * p.dout.s[1] + h * p.dout.s[2];
+      const bf16 *y = (const bf16 *)p.out.p + n * p.out.s[0] + token * p.out.s[1] + h * p.out.s[2];
+#pragma unroll
+      for (int c = 0; c < DP; c += 16)
+        if (c + wg * 8 < p.head_dim) {
+          float u[8], w[8];
+          tok::Pack<bf16, 8>::load(x + c + wg * 8, u);
+          tok::Pack<bf16, 8>::load(y + c + wg * 8, w);
+#pragma unroll
+          for (int k = 0; k < 8; k++) part = fmaf(u[k], w[k], part);
+        }
+    }
+    row_sums[wg * 128 + row] = part;
+    bar_named(1, 256);
+    const float delta = row_sums[row] + row_sums[128 + row];
+    if (wg == 0 && mine) p.ws[at] = delta;  // for the key pass
     const float sl2 = p.scale * kLog2e;
+    const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(shift, shift), delta2 = make_float2(-delta, -delta);
     bool ok = true;
     for (int j = 0; j < t1; j++) {
       const int left = end - j * 128 - wg * 64;
@@ -845,7 +898,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
 #pragma unroll
-      for (int c = 0; c < 64; c++) r[c] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c]), sl2, -lse)));
+      for (int c = 0; c < 64; c += 2) {
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, shift2);
+        r[c] = __float_as_uint(ex2(x.x)), r[c + 1] = __float_as_uint(ex2(x.y));
+      }
       ok = wait.warp(g_full, j & 1);
       if (!ok) break;
       tc_fence_after();
@@ -857,13 +913,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
-          float x = __uint_as_float(r[32 * half + c]) * (__uint_as_float(g[c]) - delta);
-          float y = __uint_as_float(r[32 * half + c + 1]) * (__uint_as_float(g[c + 1]) - delta);
+          float2 x = __fmul2_rn(make_float2(__uint_as_float(r[32 * half + c]), __uint_as_float(r[32 * half + c + 1])),
+                                __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), delta2));
           if (masked) {
-            if (32 * half + c >= left) x = 0;
-            if (32 * half + c + 1 >= left) y = 0;
+            if (32 * half + c >= left) x.x = 0;
+            if (32 * half + c + 1 >= left) x.y = 0;
           }
-          q[16 * half + c / 2] = pack2(x, y);
+          q[16 * half + c / 2] = pack2(x.x, x.y);
         }
       }
       tmem_st32(tg, q);
@@ -950,15 +1006,11 @@ int tc_splits(const AttnParams &p, const TcArgs &a) {
   return want < most ? want : most;
 }
 
-cudaError_t big(const void *f, size_t bytes) {
-  return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
 template <int DP>
 cudaError_t forward_tc(const AttnParams &p, const TcArgs &a, const CUtensorMap &mq, const CUtensorMap &mk,
                        const CUtensorMap &mv, cudaStream_t st) {
   constexpr size_t sm = FwdSmem<DP>::kBytes;
-  const cudaError_t e = big((const void *)k_attn_tc<DP>, sm);
+  const cudaError_t e = allow_smem<k_attn_tc<DP>>(sm);
   if (e != cudaSuccess) return e;
   const long long grid = (long long)p.batch * p.kv_heads * ((a.q_tiles + 1) / 2) * a.splits;
   k_attn_tc<DP><<<(unsigned)grid, kTcThreads, sm, st>>>(mq, mk, mv, p, a);
@@ -969,12 +1021,12 @@ template <int DP>
 cudaError_t backward_tc(const AttnParams &p, const TcArgs &a, const CUtensorMap &mq, const CUtensorMap &mk,
                         const CUtensorMap &mv, const CUtensorMap &mg, cudaStream_t st) {
   constexpr size_t sm = BwdSmem<DP>::kBytes;
-  cudaError_t e = big((const void *)k_attn_dq_tc<DP>, sm);
-  if (e == cudaSuccess) e = big((const void *)k_attn_dkv_tc<DP>, sm);
+  cudaError_t e = allow_smem<k_attn_dq_tc<DP>>(sm);
+  if (e == cudaSuccess) e = allow_smem<k_attn_dkv_tc<DP>>(sm);
   if (e != cudaSuccess) return e;
   const long long heads = (long long)p.batch * p.kv_heads;
-  k_attn_dkv_tc<DP><<<(unsigned)(heads * a.k_tiles), kTcThreads, sm, st>>>(mq, mk, mv, mg, p, a);
   k_attn_dq_tc<DP><<<(unsigned)(heads * a.q_tiles), kTcThreads, sm, st>>>(mq, mk, mv, mg, p, a);
+  k_attn_dkv_tc<DP><<<(unsigned)(heads * a.k_tiles), kTcThreads, sm, st>>>(mq, mk, mv, mg, p, a);
   return cudaGetLastError();
 }
 
@@ -988,7 +1040,7 @@ bool attention_tc_takes(const AttnParams &p, bool backward) {
       !tma_tensor(p.v, p.k_tokens, p.kv_heads, p.batch) || (grouped && p.q.s[2] == 0))
     return false;
   if (!backward) return wide_rows(p.out);
-  return tma_tensor(p.dout, p.q_tokens, p.heads, p.batch) && !(grouped && p.dout.s[2] == 0) && wide_rows(p.dq) &&
+  return tma_tensor(p.dout, p.q_tokens, p.heads, p.batch) && wide_rows(p.out) && !(grouped && p.dout.s[2] == 0) && wide_rows(p.dq) &&
          wide_rows(p.dk) && wide_rows(p.dv);
 }
 

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace illumina {
@@ -65,6 +66,19 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// Lets kernel K use `bytes` of dynamic shared memory on the current device;
+// the runtime is asked once a device.
+template <auto K>
+cudaError_t allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> seen{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && seen.load(std::memory_order_relaxed) >> dev & 1)) return e;
+  e = cudaFuncSetAttribute((const void *)K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && dev < 64) seen.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -174,10 +174,10 @@ SIGNATURES = {
     "illumina_op_layer_norm_backward": (_S, [C.c_int, _V, C.c_longlong, _V, C.c_longlong, C.c_longlong, C.c_int, _V, _V,
                                              _V, _V, C.c_longlong, _V, _V, _V, C.c_size_t, _V]),
     "illumina_op_layer_norm_workspace": (_S, [C.c_longlong, C.c_int, C.POINTER(C.c_size_t)]),
-    "illumina_op_rotary": (_S, [C.POINTER(RotaryArgs), _V]),
-    "illumina_op_attention_workspace": (_S, [C.POINTER(AttentionArgs), C.c_int, C.POINTER(C.c_size_t)]),
-    "illumina_op_attention": (_S, [C.POINTER(AttentionArgs), _V]),
-    "illumina_op_attention_backward": (_S, [C.POINTER(AttentionArgs), _V]),
+    "illumina_op_rotary": (_S, [_V, _V]),
+    "illumina_op_attention_workspace": (_S, [_V, C.c_int, C.POINTER(C.c_size_t)]),
+    "illumina_op_attention": (_S, [_V, _V]),
+    "illumina_op_attention_backward": (_S, [_V, _V]),
     "illumina_adamw_blocks": (_S, [C.POINTER(C.c_longlong), C.c_int, C.POINTER(C.c_longlong)]),
     "illumina_adamw_create": (_S, [C.POINTER(AdamwOptions), C.POINTER(C.c_void_p)]),
     "illumina_adamw_destroy": (_S, [_V]),

@@ -16,11 +16,19 @@ IlluminaError with status INVALID_ARG.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
+import struct
 from dataclasses import dataclass
 
 from ._lib import (ACT, ENGINE, INVALID_ARG, PRECISION_BF16, PRECISION_F32, AttentionArgs, IlluminaError, RotaryArgs,
                    check, lib, ptr, stream_handle)
+
+# illumina_rotary_args and illumina_attention_args as one packing each: a call fills some forty fields, and setting
+# them one by one takes longer than a small call's kernel
+_ROTARY_ARGS = struct.Struct("@iqqiiiiiPPi3q3qPPi3q3qPi3qPP")
+_ATTENTION_ARGS = struct.Struct("@iiiiiiiif" + "P3q" * 4 + "PPP" + "P3q" * 4 + "PN")
+assert _ROTARY_ARGS.size == C.sizeof(RotaryArgs) and _ATTENTION_ARGS.size == C.sizeof(AttentionArgs)
 
 
 def set_engine(engine: str) -> None:
@@ -105,28 +113,33 @@ def _require(ok, message):
 
 
 class _On:
-    """Makes a tensor's device and the call's stream current for a scope; `handle` is the stream's cudaStream_t."""
+    """Makes a tensor's device and the call's stream current for a scope; `handle` is the stream's cudaStream_t.
+    Usually both are current already: then this is two reads of torch's state."""
+    __slots__ = ("handle", "_scopes")
 
     def __init__(self, torch, device, stream):
-        self._scopes = []
-        if device.index != torch.cuda.current_device():
-            self._scopes.append(torch.cuda.device(device))
+        index = device.index
+        self._scopes = None
         if stream is None:
-            self.handle = torch.cuda.current_stream(device).cuda_stream
+            self.handle = torch._C._cuda_getCurrentRawStream(index)
+            if torch._C._cuda_getDevice() != index:
+                self._scopes = (torch.cuda.device(device),)
         else:
             if isinstance(stream, int):
                 stream = torch.cuda.ExternalStream(stream, device=device)
-            self._scopes.append(torch.cuda.stream(stream))
+            self._scopes = (torch.cuda.device(device), torch.cuda.stream(stream))
             self.handle = stream.cuda_stream
 
     def __enter__(self):
-        for s in self._scopes:
-            s.__enter__()
-        return self
+        if self._scopes:
+            for s in self._scopes:
+                s.__enter__()
+        return self.handle
 
     def __exit__(self, *exc):
-        for s in reversed(self._scopes):
-            s.__exit__(*exc)
+        if self._scopes:
+            for s in reversed(self._scopes):
+                s.__exit__(*exc)
 
 
 def _precision(torch, name, x):
@@ -138,21 +151,25 @@ def _precision(torch, name, x):
 
 def _tensor(torch, name, x, like=None, dims=None):
     """Checks a storage tensor: on a CUDA device, contiguous in its last dimension, of `like`'s type and device."""
-    _require(isinstance(x, torch.Tensor) and x.is_cuda, f"{name} must be a CUDA tensor")
-    _require(dims is None or x.dim() == dims, f"{name} must have {dims} dimensions")
-    _require(x.dim() > 0 and (x.shape[-1] <= 1 or x.stride(-1) == 1), f"{name} must be contiguous in its last dimension")
-    if like is not None:
-        _require(x.dtype == like.dtype and x.device == like.device, f"{name} must have the type and device of the others")
-    return x
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        _require(False, f"{name} must be a CUDA tensor")
+    shape = x.shape
+    if dims is not None and len(shape) != dims:
+        _require(False, f"{name} must have {dims} dimensions")
+    if not shape or (shape[-1] > 1 and x.stride(-1) != 1):
+        _require(False, f"{name} must be contiguous in its last dimension")
+    if like is not None and (x.dtype != like.dtype or x.get_device() != like.get_device()):
+        _require(False, f"{name} must have the type and device of the others")
 
 
 def _vector(torch, name, x, n, device, dtype=None):
-    """Checks a contiguous vector of n elements (float32 by default); None passes."""
+    """Checks a contiguous vector of n elements (float32 by default) and returns its address; None passes."""
     if x is None:
-        return
-    _require(isinstance(x, torch.Tensor) and x.dtype == (dtype or torch.float32) and x.device == device and
-             x.numel() == n and x.is_contiguous(),
-             f"{name} must be {n} contiguous {str(dtype or torch.float32)[6:]} values on the device of the others")
+        return None
+    dtype = dtype or torch.float32
+    if not (isinstance(x, torch.Tensor) and x.dtype == dtype and x.device == device and x.numel() == n and x.is_contiguous()):
+        _require(False, f"{name} must be {n} contiguous {str(dtype)[6:]} values on the device of the others")
+    return x.data_ptr()
 
 
 def _rows(torch, name, x):
@@ -170,6 +187,13 @@ def _rows(torch, name, x):
     return rows, shape[-1], shape[-1] if stride is None else stride
 
 
+@functools.lru_cache(maxsize=4096)
+def _norm_workspace(rows, c):
+    size = C.c_size_t(0)
+    check(lib().illumina_op_layer_norm_workspace(rows, c, C.byref(size)))
+    return size.value
+
+
 def layerNorm(x, weight=None, bias=None, eps=1e-6, out=None, stream=None):
     """Layer norm over the last dimension: (y, mean, rstd), the float32 statistics [rows] being what layerNormBackward
     needs. weight, bias: float32 [width] or None. out may be x."""
@@ -177,20 +201,21 @@ def layerNorm(x, weight=None, bias=None, eps=1e-6, out=None, stream=None):
     _tensor(torch, "x", x)
     precision = _precision(torch, "x", x)
     rows, c, stride = _rows(torch, "x", x)
-    _require(c > 0, "x must not have a width of zero")
-    _vector(torch, "weight", weight, c, x.device)
-    _vector(torch, "bias", bias, c, x.device)
-    with _On(torch, x.device, stream) as on:
+    if not c:
+        _require(False, "x must not have a width of zero")
+    device = x.device
+    w = _vector(torch, "weight", weight, c, device)
+    b = _vector(torch, "bias", bias, c, device)
+    with _On(torch, device, stream) as handle:
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out, out_stride = x.new_empty(x.shape), c
         else:
             _tensor(torch, "out", out, x)
             _require(out.shape == x.shape, "out must have the shape of x")
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-        mean, rstd = stats.unbind()
-        check(lib().illumina_op_layer_norm(precision, x.data_ptr(), stride, rows, c, ptr(weight), ptr(bias), eps,
-                                           out.data_ptr(), _rows(torch, "out", out)[2], mean.data_ptr(),
-                                           rstd.data_ptr(), on.handle))
+            out_stride = _rows(torch, "out", out)[2]
+        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=device).unbind()
+        check(lib().illumina_op_layer_norm(precision, x.data_ptr(), stride, rows, c, w, b, eps, out.data_ptr(), out_stride,
+                                           mean.data_ptr(), rstd.data_ptr(), handle))
     return out, mean, rstd
 
 
@@ -199,26 +224,29 @@ def layerNormBackward(dy, x, mean, rstd, weight=None, needWeight=True, stream=No
     import torch
     _tensor(torch, "x", x)
     _tensor(torch, "dy", dy, x)
-    _require(dy.shape == x.shape, "dy must have the shape of x")
+    if dy.shape != x.shape:
+        _require(False, "dy must have the shape of x")
     precision = _precision(torch, "x", x)
     rows, c, stride = _rows(torch, "x", x)
     _, _, dy_stride = _rows(torch, "dy", dy)
-    _require(c > 0, "x must not have a width of zero")
-    _vector(torch, "weight", weight, c, x.device)
-    _require(mean is not None and rstd is not None, "mean and rstd of the forward pass are needed")
-    _vector(torch, "mean", mean, rows, x.device)
-    _vector(torch, "rstd", rstd, rows, x.device)
-    with _On(torch, x.device, stream) as on:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if not c:
+        _require(False, "x must not have a width of zero")
+    device = x.device
+    w = _vector(torch, "weight", weight, c, device)
+    if mean is None or rstd is None:
+        _require(False, "mean and rstd of the forward pass are needed")
+    mean_at, rstd_at = _vector(torch, "mean", mean, rows, device), _vector(torch, "rstd", rstd, rows, device)
+    with _On(torch, device, stream) as handle:
+        dx = x.new_empty(x.shape)
         dw = db = workspace = None
-        size = C.c_size_t(0)
+        size = 0
         if needWeight:
-            check(lib().illumina_op_layer_norm_workspace(rows, c, C.byref(size)))
-            dw, db = torch.empty(c, dtype=torch.float32, device=x.device), torch.empty(c, dtype=torch.float32, device=x.device)
-            workspace = torch.empty(size.value, dtype=torch.uint8, device=x.device)
-        check(lib().illumina_op_layer_norm_backward(precision, dy.data_ptr(), dy_stride, x.data_ptr(), stride, rows, c,
-                                                    ptr(weight), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), c,
-                                                    ptr(dw), ptr(db), ptr(workspace), size.value, on.handle))
+            size = _norm_workspace(rows, c)
+            dw, db = torch.empty((2, c), dtype=torch.float32, device=device).unbind()
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        check(lib().illumina_op_layer_norm_backward(precision, dy.data_ptr(), dy_stride, x.data_ptr(), stride, rows, c, w,
+                                                    mean_at, rstd_at, dx.data_ptr(), c, ptr(dw), ptr(db), ptr(workspace),
+                                                    size, handle))
     return dx, dw, db
 
 
@@ -272,63 +300,61 @@ def rotary(q, positions, plan, k=None, inverse=False, outQ=None, outK=None, stre
     if k is not None:
         _tensor(torch, "k", k, q, 4)
         _require((k.shape[0], k.shape[1], k.shape[3]) == (b, t, d), "k must have the batch, tokens and head size of q")
-    args = RotaryArgs(precision=precision, batch=b, tokens=t, head_dim=d, pairs=plan.turns.numel(), axes=plan.axes,
-                      interleaved=plan.interleaved, inverse=bool(inverse), positions=positions.data_ptr(),
-                      positions_float=positions.dtype == torch.float32, turns=plan.turns.data_ptr(),
-                      axis=plan.axis.data_ptr())
     ps = positions.stride()
-    args.position_stride[:] = (ps[0], ps[1], ps[2]) if len(ps) == 3 else (ps[0], 0, ps[1])
-    with _On(torch, q.device, stream) as on:
-        results = []
-        for slot, x, out, name in ((args.first, q, outQ, "outQ"), (args.second, k, outK, "outK")):
+    with _On(torch, q.device, stream) as handle:
+        outs, tensors = [], []
+        for x, out, name in ((q, outQ, "outQ"), (k, outK, "outK")):
             if x is None:
+                tensors += (0, 0, 0, 0, 0, 0, 0, 0, 0)
                 continue
             if out is None:
-                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                out = x.new_empty(x.shape)
             else:
                 _tensor(torch, name, out, x, 4)
                 _require(out.shape == x.shape, f"{name} must have the shape of its input")
-            slot.x, slot.y, slot.heads = x.data_ptr(), out.data_ptr(), x.shape[2]
-            slot.x_stride[:], slot.y_stride[:] = x.stride()[:3], out.stride()[:3]
-            results.append(out)
-        check(lib().illumina_op_rotary(C.byref(args), on.handle))
-    return results[0] if k is None else tuple(results)
+            tensors += (x.data_ptr(), out.data_ptr(), x.shape[2], *x.stride()[:3], *out.stride()[:3])
+            outs.append(out)
+        turns, axis = plan.turns, plan.axis
+        args = _ROTARY_ARGS.pack(precision, b, t, d, turns.numel(), plan.axes, plan.interleaved, bool(inverse), *tensors,
+                                 positions.data_ptr(), positions.dtype == torch.float32, ps[0],
+                                 ps[1] if len(ps) == 3 else 0, ps[-1], turns.data_ptr(), axis.data_ptr())
+        check(lib().illumina_op_rotary(args, handle))
+    return outs[0] if k is None else tuple(outs)
 
 
-def _set(slot, x):
-    slot.data = x.data_ptr()
-    slot.stride[:] = x.stride()[:3]
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(precision, b, h, hk, d, tq, tk, backward):
+    args = AttentionArgs(precision=precision, batch=b, heads=h, kv_heads=hk, head_dim=d, q_tokens=tq, k_tokens=tk, scale=1.0)
+    size = C.c_size_t(0)
+    check(lib().illumina_op_attention_workspace(C.byref(args), backward, C.byref(size)))
+    return size.value
 
 
-def _attention_args(torch, q, k, v, scale, causalBlock, qLens, kLens):
-    _tensor(torch, "q", q, dims=4)
+def _attention(torch, q, k, v, scale, causalBlock, qLens, kLens):
+    """Checks an attention call; the leading fields of its arguments, the fields of q, k and v, and the lengths'."""
+    _tensor(torch, "q", q, None, 4)
     _tensor(torch, "k", k, q, 4)
     _tensor(torch, "v", v, q, 4)
-    (b, tq, h, d), (_, tk, hk, _) = q.shape, k.shape
-    _require(k.shape == v.shape and k.shape[0] == b and k.shape[3] == d, "k and v must have q's batch and head size, and one shape")
-    _require(hk > 0 and h % hk == 0, "q's heads must be a multiple of the key heads")
+    (b, tq, h, d), (kb, tk, hk, kd) = q.shape, k.shape
+    if k.shape != v.shape or kb != b or kd != d:
+        _require(False, "k and v must have q's batch and head size, and one shape")
+    if hk < 1 or h % hk:
+        _require(False, "q's heads must be a multiple of the key heads")
     _require(1 <= d <= 128, "head sizes from 1 to 128 are supported")
     _require(max(b, h, tq, tk) < 2 ** 30, "attention: size beyond 2^30")
     _require(isinstance(causalBlock, int) and 0 <= causalBlock < 2 ** 31, "causalBlock must be a token count, 0 for none")
-    _vector(torch, "qLens", qLens, b, q.device, torch.int32)
-    _vector(torch, "kLens", kLens, b, q.device, torch.int32)
-    args = AttentionArgs(precision=_precision(torch, "q", q), batch=b, heads=h, kv_heads=hk, head_dim=d, q_tokens=tq,
-                         k_tokens=tk, causal_block=causalBlock, scale=d ** -0.5 if scale is None else scale,
-                         q_lens=ptr(qLens), k_lens=ptr(kLens))
-    _set(args.q, q)
-    _set(args.k, k)
-    _set(args.v, v)
-    return args
+    device = q.device
+    lens = (_vector(torch, "qLens", qLens, b, device, torch.int32) or 0,
+            _vector(torch, "kLens", kLens, b, device, torch.int32) or 0)
+    sizes = (_precision(torch, "q", q), b, h, hk, d, tq, tk)
+    return sizes, (causalBlock, d ** -0.5 if scale is None else scale, *_fields(q), *_fields(k), *_fields(v)), lens
 
 
-def _workspace(torch, args, backward, device):
-    size = C.c_size_t(0)
-    check(lib().illumina_op_attention_workspace(C.byref(args), backward, C.byref(size)))
-    if not size.value:
-        return None
-    workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
-    args.workspace, args.workspace_bytes = workspace.data_ptr(), size.value
-    return workspace
+def _fields(x):
+    return (x.data_ptr(), *x.stride()[:3])
+
+
+_NO_TENSORS = (0,) * 16
 
 
 def attention(q, k, v, scale=None, causalBlock=0, qLens=None, kLens=None, stream=None):
@@ -340,31 +366,35 @@ def attention(q, k, v, scale=None, causalBlock=0, qLens=None, kLens=None, stream
     sees its own block of n keys and those before it (1: causal tokens; the tokens of a frame: causal frames). Rows
     that see no key are zeros with lse -inf."""
     import torch
-    args = _attention_args(torch, q, k, v, scale, causalBlock, qLens, kLens)
-    with _On(torch, q.device, stream) as on:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
-        _set(args.out, out)
-        args.lse = lse.data_ptr()
-        workspace = _workspace(torch, args, 0, q.device)  # noqa: F841 - alive until the launch is queued
-        check(lib().illumina_op_attention(C.byref(args), on.handle))
+    sizes, inputs, lens = _attention(torch, q, k, v, scale, causalBlock, qLens, kLens)
+    device = q.device
+    with _On(torch, device, stream) as handle:
+        out = q.new_empty(q.shape)
+        lse = torch.empty((sizes[1], sizes[2], sizes[5]), dtype=torch.float32, device=device)
+        size = _attention_workspace(*sizes, 0)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        args = _ATTENTION_ARGS.pack(*sizes, *inputs, *_fields(out), *lens, lse.data_ptr(), *_NO_TENSORS,
+                                    ptr(workspace) or 0, size)
+        check(lib().illumina_op_attention(args, handle))
     return out, lse
 
 
 def attentionBackward(dOut, q, k, v, out, lse, scale=None, causalBlock=0, qLens=None, kLens=None, stream=None):
     """Gradients (dq, dk, dv) of attention, from its results out and lse and the same masks."""
     import torch
-    args = _attention_args(torch, q, k, v, scale, causalBlock, qLens, kLens)
+    sizes, inputs, lens = _attention(torch, q, k, v, scale, causalBlock, qLens, kLens)
     for name, x in (("dOut", dOut), ("out", out)):
         _tensor(torch, name, x, q, 4)
-        _require(x.shape == q.shape, f"{name} must have the shape of q")
+        if x.shape != q.shape:
+            _require(False, f"{name} must have the shape of q")
+    device = q.device
     _require(lse is not None, "lse of the forward pass is needed")
-    _vector(torch, "lse", lse, q.shape[0] * q.shape[2] * q.shape[1], q.device)
-    with _On(torch, q.device, stream) as on:
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        args.lse = lse.data_ptr()
-        for slot, x in ((args.dout, dOut), (args.out, out), (args.dq, dq), (args.dk, dk), (args.dv, dv)):
-            _set(slot, x)
-        workspace = _workspace(torch, args, 1, q.device)  # noqa: F841 - alive until the launch is queued
-        check(lib().illumina_op_attention_backward(C.byref(args), on.handle))
+    lse_at = _vector(torch, "lse", lse, sizes[1] * sizes[2] * sizes[5], device)
+    with _On(torch, device, stream) as handle:
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        size = _attention_workspace(*sizes, 1)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        args = _ATTENTION_ARGS.pack(*sizes, *inputs, *_fields(out), *lens, lse_at, *_fields(dOut), *_fields(dq),
+                                    *_fields(dk), *_fields(dv), workspace.data_ptr(), size)
+        check(lib().illumina_op_attention_backward(args, handle))
     return dq, dk, dv

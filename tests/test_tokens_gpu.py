@@ -278,20 +278,22 @@ def test_attention_padding_rows_and_guards(torch, ops, dtype):
     want_out, want_lse = ops.attention(q, k, v, **masks)
     want = ops.attentionBackward(dout, q, k, v, want_out, want_lse, **masks)
     assert not want_out[1, 60:].any() and not want[0][1, 60:].any() and not want[1][1, 33:].any() and not want[2][1, 33:].any()
-    args = ops._attention_args(torch, q, k, v, None, 1, masks["qLens"], masks["kLens"])
 
     def guarded(like):
         big = torch.full((like.shape[0], like.shape[1] + 2, like.shape[2] + 1, 72), 7.0, dtype=like.dtype, device="cuda")
         return big, big[:, 1:-1, :-1, :64]
 
+    def field(x):
+        return _lib.AttentionTensor(x.data_ptr(), (C.c_longlong * 3)(*x.stride()[:3]))
+
     outs = {n: guarded(x) for n, x in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
-    args.lse = want_lse.data_ptr()
-    for n, (_, x) in outs.items():
-        ops._set(getattr(args, n), x)
-    ops._set(args.dout, dout)
-    keep = ops._workspace(torch, args, 0, q.device)  # noqa: F841
+    work = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    args = _lib.AttentionArgs(precision=q.dtype == torch.bfloat16, batch=2, heads=4, kv_heads=2, head_dim=64, q_tokens=130,
+                              k_tokens=140, causal_block=1, scale=64 ** -0.5, q=field(q), k=field(k), v=field(v),
+                              q_lens=masks["qLens"].data_ptr(), k_lens=masks["kLens"].data_ptr(), lse=want_lse.data_ptr(),
+                              dout=field(dout), workspace=work.data_ptr(), workspace_bytes=work.numel(),
+                              **{n: field(x) for n, (_, x) in outs.items()})
     _lib.check(_lib.lib().illumina_op_attention(C.byref(args), torch.cuda.current_stream().cuda_stream))
-    keep2 = ops._workspace(torch, args, 1, q.device)  # noqa: F841
     _lib.check(_lib.lib().illumina_op_attention_backward(C.byref(args), torch.cuda.current_stream().cuda_stream))
     for (n, (big, x)), w in zip(outs.items(), (want_out, *want)):
         assert torch.equal(x, w), n
