@@ -86,25 +86,50 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
 }
 constexpr uint32_t kBMnMajor = 1u << 16;
 
-// d[128][n] (+)= a(image rows)[128][nk * 16] * b(image rows)[n][nk * 16]'
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, int nk, uint32_t idesc) {
-  for (int k = 0; k < nk; k++) {
-    const uint32_t o = (k >> 2) * kImage + (k & 3) * 32;
-    mma_f16(d, smem_desc(a + o), smem_desc(b + o), idesc, k > 0);
+// The product warp runs these as a whole, with the instruction itself
+// predicated on its first lane: in code that diverged to one lane the compiler
+// moves every descriptor into uniform registers anew, which took about 90
+// cycles a product.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+// d[128][n] = a(image rows)[128][nk * 16] * b(image rows)[n][nk * 16]', with
+// a and b K-major descriptors of the tiles.
+template <int DP>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, int nk, uint32_t idesc, uint32_t lead) {
+#pragma unroll
+  for (int k = 0; k < DP / 16; k++) {
+    constexpr uint32_t image = kImage >> 4;
+    const uint32_t o = (k >> 2) * image + (k & 3) * 2;
+    if (k < nk) mma_ss(d, a + o, b + o, idesc, k > 0, lead);
   }
 }
-// d[128][n] (+)= a(TMEM, bf16 pairs)[128][128] * b(image)[128][n]; the second
-// half of a's columns begins `half` TMEM columns after the first.
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t half, uint32_t b, uint32_t idesc, bool first) {
+// d[128][n] (+)= a(TMEM, bf16 pairs)[128][128] * b(image)[128][n], with b an
+// MN-major descriptor; the second half of a's columns begins `half` TMEM
+// columns after the first.
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t half, uint64_t b, uint32_t idesc, bool first,
+                                         uint32_t lead) {
 #pragma unroll
-  for (int k = 0; k < 8; k++) {
-    const uint32_t at = a + (k >> 2) * half + (k & 3) * 8;
-    const uint32_t acc = first && k == 0 ? 0u : 1u;
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(at), "l"(desc_mn(b + k * 2048)), "r"(idesc), "r"(acc)
-        : "memory");
-  }
+  for (int k = 0; k < 8; k++)
+    mma_ts(d, a + (k >> 2) * half + (k & 3) * 8, b + k * 128, idesc, first && k == 0 ? 0u : 1u, lead);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -303,7 +328,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = max(0, issued_k - L::kStages); i < issued_k; i++) mbar_wait(k_full + i % L::kStages, (i / L::kStages) & 1);
       for (int i = max(0, issued_v - L::kStages); i < issued_v; i++) mbar_wait(v_full + i % L::kStages, (i / L::kStages) & 1);
     } else if (warp == kMmaWarp && t0 < most) {
-      const bool lead = (threadIdx.x & 31) == 0;
+      const uint32_t lead = (threadIdx.x & 31) == 0;
+      const uint64_t dq = smem_desc(smem_u32(sq)), dk = smem_desc(smem_u32(sk)), dv = desc_mn(smem_u32(sv));
+      constexpr uint32_t kStep = L::kTile >> 4;  // descriptors of the next tile
       const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
       const int nk = a.n16 / 16;
       bool ok = true;
@@ -312,14 +339,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (ok && t0 < t1[i]) ok = wait.warp(q_full + i, 0);
       ok = ok && wait.warp(k_full, 0);
       tc_fence_after();
-      if (ok && lead) {
+      if (ok) {
 #pragma unroll
         for (int i = 0; i < 2; i++)
           if (t0 < t1[i]) {
-            mma_rows(tmem + i * 128, smem_u32(sq + i * L::kTile), smem_u32(sk), nk, id_s);
-            mma_commit(s_full + i);
+            mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk, nk, id_s, lead);
+            commit(s_full + i, lead);
           }
-        mma_commit(k_empty);
+        commit(k_empty, lead);
       }
       for (int j = t0; j < most && ok; j++) {
         const int it = j - t0, s = it % L::kStages, s1 = (it + 1) % L::kStages;
@@ -334,26 +361,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ok = wait.warp(p_full + i, it & 1);
           if (!ok) continue;
           tc_fence_after();
-          if (lead) {
-            mma_tmem(tmem + 256 + i * DP, tmem + i * 128, 32, smem_u32(sv + s * L::kTile), id_o, j == t0);
-            mma_commit(o_full + i);
-          }
+          mma_tmem(tmem + 256 + i * DP, tmem + i * 128, 32, dv + s * kStep, id_o, j == t0, lead);
+          commit(o_full + i, lead);
           if (j + 1 < t1[i]) {
             if (!have_k) ok = wait.warp(k_full + s1, ((it + 1) / L::kStages) & 1);
             if (!ok) continue;
             have_k = true;
-            if (lead) {
-              mma_rows(tmem + i * 128, smem_u32(sq + i * L::kTile), smem_u32(sk + s1 * L::kTile), nk, id_s);
-              mma_commit(s_full + i);
-            }
+            mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk + s1 * kStep, nk, id_s, lead);
+            commit(s_full + i, lead);
           }
         }
         if (!ok) break;
-        if (lead) {
-          mma_commit(v_empty + s);
-          if (more) mma_commit(k_empty + s1);
-        }
-        __syncwarp();
+        commit(v_empty + s, lead);
+        if (more) commit(k_empty + s1, lead);
       }
     }
     __syncwarp();
@@ -563,7 +583,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_wait(kv_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
   } else if (warp == kMmaWarp && some) {
-    const bool lead = (threadIdx.x & 31) == 0;
+    const uint32_t lead = (threadIdx.x & 31) == 0;
+    const uint64_t dk = smem_desc(smem_u32(sk)), dv = smem_desc(smem_u32(sv)), dq = smem_desc(smem_u32(sq)),
+                   dg = smem_desc(smem_u32(sg)), dq_mn = desc_mn(smem_u32(sq)), dg_mn = desc_mn(smem_u32(sg));
+    constexpr uint32_t kStep = L::kTile >> 4;
     const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
     // query tile j is in shared memory, its padding cleared
@@ -579,44 +602,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       return true;
     };
     bool ok = wait.warp(kv_full, 0) && ready(t0);
-    if (ok && lead) {
-      mma_rows(t_s, smem_u32(sk), smem_u32(sq), nk, id_s);
-      mma_commit(s_full);
-      mma_rows(t_g, smem_u32(sv), smem_u32(sg), nk, id_s);
-      mma_commit(g_full);
+    if (ok) {
+      mma_rows<DP>(t_s, dk, dq, nk, id_s, lead);
+      commit(s_full, lead);
+      mma_rows<DP>(t_g, dv, dg, nk, id_s, lead);
+      commit(g_full, lead);
     }
-    __syncwarp();
     for (int j = t0; j < t1 && ok; j++) {
       const int it = j - t0, s = it % L::kStages, s1 = (it + 1) % L::kStages;
       const bool more = j + 1 < t1;
       ok = wait.warp(p_full, it & 1);
       if (!ok) break;
       tc_fence_after();
-      if (lead) mma_tmem(t_dv, t_s, 64, smem_u32(sg + s * L::kTile), id_o, it == 0);
-      __syncwarp();
+      mma_tmem(t_dv, t_s, 64, dg_mn + s * kStep, id_o, it == 0, lead);
       if (more) {
         ok = ready(j + 1);
         if (!ok) break;
-        if (lead) {
-          mma_rows(t_s, smem_u32(sk), smem_u32(sq + s1 * L::kTile), nk, id_s);
-          mma_commit(s_full);
-        }
-        __syncwarp();
+        mma_rows<DP>(t_s, dk, dq + s1 * kStep, nk, id_s, lead);
+        commit(s_full, lead);
       }
       ok = wait.warp(d_full, it & 1);
       if (!ok) break;
       tc_fence_after();
-      if (lead) {
-        mma_tmem(t_dk, t_g, 64, smem_u32(sq + s * L::kTile), id_o, it == 0);
-        mma_commit(empty + s);
-        if (more) {
-          mma_rows(t_g, smem_u32(sv), smem_u32(sg + s1 * L::kTile), nk, id_s);
-          mma_commit(g_full);
-        } else {
-          mma_commit(done);
-        }
+      mma_tmem(t_dk, t_g, 64, dq_mn + s * kStep, id_o, it == 0, lead);
+      commit(empty + s, lead);
+      if (more) {
+        mma_rows<DP>(t_g, dv, dg + s1 * kStep, nk, id_s, lead);
+        commit(g_full, lead);
+      } else {
+        commit(done, lead);
       }
-      __syncwarp();
     }
   } else if (warp < kProducerWarp) {
     const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
@@ -627,8 +642,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const float sl2 = p.scale * kLog2e;
     float *mine_lse = row_sums + warp * 128, *mine_delta = mine_lse + 64;
     const float2 scale2 = make_float2(sl2, sl2);
-    // -lse (base 2; -inf where the row has no probabilities) and delta of the
-    // two columns this lane fetches of query tile j
+    // lse and delta of the two columns this lane fetches of query tile j, as
+    // they come: nothing waits for them until the next tile begins
     float nl[2], nd[2];
     auto fetch = [&](int j) {
 #pragma unroll
@@ -638,8 +653,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         nl[k] = -INFINITY, nd[k] = 0;
         if (r < a.group * a.tpt && token < mask.q_len) {
           const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
-          const float v = p.lse[at];
-          nl[k] = v == -INFINITY ? -INFINITY : -v * kLog2e;
+          nl[k] = p.lse[at];
           nd[k] = p.ws[at];
         }
       }
@@ -650,7 +664,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int it = j - t0;
       __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 2; k++) mine_lse[k * 32 + lane] = nl[k], mine_delta[k * 32 + lane] = -nd[k];
+      for (int k = 0; k < 2; k++) {
+        // exponent's shift in base 2; a row without probabilities (lse -inf) gets none here either
+        mine_lse[k * 32 + lane] = nl[k] == -INFINITY ? -INFINITY : -nl[k] * kLog2e;
+        mine_delta[k * 32 + lane] = -nd[k];
+      }
       __syncwarp();
       // probabilities are NaN where a row's lse is, and nowhere else
       const bool spoiled = __any_sync(0xffffffffu, nl[0] != nl[0] || nl[1] != nl[1]);
@@ -807,7 +825,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_wait(q_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
   } else if (warp == kMmaWarp && t1 > 0) {
-    const bool lead = (threadIdx.x & 31) == 0;
+    const uint32_t lead = (threadIdx.x & 31) == 0;
+    const uint64_t dq = smem_desc(smem_u32(sq)), dg = smem_desc(smem_u32(sg)), dk = smem_desc(smem_u32(sk)),
+                   dv = smem_desc(smem_u32(sv)), dk_mn = desc_mn(smem_u32(sk));
+    constexpr uint32_t kStep = L::kTile >> 4;
     const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
     auto ready = [&](int j) {
@@ -818,39 +839,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       return true;
     };
     bool ok = wait.warp(q_full, 0) && ready(0);
-    if (ok && lead) {
-      mma_rows(t_s, smem_u32(sq), smem_u32(sk), nk, id_s);
-      mma_commit(s_full);
-      mma_rows(t_g, smem_u32(sg), smem_u32(sv), nk, id_s);
-      mma_commit(g_full);
+    if (ok) {
+      mma_rows<DP>(t_s, dq, dk, nk, id_s, lead);
+      commit(s_full, lead);
+      mma_rows<DP>(t_g, dg, dv, nk, id_s, lead);
+      commit(g_full, lead);
     }
-    __syncwarp();
     for (int j = 0; j < t1 && ok; j++) {
       const int s = j % L::kStages, s1 = (j + 1) % L::kStages;
       const bool more = j + 1 < t1;
       if (more) {
         ok = wait.warp(s_free, j & 1) && ready(j + 1);
         if (!ok) break;
-        if (lead) {
-          mma_rows(t_s, smem_u32(sq), smem_u32(sk + s1 * L::kTile), nk, id_s);
-          mma_commit(s_full);
-        }
-        __syncwarp();
+        mma_rows<DP>(t_s, dq, dk + s1 * kStep, nk, id_s, lead);
+        commit(s_full, lead);
       }
       ok = wait.warp(d_full, j & 1);
       if (!ok) break;
       tc_fence_after();
-      if (lead) {
-        mma_tmem(t_dq, t_g, 64, smem_u32(sk + s * L::kTile), id_o, j == 0);
-        mma_commit(empty + s);
-        if (more) {
-          mma_rows(t_g, smem_u32(sg), smem_u32(sv + s1 * L::kTile), nk, id_s);
-          mma_commit(g_full);
-        } else {
-          mma_commit(done);
-        }
+      mma_tmem(t_dq, t_g, 64, dk_mn + s * kStep, id_o, j == 0, lead);
+      commit(empty + s, lead);
+      if (more) {
+        mma_rows<DP>(t_g, dg, dv + s1 * kStep, nk, id_s, lead);
+        commit(g_full, lead);
+      } else {
+        commit(done, lead);
       }
-      __syncwarp();
     }
   } else if (warp < kProducerWarp) {
     const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
