@@ -86,51 +86,48 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
 }
 constexpr uint32_t kBMnMajor = 1u << 16;
 
-// The product warp runs these as a whole, with the instruction itself
-// predicated on its first lane: in code that diverged to one lane the compiler
-// moves every descriptor into uniform registers anew, which took about 90
-// cycles a product.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+// Products are issued by one thread, chosen by elect.sync: behind its answer
+// the compiler keeps descriptors in uniform registers. An issue then takes 31
+// cycles (64-column accumulator, operand in TMEM: the tensor core's own rate),
+// 47 (64 columns from shared memory, whose bandwidth bounds it) or 63 (128
+// columns); behind a comparison of the thread index 44, 48 and 63, and with
+// the instruction predicated in converged code 67 to 72.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t *bar, uint32_t lead) {
-  asm volatile(
-      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
-      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
-      "r"(lead)
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
 // d[128][n] = a(image rows)[128][nk * 16] * b(image rows)[n][nk * 16]', with
 // a and b K-major descriptors of the tiles.
 template <int DP>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, int nk, uint32_t idesc, uint32_t lead) {
+__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, int nk, uint32_t idesc) {
 #pragma unroll
   for (int k = 0; k < DP / 16; k++) {
     constexpr uint32_t image = kImage >> 4;
     const uint32_t o = (k >> 2) * image + (k & 3) * 2;
-    if (k < nk) mma_ss(d, a + o, b + o, idesc, k > 0, lead);
+    if (k < nk) mma_ss(d, a + o, b + o, idesc, k > 0);
   }
 }
-// d[128][n] (+)= a(TMEM, bf16 pairs)[128][128] * b(image)[128][n], with b an
-// MN-major descriptor; the second half of a's columns begins `half` TMEM
-// columns after the first.
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t half, uint64_t b, uint32_t idesc, bool first,
-                                         uint32_t lead) {
+// d[128][n] (+)= a(TMEM, bf16 pairs)[128][K] * b(image)[K][n], with b an
+// MN-major descriptor.
+template <int K>
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool first) {
 #pragma unroll
-  for (int k = 0; k < 8; k++)
-    mma_ts(d, a + (k >> 2) * half + (k & 3) * 8, b + k * 128, idesc, first && k == 0 ? 0u : 1u, lead);
+  for (int k = 0; k < K / 16; k++) mma_ts(d, a + k * 8, b + k * 128, idesc, first && k == 0 ? 0u : 1u);
 }
+constexpr uint32_t kHalfRows = 64 * 128 >> 4;  // descriptor step from row 0 to row 64 of an image
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -210,9 +207,12 @@ __device__ __forceinline__ void store_zeros(bf16 *dst, int n) {
 // The end of every kernel: copies and products of a CTA that gave up are
 // drained, then TMEM is freed.
 __device__ __forceinline__ void leave(uint32_t tmem, int warp, volatile int *fail, uint64_t *drain, int *err) {
-  if (warp == kMmaWarp && (threadIdx.x & 31) == 0) {
-    mma_commit(drain);
-    mbar_wait(drain, 0);
+  if (warp == kMmaWarp) {
+    if (elect_one()) {  // the thread that issued the products
+      mma_commit(drain);
+      mbar_wait(drain, 0);
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = max(0, issued_k - L::kStages); i < issued_k; i++) mbar_wait(k_full + i % L::kStages, (i / L::kStages) & 1);
       for (int i = max(0, issued_v - L::kStages); i < issued_v; i++) mbar_wait(v_full + i % L::kStages, (i / L::kStages) & 1);
     } else if (warp == kMmaWarp && t0 < most) {
-      const uint32_t lead = (threadIdx.x & 31) == 0;
+      const bool lead = elect_one();
       const uint64_t dq = smem_desc(smem_u32(sq)), dk = smem_desc(smem_u32(sk)), dv = desc_mn(smem_u32(sv));
       constexpr uint32_t kStep = L::kTile >> 4;  // descriptors of the next tile
       const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
@@ -339,15 +339,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (ok && t0 < t1[i]) ok = wait.warp(q_full + i, 0);
       ok = ok && wait.warp(k_full, 0);
       tc_fence_after();
-      if (ok) {
+      if (ok && lead) {
 #pragma unroll
         for (int i = 0; i < 2; i++)
           if (t0 < t1[i]) {
-            mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk, nk, id_s, lead);
-            commit(s_full + i, lead);
+            mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk, nk, id_s);
+            mma_commit(s_full + i);
           }
-        commit(k_empty, lead);
+        mma_commit(k_empty);
       }
+      __syncwarp();
       for (int j = t0; j < most && ok; j++) {
         const int it = j - t0, s = it % L::kStages, s1 = (it + 1) % L::kStages;
         ok = wait.warp(v_full + s, (it / L::kStages) & 1);
@@ -361,19 +362,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ok = wait.warp(p_full + i, it & 1);
           if (!ok) continue;
           tc_fence_after();
-          mma_tmem(tmem + 256 + i * DP, tmem + i * 128, 32, dv + s * kStep, id_o, j == t0, lead);
-          commit(o_full + i, lead);
+          if (lead) {
+            mma_tmem<128>(tmem + 256 + i * DP, tmem + i * 128, dv + s * kStep, id_o, j == t0);
+            mma_commit(o_full + i);
+          }
           if (j + 1 < t1[i]) {
             if (!have_k) ok = wait.warp(k_full + s1, ((it + 1) / L::kStages) & 1);
             if (!ok) continue;
             have_k = true;
-            mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk + s1 * kStep, nk, id_s, lead);
-            commit(s_full + i, lead);
+            if (lead) {
+              mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk + s1 * kStep, nk, id_s);
+              mma_commit(s_full + i);
+            }
           }
         }
         if (!ok) break;
-        commit(v_empty + s, lead);
-        if (more) commit(k_empty + s1, lead);
+        if (lead) {
+          mma_commit(v_empty + s);
+          if (more) mma_commit(k_empty + s1);
+        }
+        __syncwarp();
       }
     }
     __syncwarp();
@@ -509,10 +517,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // ---------------------------------------------------------------------------
 // Backward, dK and dV: one key tile (its rows are the TMEM lanes) past the
 // query tiles that see it. Per query tile: S' = K Q', dP' = V dO', and from
-// TMEM dV += P' dO, dK += dS' Q. The products of one tile run while the other
-// phase's arithmetic does: dP' under the exponentials, dV and the next S'
-// under dS, dK under the next exponentials. The two warpgroups take 64 query
-// columns each.
+// TMEM dV += P' dO, dK += dS' Q. The two warpgroups take 64 query columns
+// each, as two pipelines of their own that the product warp serves in turn:
+//   P0(j): dV, S0(j+1)   dS0(j): dK, dP0(j+1)   P1(j): dV, S1(j+1)   dS1(j): dK, dP1(j+1)
+// so that they run half a tile apart: one is in its exponentials while the
+// other is in its products and differences, and a warpgroup finds its next
+// operands ready. The order of the sums is fixed.
 // ---------------------------------------------------------------------------
 
 template <int DP>
@@ -534,9 +544,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t *sk = base, *sv = sk + L::kTile, *sq = sv + L::kTile, *sg = sq + L::kStages * L::kTile;
   float *row_sums = reinterpret_cast<float *>(sg + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sg + L::kStages * L::kTile + L::kRowSums);
-  uint64_t *kv_full = bars, *s_full = bars + 1, *g_full = bars + 2, *p_full = bars + 3, *d_full = bars + 4,
-           *done = bars + 5, *drain = bars + 6, *full = bars + 7, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 7 + 2 * L::kStages);
+  uint64_t *kv_full = bars, *s_full = bars + 1, *g_full = bars + 3, *p_full = bars + 5, *d_full = bars + 7,
+           *done = bars + 9, *drain = bars + 10, *full = bars + 11, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 11 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5;
 
@@ -552,7 +562,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 7; b++) mbar_init(b, b == p_full || b == d_full ? 8 : 1);
+    for (uint64_t *b = bars; b < bars + 11; b++) mbar_init(b, b >= p_full && b < done ? 4 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
@@ -583,11 +593,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_wait(kv_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
   } else if (warp == kMmaWarp && some) {
-    const uint32_t lead = (threadIdx.x & 31) == 0;
+    const bool lead = elect_one();
     const uint64_t dk = smem_desc(smem_u32(sk)), dv = smem_desc(smem_u32(sv)), dq = smem_desc(smem_u32(sq)),
                    dg = smem_desc(smem_u32(sg)), dq_mn = desc_mn(smem_u32(sq)), dg_mn = desc_mn(smem_u32(sg));
     constexpr uint32_t kStep = L::kTile >> 4;
-    const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
+    const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
     // query tile j is in shared memory, its padding cleared
     auto ready = [&](int j) {
@@ -602,37 +612,49 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       return true;
     };
     bool ok = wait.warp(kv_full, 0) && ready(t0);
-    if (ok) {
-      mma_rows<DP>(t_s, dk, dq, nk, id_s, lead);
-      commit(s_full, lead);
-      mma_rows<DP>(t_g, dv, dg, nk, id_s, lead);
-      commit(g_full, lead);
+    if (ok && lead) {
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        mma_rows<DP>(t_s + w * 64, dk, dq + w * kHalfRows, nk, id_s);
+        mma_commit(s_full + w);
+        mma_rows<DP>(t_g + w * 64, dv, dg + w * kHalfRows, nk, id_s);
+        mma_commit(g_full + w);
+      }
     }
+    __syncwarp();
     for (int j = t0; j < t1 && ok; j++) {
       const int it = j - t0, s = it % L::kStages, s1 = (it + 1) % L::kStages;
       const bool more = j + 1 < t1;
-      ok = wait.warp(p_full, it & 1);
-      if (!ok) break;
-      tc_fence_after();
-      mma_tmem(t_dv, t_s, 64, dg_mn + s * kStep, id_o, it == 0, lead);
-      if (more) {
-        ok = ready(j + 1);
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        ok = ok && wait.warp(p_full + w, it & 1);
         if (!ok) break;
-        mma_rows<DP>(t_s, dk, dq + s1 * kStep, nk, id_s, lead);
-        commit(s_full, lead);
-      }
-      ok = wait.warp(d_full, it & 1);
-      if (!ok) break;
-      tc_fence_after();
-      mma_tmem(t_dk, t_g, 64, dq_mn + s * kStep, id_o, it == 0, lead);
-      commit(empty + s, lead);
-      if (more) {
-        mma_rows<DP>(t_g, dv, dg + s1 * kStep, nk, id_s, lead);
-        commit(g_full, lead);
-      } else {
-        commit(done, lead);
+        tc_fence_after();
+        if (lead) mma_tmem<64>(t_dv, t_s + w * 64, dg_mn + s * kStep + w * kHalfRows, id_o, it == 0 && w == 0);
+        if (more) {
+          if (w == 0) ok = ready(j + 1);
+          if (!ok) break;
+          if (lead) {
+            mma_rows<DP>(t_s + w * 64, dk, dq + s1 * kStep + w * kHalfRows, nk, id_s);
+            mma_commit(s_full + w);
+          }
+        }
+        ok = wait.warp(d_full + w, it & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lead) {
+          mma_tmem<64>(t_dk, t_g + w * 64, dq_mn + s * kStep + w * kHalfRows, id_o, it == 0 && w == 0);
+          if (w == 1) mma_commit(empty + s);
+          if (more) {
+            mma_rows<DP>(t_g + w * 64, dv, dg + s1 * kStep + w * kHalfRows, nk, id_s);
+            mma_commit(g_full + w);
+          }
+        }
+        __syncwarp();
       }
     }
+    if (ok && lead) mma_commit(done);
+    __syncwarp();
   } else if (warp < kProducerWarp) {
     const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
@@ -645,16 +667,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // lse and delta of the two columns this lane fetches of query tile j, as
     // they come: nothing waits for them until the next tile begins
     float nl[2], nd[2];
+    int column[2];          // token within a query tile
+    const float *lse_of[2], *delta_of[2];  // of its head
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int r = wg * 64 + k * 32 + lane;
+      column[k] = r < a.group * a.tpt ? r / a.group : INT_MAX / 2;
+      const long long at = ((long long)n * p.heads + hk * a.group + r % a.group) * p.q_tokens;
+      lse_of[k] = p.lse + at, delta_of[k] = p.ws + at;
+    }
     auto fetch = [&](int j) {
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        const int r = wg * 64 + k * 32 + lane;
-        const int token = j * a.tpt + r / a.group, h = hk * a.group + r % a.group;
+        const int token = j * a.tpt + column[k];
         nl[k] = -INFINITY, nd[k] = 0;
-        if (r < a.group * a.tpt && token < mask.q_len) {
-          const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
-          nl[k] = p.lse[at];
-          nd[k] = p.ws[at];
+        if (token < mask.q_len) {
+          nl[k] = lse_of[k][token];
+          nd[k] = delta_of[k][token];
         }
       }
     };
@@ -674,10 +703,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool spoiled = __any_sync(0xffffffffu, nl[0] != nl[0] || nl[1] != nl[1]);
       if (j + 1 < t1) fetch(j + 1);
       // columns below `skip` are queries that do not see this key
-      const long long skip_ll = ((long long)begin - (long long)j * a.tpt) * a.group - wg * 64;
-      const int skip = (int)min(max(skip_ll, 0ll), 64ll);
+      const int skip = min(max(min(max(begin - j * a.tpt, 0), 128) * a.group - wg * 64, 0), 64);
       const bool masked = __any_sync(0xffffffffu, skip > 0);
-      ok = wait.warp(s_full, it & 1);
+      ok = wait.warp(s_full + wg, it & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t r[64];
@@ -709,8 +737,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-      ok = wait.warp(g_full, it & 1);
+      if (lane == 0) mbar_arrive(p_full + wg);
+      ok = wait.warp(g_full + wg, it & 1);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
@@ -740,7 +768,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(d_full);
+      if (lane == 0) mbar_arrive(d_full + wg);
     }
     if (some && ok) ok = wait.warp(done, 0);
     tc_fence_after();
@@ -765,7 +793,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // ---------------------------------------------------------------------------
 // Backward, dQ: one query tile past the key tiles it sees. S = Q K' and
 // dP = dO V' are recomputed, dQ += dS K from TMEM. The warpgroups take 64 key
-// columns each; a thread's lse and delta stay in registers. This pass runs
+// columns each, as two pipelines half a tile apart (as above); a thread's lse and delta stay in registers. This pass runs
 // first and leaves the row sums delta in the workspace for the other.
 // ---------------------------------------------------------------------------
 
@@ -780,9 +808,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t *sq = base, *sg = sq + L::kTile, *sk = sg + L::kTile, *sv = sk + L::kStages * L::kTile;
   float *row_sums = reinterpret_cast<float *>(sv + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile + L::kRowSums);
-  uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 2, *s_free = bars + 3, *d_full = bars + 4,
-           *done = bars + 5, *drain = bars + 6, *full = bars + 7, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 7 + 2 * L::kStages);
+  uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 3, *s_free = bars + 5, *d_full = bars + 7,
+           *done = bars + 9, *drain = bars + 10, *full = bars + 11, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 11 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5;
 
@@ -797,7 +825,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 7; b++) mbar_init(b, b == s_free || b == d_full ? 8 : 1);
+    for (uint64_t *b = bars; b < bars + 11; b++) mbar_init(b, b >= s_free && b < done ? 4 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
@@ -825,11 +853,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_wait(q_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
   } else if (warp == kMmaWarp && t1 > 0) {
-    const uint32_t lead = (threadIdx.x & 31) == 0;
+    const bool lead = elect_one();
     const uint64_t dq = smem_desc(smem_u32(sq)), dg = smem_desc(smem_u32(sg)), dk = smem_desc(smem_u32(sk)),
                    dv = smem_desc(smem_u32(sv)), dk_mn = desc_mn(smem_u32(sk));
     constexpr uint32_t kStep = L::kTile >> 4;
-    const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
+    const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
     auto ready = [&](int j) {
       const int s = j % L::kStages;
@@ -839,33 +867,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       return true;
     };
     bool ok = wait.warp(q_full, 0) && ready(0);
-    if (ok) {
-      mma_rows<DP>(t_s, dq, dk, nk, id_s, lead);
-      commit(s_full, lead);
-      mma_rows<DP>(t_g, dg, dv, nk, id_s, lead);
-      commit(g_full, lead);
+    if (ok && lead) {
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        mma_rows<DP>(t_s + w * 64, dq, dk + w * kHalfRows, nk, id_s);
+        mma_commit(s_full + w);
+        mma_rows<DP>(t_g + w * 64, dg, dv + w * kHalfRows, nk, id_s);
+        mma_commit(g_full + w);
+      }
     }
+    __syncwarp();
     for (int j = 0; j < t1 && ok; j++) {
       const int s = j % L::kStages, s1 = (j + 1) % L::kStages;
       const bool more = j + 1 < t1;
-      if (more) {
-        ok = wait.warp(s_free, j & 1) && ready(j + 1);
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        if (more) {
+          ok = ok && wait.warp(s_free + w, j & 1);
+          if (ok && w == 0) ok = ready(j + 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (lead) {
+            mma_rows<DP>(t_s + w * 64, dq, dk + s1 * kStep + w * kHalfRows, nk, id_s);
+            mma_commit(s_full + w);
+          }
+        }
+        ok = wait.warp(d_full + w, j & 1);
         if (!ok) break;
-        mma_rows<DP>(t_s, dq, dk + s1 * kStep, nk, id_s, lead);
-        commit(s_full, lead);
-      }
-      ok = wait.warp(d_full, j & 1);
-      if (!ok) break;
-      tc_fence_after();
-      mma_tmem(t_dq, t_g, 64, dk_mn + s * kStep, id_o, j == 0, lead);
-      commit(empty + s, lead);
-      if (more) {
-        mma_rows<DP>(t_g, dg, dv + s1 * kStep, nk, id_s, lead);
-        commit(g_full, lead);
-      } else {
-        commit(done, lead);
+        tc_fence_after();
+        if (lead) {
+          mma_tmem<64>(t_dq, t_g + w * 64, dk_mn + s * kStep + w * kHalfRows, id_o, j == 0 && w == 0);
+          if (w == 1) mma_commit(empty + s);
+          if (more) {
+            mma_rows<DP>(t_g + w * 64, dg, dv + s1 * kStep + w * kHalfRows, nk, id_s);
+            mma_commit(g_full + w);
+          }
+        }
+        __syncwarp();
       }
     }
+    if (ok && lead) mma_commit(done);
+    __syncwarp();
   } else if (warp < kProducerWarp) {
     const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
@@ -901,7 +943,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int j = 0; j < t1; j++) {
       const int left = end - j * 128 - wg * 64;
       const bool masked = __any_sync(0xffffffffu, left < 64);
-      ok = wait.warp(s_full, j & 1);
+      ok = wait.warp(s_full + wg, j & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t r[64];
@@ -910,13 +952,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_free);
+      if (lane == 0) mbar_arrive(s_free + wg);
 #pragma unroll
       for (int c = 0; c < 64; c += 2) {
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, shift2);
         r[c] = __float_as_uint(ex2(x.x)), r[c + 1] = __float_as_uint(ex2(x.y));
       }
-      ok = wait.warp(g_full, j & 1);
+      ok = wait.warp(g_full + wg, j & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t q[32];
@@ -940,7 +982,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(d_full);
+      if (lane == 0) mbar_arrive(d_full + wg);
     }
     if (t1 > 0 && ok) ok = wait.warp(done, 0);
     tc_fence_after();

@@ -57,7 +57,7 @@ gpu::AttnParams attn_params(const illumina_attention_args *a, bool backward, boo
   require(a->kv_heads > 0 ? a->heads % a->kv_heads == 0 : a->heads == 0,
           "attention: heads must be a multiple of kv_heads");
   require(a->head_dim >= 1 && a->head_dim <= 128, "attention: head_dim outside [1, 128]");
-  require(a->q_tokens <= (1 << 30) && a->k_tokens <= (1 << 30), "attention: more than 2^30 tokens");
+  require(a->q_tokens <= (1 << 28) && a->k_tokens <= (1 << 28), "attention: more than 2^28 tokens");
   require(a->causal_block >= 0, "attention: negative causal_block");
   const double rows = (double)a->batch * a->heads * ((double)a->q_tokens + 32) / 32;
   const double keys = (double)a->batch * a->kv_heads * ((double)a->k_tokens + 32) / 32;

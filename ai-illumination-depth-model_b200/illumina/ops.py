@@ -341,7 +341,7 @@ def _attention(torch, q, k, v, scale, causalBlock, qLens, kLens):
     if hk < 1 or h % hk:
         _require(False, "q's heads must be a multiple of the key heads")
     _require(1 <= d <= 128, "head sizes from 1 to 128 are supported")
-    _require(max(b, h, tq, tk) < 2 ** 30, "attention: size beyond 2^30")
+    _require(max(b, h, tq, tk) <= 2 ** 28, "attention: size beyond 2^28")
     _require(isinstance(causalBlock, int) and 0 <= causalBlock < 2 ** 31, "causalBlock must be a token count, 0 for none")
     device = q.device
     lens = (_vector(torch, "qLens", qLens, b, device, torch.int32) or 0,
