@@ -16,12 +16,15 @@
 // read once for all of them, and a single token's heads fill one tile.
 //
 // Warps: two warpgroups compute (one TMEM lane, that is one row, a thread, so
-// a row's maximum and sum need no shuffles), one warp issues the copies, one
-// the products. All waits are on mbarriers and bounded.
+// a row's maximum and sum need no shuffles), one thread issues the copies, one
+// the products. All waits are on mbarriers and bounded. The product thread's
+// loops are kept rolled: its instructions run seldom, between the long bodies
+// of the computing warps, and every fetch that misses the instruction cache
+// delays both pipelines.
 //
 // Rows of padding inside the last tile may hold NaN: where such rows are a
 // contraction index (V; K in dQ; Q and dO in dK, dV), 0 * NaN would spoil the
-// sum, so the product warp clears them in shared memory first.
+// sum, so another warp clears them in shared memory first.
 #include "attention.cuh"
 #include "kernels.h"
 #include "tc_common.cuh"
@@ -42,7 +45,7 @@ using tok::allow_smem;
 using tok::bf16;
 
 constexpr int kTcThreads = 384;
-constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kClearWarp = 10;
 constexpr uint32_t kImage = 128 * 128;  // 128 rows x 64 bf16 columns
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -187,6 +190,12 @@ __device__ __forceinline__ void clear_rows(uint8_t *tile, int boxes, int from) {
   __syncwarp();
 }
 
+// The product thread has the tile that holds padding and asks for its clearing.
+__device__ __forceinline__ bool cleared(const Waiter &wait, uint64_t *ask, uint64_t *clean) {
+  mbar_arrive(ask);
+  return wait(clean, 0);
+}
+
 // Writes n (a multiple of 8, at most 32) values as bf16, times f.
 __device__ __forceinline__ void store_bf16(bf16 *dst, const uint32_t *r, int n, float f) {
 #pragma unroll
@@ -207,6 +216,7 @@ __device__ __forceinline__ void store_zeros(bf16 *dst, int n) {
 // The end of every kernel: copies and products of a CTA that gave up are
 // drained, then TMEM is freed.
 __device__ __forceinline__ void leave(uint32_t tmem, int warp, volatile int *fail, uint64_t *drain, int *err) {
+  __syncwarp();
   if (warp == kMmaWarp) {
     if (elect_one()) {  // the thread that issued the products
       mma_commit(drain);
@@ -252,9 +262,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t *sq = base, *sk = sq + 2 * L::kTile, *sv = sk + L::kStages * L::kTile;
   uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile);
   uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 4, *o_full = bars + 6, *drain = bars + 8,
-           *k_full = bars + 9, *k_empty = k_full + L::kStages, *v_full = k_empty + L::kStages,
+           *ask = bars + 9, *clean = bars + 10, *k_full = bars + 11, *k_empty = k_full + L::kStages, *v_full = k_empty + L::kStages,
            *v_empty = v_full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 9 + 4 * L::kStages);
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 11 + 4 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5;
 
@@ -283,11 +293,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
   for (int i = 0; i < 2; i++) t1[i] = min(t1[i], t0 + per);
   most = max(t1[0], t1[1]);
+  const int clear_at = mask.k_len % 128 ? mask.k_len / 128 : INT_MAX;  // the value tile that holds padding
 
   if (threadIdx.x == 0) {
     *fail = 0;
     for (int i = 0; i < 2; i++) mbar_init(q_full + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1);
     mbar_init(drain, 1);
+    mbar_init(ask, 1);
+    mbar_init(clean, 1);
     for (int i = 0; i < L::kStages; i++)
       mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
     fence_barrier_init();
@@ -327,61 +340,52 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (queries >> i & 1) mbar_wait(q_full + i, 0);
       for (int i = max(0, issued_k - L::kStages); i < issued_k; i++) mbar_wait(k_full + i % L::kStages, (i / L::kStages) & 1);
       for (int i = max(0, issued_v - L::kStages); i < issued_v; i++) mbar_wait(v_full + i % L::kStages, (i / L::kStages) & 1);
-    } else if (warp == kMmaWarp && t0 < most) {
-      const bool lead = elect_one();
+    } else if (warp == kClearWarp && clear_at < most && clear_at >= t0) {
+      const int it = clear_at - t0, s = it % L::kStages;
+      if (wait.warp(ask, 0) && wait.warp(v_full + s, (it / L::kStages) & 1)) {
+        clear_rows(sv + s * L::kTile, L::kBoxes, mask.k_len - clear_at * 128);
+        if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
+      }
+    } else if (warp == kMmaWarp && t0 < most && elect_one()) {
       const uint64_t dq = smem_desc(smem_u32(sq)), dk = smem_desc(smem_u32(sk)), dv = desc_mn(smem_u32(sv));
       constexpr uint32_t kStep = L::kTile >> 4;  // descriptors of the next tile
       const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
       const int nk = a.n16 / 16;
-      bool ok = true;
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-        if (ok && t0 < t1[i]) ok = wait.warp(q_full + i, 0);
-      ok = ok && wait.warp(k_full, 0);
-      tc_fence_after();
-      if (ok && lead) {
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-          if (t0 < t1[i]) {
-            mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk, nk, id_s);
+      const int end0 = t1[0], end1 = t1[1];
+      bool ok = wait(k_full, 0);
+#pragma unroll 1
+      for (int i = 0; i < 2; i++) {
+        if (t0 >= (i ? end1 : end0)) continue;
+        ok = ok && wait(q_full + i, 0);
+        if (!ok) break;
+        mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk, nk, id_s);
+        mma_commit(s_full + i);
+      }
+      if (ok) mma_commit(k_empty);
+      int s = 0, turn = 0;  // stage of tile j, parity of its use
+      for (int j = t0; j < most && ok; j++) {
+        const int s1 = s + 1 == L::kStages ? 0 : s + 1, turn1 = s1 ? turn : turn ^ 1, parity = (j - t0) & 1;
+        const bool more = j + 1 < most;
+        ok = wait(v_full + s, turn) && (j != clear_at || cleared(wait, ask, clean)) && (!more || wait(k_full + s1, turn1));
+        if (!ok) break;
+#pragma unroll 1
+        for (int i = 0; i < 2; i++) {
+          const int end = i ? end1 : end0;
+          if (j >= end) continue;
+          ok = wait(p_full + i, parity);
+          if (!ok) break;
+          tc_fence_after();
+          mma_tmem<128>(tmem + 256 + i * DP, tmem + i * 128, dv + s * kStep, id_o, j == t0);
+          mma_commit(o_full + i);
+          if (j + 1 < end) {
+            mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk + s1 * kStep, nk, id_s);
             mma_commit(s_full + i);
           }
-        mma_commit(k_empty);
-      }
-      __syncwarp();
-      for (int j = t0; j < most && ok; j++) {
-        const int it = j - t0, s = it % L::kStages, s1 = (it + 1) % L::kStages;
-        ok = wait.warp(v_full + s, (it / L::kStages) & 1);
-        if (!ok) break;
-        if ((j + 1) * 128 > mask.k_len) clear_rows(sv + s * L::kTile, L::kBoxes, mask.k_len - j * 128);
-        const bool more = j + 1 < most;
-        bool have_k = false;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          if (j >= t1[i] || !ok) continue;
-          ok = wait.warp(p_full + i, it & 1);
-          if (!ok) continue;
-          tc_fence_after();
-          if (lead) {
-            mma_tmem<128>(tmem + 256 + i * DP, tmem + i * 128, dv + s * kStep, id_o, j == t0);
-            mma_commit(o_full + i);
-          }
-          if (j + 1 < t1[i]) {
-            if (!have_k) ok = wait.warp(k_full + s1, ((it + 1) / L::kStages) & 1);
-            if (!ok) continue;
-            have_k = true;
-            if (lead) {
-              mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk + s1 * kStep, nk, id_s);
-              mma_commit(s_full + i);
-            }
-          }
         }
         if (!ok) break;
-        if (lead) {
-          mma_commit(v_empty + s);
-          if (more) mma_commit(k_empty + s1);
-        }
-        __syncwarp();
+        mma_commit(v_empty + s);
+        if (more) mma_commit(k_empty + s1);
+        s = s1, turn = turn1;
       }
     }
     __syncwarp();
@@ -545,8 +549,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   float *row_sums = reinterpret_cast<float *>(sg + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sg + L::kStages * L::kTile + L::kRowSums);
   uint64_t *kv_full = bars, *s_full = bars + 1, *g_full = bars + 3, *p_full = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *full = bars + 11, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 11 + 2 * L::kStages);
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *full = bars + 13, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 13 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5;
 
@@ -559,10 +563,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int t0 = key0 < mask.k_len ? mask.row_begin(key0) / a.tpt : 0;
   const int t1 = key0 < mask.k_len ? (mask.q_len + a.tpt - 1) / a.tpt : 0;
   const bool some = t0 < t1;
+  const int clear_at = mask.q_len % a.tpt ? mask.q_len / a.tpt : INT_MAX;  // the query tile that holds padding
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 11; b++) mbar_init(b, b >= p_full && b < done ? 4 : 1);
+    for (uint64_t *b = bars; b < bars + 13; b++) mbar_init(b, b >= p_full && b < done ? 4 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
@@ -592,69 +597,56 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     mbar_wait(kv_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
-  } else if (warp == kMmaWarp && some) {
-    const bool lead = elect_one();
+  } else if (warp == kClearWarp && clear_at < t1 && clear_at >= t0) {
+    const int it = clear_at - t0, s = it % L::kStages, from = (mask.q_len - clear_at * a.tpt) * a.group;
+    if (wait.warp(ask, 0) && wait.warp(full + s, (it / L::kStages) & 1)) {
+      clear_rows(sq + s * L::kTile, L::kBoxes, from);
+      clear_rows(sg + s * L::kTile, L::kBoxes, from);
+      if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
+    }
+  } else if (warp == kMmaWarp && some && elect_one()) {
     const uint64_t dk = smem_desc(smem_u32(sk)), dv = smem_desc(smem_u32(sv)), dq = smem_desc(smem_u32(sq)),
                    dg = smem_desc(smem_u32(sg)), dq_mn = desc_mn(smem_u32(sq)), dg_mn = desc_mn(smem_u32(sg));
     constexpr uint32_t kStep = L::kTile >> 4;
     const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
-    // query tile j is in shared memory, its padding cleared
-    auto ready = [&](int j) {
-      const int it = j - t0, s = it % L::kStages;
-      if (!wait.warp(full + s, (it / L::kStages) & 1)) return false;
-      const int from = (mask.q_len - j * a.tpt) * a.group;
-      if (from < a.group * a.tpt) {
-        clear_rows(sq + s * L::kTile, L::kBoxes, from);
-        clear_rows(sg + s * L::kTile, L::kBoxes, from);
-      }
-      tc_fence_after();
-      return true;
-    };
-    bool ok = wait.warp(kv_full, 0) && ready(t0);
-    if (ok && lead) {
-#pragma unroll
-      for (int w = 0; w < 2; w++) {
-        mma_rows<DP>(t_s + w * 64, dk, dq + w * kHalfRows, nk, id_s);
-        mma_commit(s_full + w);
-        mma_rows<DP>(t_g + w * 64, dv, dg + w * kHalfRows, nk, id_s);
-        mma_commit(g_full + w);
-      }
+    bool ok = wait(kv_full, 0) && wait(full, 0) && (t0 != clear_at || cleared(wait, ask, clean));
+#pragma unroll 1
+    for (int w = 0; w < 2 && ok; w++) {
+      mma_rows<DP>(t_s + w * 64, dk, dq + w * kHalfRows, nk, id_s);
+      mma_commit(s_full + w);
+      mma_rows<DP>(t_g + w * 64, dv, dg + w * kHalfRows, nk, id_s);
+      mma_commit(g_full + w);
     }
-    __syncwarp();
+    int s = 0, turn = 0;
     for (int j = t0; j < t1 && ok; j++) {
-      const int it = j - t0, s = it % L::kStages, s1 = (it + 1) % L::kStages;
+      const int s1 = s + 1 == L::kStages ? 0 : s + 1, turn1 = s1 ? turn : turn ^ 1, parity = (j - t0) & 1;
       const bool more = j + 1 < t1;
-#pragma unroll
+#pragma unroll 1
       for (int w = 0; w < 2; w++) {
-        ok = ok && wait.warp(p_full + w, it & 1);
+        ok = wait(p_full + w, parity);
         if (!ok) break;
         tc_fence_after();
-        if (lead) mma_tmem<64>(t_dv, t_s + w * 64, dg_mn + s * kStep + w * kHalfRows, id_o, it == 0 && w == 0);
+        mma_tmem<64>(t_dv, t_s + w * 64, dg_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0);
         if (more) {
-          if (w == 0) ok = ready(j + 1);
+          if (w == 0) ok = wait(full + s1, turn1) && (j + 1 != clear_at || cleared(wait, ask, clean));
           if (!ok) break;
-          if (lead) {
-            mma_rows<DP>(t_s + w * 64, dk, dq + s1 * kStep + w * kHalfRows, nk, id_s);
-            mma_commit(s_full + w);
-          }
+          mma_rows<DP>(t_s + w * 64, dk, dq + s1 * kStep + w * kHalfRows, nk, id_s);
+          mma_commit(s_full + w);
         }
-        ok = wait.warp(d_full + w, it & 1);
+        ok = wait(d_full + w, parity);
         if (!ok) break;
         tc_fence_after();
-        if (lead) {
-          mma_tmem<64>(t_dk, t_g + w * 64, dq_mn + s * kStep + w * kHalfRows, id_o, it == 0 && w == 0);
-          if (w == 1) mma_commit(empty + s);
-          if (more) {
-            mma_rows<DP>(t_g + w * 64, dv, dg + s1 * kStep + w * kHalfRows, nk, id_s);
-            mma_commit(g_full + w);
-          }
+        mma_tmem<64>(t_dk, t_g + w * 64, dq_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0);
+        if (w == 1) mma_commit(empty + s);
+        if (more) {
+          mma_rows<DP>(t_g + w * 64, dv, dg + s1 * kStep + w * kHalfRows, nk, id_s);
+          mma_commit(g_full + w);
         }
-        __syncwarp();
       }
+      s = s1, turn = turn1;
     }
-    if (ok && lead) mma_commit(done);
-    __syncwarp();
+    if (ok) mma_commit(done);
   } else if (warp < kProducerWarp) {
     const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
@@ -809,8 +801,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   float *row_sums = reinterpret_cast<float *>(sv + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile + L::kRowSums);
   uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 3, *s_free = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *full = bars + 11, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 11 + 2 * L::kStages);
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *full = bars + 13, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 13 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5;
 
@@ -822,10 +814,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const AttnMask mask(p, n);
   const int first = qt * a.tpt;
   const int t1 = first < mask.q_len ? (mask.key_end(min(first + a.tpt, mask.q_len) - 1) + 127) / 128 : 0;
+  const int clear_at = mask.k_len % 128 ? mask.k_len / 128 : INT_MAX;  // the key tile that holds padding
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 11; b++) mbar_init(b, b >= s_free && b < done ? 4 : 1);
+    for (uint64_t *b = bars; b < bars + 13; b++) mbar_init(b, b >= s_free && b < done ? 4 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
@@ -852,62 +845,53 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     mbar_wait(q_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
-  } else if (warp == kMmaWarp && t1 > 0) {
-    const bool lead = elect_one();
+  } else if (warp == kClearWarp && clear_at < t1) {
+    const int s = clear_at % L::kStages;
+    if (wait.warp(ask, 0) && wait.warp(full + s, (clear_at / L::kStages) & 1)) {
+      clear_rows(sk + s * L::kTile, L::kBoxes, mask.k_len - clear_at * 128);
+      if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
+    }
+  } else if (warp == kMmaWarp && t1 > 0 && elect_one()) {
     const uint64_t dq = smem_desc(smem_u32(sq)), dg = smem_desc(smem_u32(sg)), dk = smem_desc(smem_u32(sk)),
                    dv = smem_desc(smem_u32(sv)), dk_mn = desc_mn(smem_u32(sk));
     constexpr uint32_t kStep = L::kTile >> 4;
     const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
-    auto ready = [&](int j) {
-      const int s = j % L::kStages;
-      if (!wait.warp(full + s, (j / L::kStages) & 1)) return false;
-      if ((j + 1) * 128 > mask.k_len) clear_rows(sk + s * L::kTile, L::kBoxes, mask.k_len - j * 128);
-      tc_fence_after();
-      return true;
-    };
-    bool ok = wait.warp(q_full, 0) && ready(0);
-    if (ok && lead) {
-#pragma unroll
-      for (int w = 0; w < 2; w++) {
-        mma_rows<DP>(t_s + w * 64, dq, dk + w * kHalfRows, nk, id_s);
-        mma_commit(s_full + w);
-        mma_rows<DP>(t_g + w * 64, dg, dv + w * kHalfRows, nk, id_s);
-        mma_commit(g_full + w);
-      }
+    bool ok = wait(q_full, 0) && wait(full, 0) && (clear_at != 0 || cleared(wait, ask, clean));
+#pragma unroll 1
+    for (int w = 0; w < 2 && ok; w++) {
+      mma_rows<DP>(t_s + w * 64, dq, dk + w * kHalfRows, nk, id_s);
+      mma_commit(s_full + w);
+      mma_rows<DP>(t_g + w * 64, dg, dv + w * kHalfRows, nk, id_s);
+      mma_commit(g_full + w);
     }
-    __syncwarp();
+    int s = 0, turn = 0;
     for (int j = 0; j < t1 && ok; j++) {
-      const int s = j % L::kStages, s1 = (j + 1) % L::kStages;
+      const int s1 = s + 1 == L::kStages ? 0 : s + 1, turn1 = s1 ? turn : turn ^ 1, parity = j & 1;
       const bool more = j + 1 < t1;
-#pragma unroll
+#pragma unroll 1
       for (int w = 0; w < 2; w++) {
         if (more) {
-          ok = ok && wait.warp(s_free + w, j & 1);
-          if (ok && w == 0) ok = ready(j + 1);
+          ok = wait(s_free + w, parity);
+          if (ok && w == 0) ok = wait(full + s1, turn1) && (j + 1 != clear_at || cleared(wait, ask, clean));
           if (!ok) break;
           tc_fence_after();
-          if (lead) {
-            mma_rows<DP>(t_s + w * 64, dq, dk + s1 * kStep + w * kHalfRows, nk, id_s);
-            mma_commit(s_full + w);
-          }
+          mma_rows<DP>(t_s + w * 64, dq, dk + s1 * kStep + w * kHalfRows, nk, id_s);
+          mma_commit(s_full + w);
         }
-        ok = wait.warp(d_full + w, j & 1);
+        ok = wait(d_full + w, parity);
         if (!ok) break;
         tc_fence_after();
-        if (lead) {
-          mma_tmem<64>(t_dq, t_g + w * 64, dk_mn + s * kStep + w * kHalfRows, id_o, j == 0 && w == 0);
-          if (w == 1) mma_commit(empty + s);
-          if (more) {
-            mma_rows<DP>(t_g + w * 64, dg, dv + s1 * kStep + w * kHalfRows, nk, id_s);
-            mma_commit(g_full + w);
-          }
+        mma_tmem<64>(t_dq, t_g + w * 64, dk_mn + s * kStep + w * kHalfRows, id_o, j == 0 && w == 0);
+        if (w == 1) mma_commit(empty + s);
+        if (more) {
+          mma_rows<DP>(t_g + w * 64, dg, dv + s1 * kStep + w * kHalfRows, nk, id_s);
+          mma_commit(g_full + w);
         }
-        __syncwarp();
       }
+      s = s1, turn = turn1;
     }
-    if (ok && lead) mma_commit(done);
-    __syncwarp();
+    if (ok) mma_commit(done);
   } else if (warp < kProducerWarp) {
     const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
