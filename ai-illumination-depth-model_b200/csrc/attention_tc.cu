@@ -44,8 +44,15 @@ using namespace tcx;
 using tok::allow_smem;
 using tok::bf16;
 
-constexpr int kTcThreads = 384;
-constexpr int kProducerWarp = 8, kMmaWarp = 9, kClearWarp = 10;
+// Compute warpgroups, then one of single warps: copies, products, clearing of
+// padding, row sums.
+constexpr int kFwdGroups = 2, kBwdGroups = 4;
+constexpr int threads_of(int groups) { return 128 * (groups + 1); }
+struct Roles {
+  int copy, product, clear, sums;
+  __host__ __device__ constexpr explicit Roles(int groups)
+      : copy(4 * groups), product(4 * groups + 1), clear(4 * groups + 2), sums(4 * groups + 3) {}
+};
 constexpr uint32_t kImage = 128 * 128;  // 128 rows x 64 bf16 columns
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -65,6 +72,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t *r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(a));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t a, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(a));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t *r) {
@@ -124,11 +138,12 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, int
   }
 }
 // d[128][n] (+)= a(TMEM, bf16 pairs)[128][K] * b(image)[K][n], with b an
-// MN-major descriptor.
+// MN-major descriptor; every 32 of K lie `gap` columns apart.
 template <int K>
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool first) {
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool first, uint32_t gap = 16) {
 #pragma unroll
-  for (int k = 0; k < K / 16; k++) mma_ts(d, a + k * 8, b + k * 128, idesc, first && k == 0 ? 0u : 1u);
+  for (int k = 0; k < K / 16; k++)
+    mma_ts(d, a + (k >> 1) * gap + (k & 1) * 8, b + k * 128, idesc, first && k == 0 ? 0u : 1u);
 }
 constexpr uint32_t kHalfRows = 64 * 128 >> 4;  // descriptor step from row 0 to row 64 of an image
 
@@ -147,20 +162,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// Two finite values >= 0 as bf16, rounded to the nearest (ties away from
-// zero). The conversion instruction shares the pipe of the exponentials, which
-// bounds these kernels; two integer additions and a byte permutation do not.
-__device__ __forceinline__ uint32_t pack2_finite(float lo, float hi) {
-  return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
+// Without a suspend time the wait is the barrier's own: it returns as soon as
+// the phase completes. (With one, a failed test is followed by a sleep.)
+__device__ __forceinline__ bool try_wait(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // A wait that ends when another role of the CTA has given up, too.
 struct Waiter {
   volatile int *fail;
   __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity) const {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (try_wait(bar, parity)) return true;
     const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
+    while (!try_wait(bar, parity)) {
       if (*fail || clock64() - t0 > kWaitCycles) {
         *fail = 1;
         return false;
@@ -190,6 +210,20 @@ __device__ __forceinline__ void clear_rows(uint8_t *tile, int boxes, int from) {
   __syncwarp();
 }
 
+// The two warps that share an SM quarter begin their exponentials in turns (g:
+// warpgroup, others: iterations of the other warpgroup): in step they would
+// share its exponential unit, and leave it idle together during everything
+// else. The turn passes after a quarter of them: one warp alone does not fill
+// the unit.
+__device__ __forceinline__ bool my_turn(const Waiter &wait, uint64_t *turn, int g, int it, int others) {
+  uint64_t *bar = turn + 4 * g + (threadIdx.x >> 5 & 3);
+  if (g == 0) return it == 0 || it > others || wait.warp(bar, (it - 1) & 1);
+  return it >= others || wait.warp(bar, it & 1);
+}
+__device__ __forceinline__ void pass_turn(uint64_t *turn, int g) {
+  if ((threadIdx.x & 31) == 0) mbar_arrive(turn + 4 * (g ^ 1) + (threadIdx.x >> 5 & 3));
+}
+
 // The product thread has the tile that holds padding and asks for its clearing.
 __device__ __forceinline__ bool cleared(const Waiter &wait, uint64_t *ask, uint64_t *clean) {
   mbar_arrive(ask);
@@ -215,9 +249,9 @@ __device__ __forceinline__ void store_zeros(bf16 *dst, int n) {
 
 // The end of every kernel: copies and products of a CTA that gave up are
 // drained, then TMEM is freed.
-__device__ __forceinline__ void leave(uint32_t tmem, int warp, volatile int *fail, uint64_t *drain, int *err) {
+__device__ __forceinline__ void leave(uint32_t tmem, bool product_warp, volatile int *fail, uint64_t *drain, int *err) {
   __syncwarp();
-  if (warp == kMmaWarp) {
+  if (product_warp) {
     if (elect_one()) {  // the thread that issued the products
       mma_commit(drain);
       mbar_wait(drain, 0);
@@ -227,7 +261,7 @@ __device__ __forceinline__ void leave(uint32_t tmem, int warp, volatile int *fai
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *fail) report_gave_up(err);
-  if (warp == kMmaWarp) {
+  if (product_warp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -249,23 +283,28 @@ template <int DP>
 struct FwdSmem {
   static constexpr int kBoxes = DP / 64, kStages = DP == 64 ? 3 : 2;
   static constexpr uint32_t kTile = kBoxes * kImage;
-  static constexpr size_t kBytes = 1024 + (2 + 2 * kStages) * kTile + 256;
+  static constexpr size_t kBytes = 1024 + (2 + 2 * kStages) * kTile + 512;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
     k_attn_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
               const __grid_constant__ CUtensorMap mv, const AttnParams p, const TcArgs a) {
   using L = FwdSmem<DP>;
+  // TMEM: S 2 x 128 columns, O 2 x DP. Where 128 columns are left, P has a
+  // place of its own and the next S is computed while this one becomes P;
+  // else P replaces S.
+  constexpr bool kApart = DP == 64;
   extern __shared__ uint8_t raw[];
   uint8_t *base = align1024(raw);
   uint8_t *sq = base, *sk = sq + 2 * L::kTile, *sv = sk + L::kStages * L::kTile;
   uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile);
   uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 4, *o_full = bars + 6, *drain = bars + 8,
-           *ask = bars + 9, *clean = bars + 10, *k_full = bars + 11, *k_empty = k_full + L::kStages, *v_full = k_empty + L::kStages,
+           *ask = bars + 9, *clean = bars + 10, *s_free = bars + 11, *turn = bars + 13, *k_full = bars + 21, *k_empty = k_full + L::kStages, *v_full = k_empty + L::kStages,
            *v_empty = v_full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 11 + 4 * L::kStages);
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 21 + 4 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
+  constexpr Roles roles(kFwdGroups);
   const int warp = threadIdx.x >> 5;
 
   long long id = blockIdx.x;
@@ -297,24 +336,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (int i = 0; i < 2; i++) mbar_init(q_full + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1);
+    for (int i = 0; i < 2; i++) mbar_init(q_full + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1), mbar_init(s_free + i, 4);
     mbar_init(drain, 1);
     mbar_init(ask, 1);
     mbar_init(clean, 1);
+    for (int i = 0; i < 8; i++) mbar_init(turn + i, 1);
     for (int i = 0; i < L::kStages; i++)
       mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
     fence_barrier_init();
   }
-  if (warp == kMmaWarp) tmem_alloc(tmem_ptr, 512);
+  if (warp == roles.product) tmem_alloc(tmem_ptr, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const Waiter wait{fail};
 
-  if (warp >= kProducerWarp) {
+  if (warp >= roles.copy) {
     reg_dealloc<88>();
-    if (warp == kProducerWarp && (threadIdx.x & 31) == 0 && t0 < most) {
+    if (warp == roles.copy && (threadIdx.x & 31) == 0 && t0 < most) {
       int queries = 0;
       for (int i = 0; i < 2; i++)
         if (t0 < t1[i]) {
@@ -340,13 +380,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (queries >> i & 1) mbar_wait(q_full + i, 0);
       for (int i = max(0, issued_k - L::kStages); i < issued_k; i++) mbar_wait(k_full + i % L::kStages, (i / L::kStages) & 1);
       for (int i = max(0, issued_v - L::kStages); i < issued_v; i++) mbar_wait(v_full + i % L::kStages, (i / L::kStages) & 1);
-    } else if (warp == kClearWarp && clear_at < most && clear_at >= t0) {
+    } else if (warp == roles.clear && clear_at < most && clear_at >= t0) {
       const int it = clear_at - t0, s = it % L::kStages;
       if (wait.warp(ask, 0) && wait.warp(v_full + s, (it / L::kStages) & 1)) {
         clear_rows(sv + s * L::kTile, L::kBoxes, mask.k_len - clear_at * 128);
         if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
       }
-    } else if (warp == kMmaWarp && t0 < most && elect_one()) {
+    } else if (warp == roles.product && t0 < most && elect_one()) {
       const uint64_t dq = smem_desc(smem_u32(sq)), dk = smem_desc(smem_u32(sk)), dv = desc_mn(smem_u32(sv));
       constexpr uint32_t kStep = L::kTile >> 4;  // descriptors of the next tile
       const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
@@ -362,11 +402,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mma_commit(s_full + i);
       }
       if (ok) mma_commit(k_empty);
-      int s = 0, turn = 0;  // stage of tile j, parity of its use
+      int s = 0, use = 0;  // stage of tile j, parity of its use
       for (int j = t0; j < most && ok; j++) {
-        const int s1 = s + 1 == L::kStages ? 0 : s + 1, turn1 = s1 ? turn : turn ^ 1, parity = (j - t0) & 1;
+        const int s1 = s + 1 == L::kStages ? 0 : s + 1, use1 = s1 ? use : use ^ 1, parity = (j - t0) & 1;
         const bool more = j + 1 < most;
-        ok = wait(v_full + s, turn) && (j != clear_at || cleared(wait, ask, clean)) && (!more || wait(k_full + s1, turn1));
+        if constexpr (kApart) {
+          if (more) {
+            ok = wait(k_full + s1, use1);
+#pragma unroll 1
+            for (int i = 0; i < 2 && ok; i++) {
+              if (j + 1 >= (i ? end1 : end0)) continue;
+              ok = wait(s_free + i, parity);
+              if (!ok) break;
+              tc_fence_after();
+              mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk + s1 * kStep, nk, id_s);
+              mma_commit(s_full + i);
+            }
+            if (!ok) break;
+            mma_commit(k_empty + s1);
+          }
+        }
+        ok = wait(v_full + s, use) && (j != clear_at || cleared(wait, ask, clean)) &&
+             (kApart || !more || wait(k_full + s1, use1));
         if (!ok) break;
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
@@ -375,17 +432,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ok = wait(p_full + i, parity);
           if (!ok) break;
           tc_fence_after();
-          mma_tmem<128>(tmem + 256 + i * DP, tmem + i * 128, dv + s * kStep, id_o, j == t0);
+          mma_tmem<128>(tmem + 256 + i * DP, kApart ? tmem + 384 + i * 64 : tmem + i * 128, dv + s * kStep, id_o, j == t0);
           mma_commit(o_full + i);
-          if (j + 1 < end) {
+          if (!kApart && j + 1 < end) {
             mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk + s1 * kStep, nk, id_s);
             mma_commit(s_full + i);
           }
         }
         if (!ok) break;
         mma_commit(v_empty + s);
-        if (more) mma_commit(k_empty + s1);
-        s = s1, turn = turn1;
+        if (!kApart && more) mma_commit(k_empty + s1);
+        s = s1, use = use1;
       }
     }
     __syncwarp();
@@ -394,6 +451,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int i = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // 32 TMEM lanes a warp
     const uint32_t ts = tmem + lane_base + i * 128, to = tmem + lane_base + 256 + i * DP;
+    const uint32_t tp = kApart ? tmem + lane_base + 384 + i * 64 : ts;
     const int tile = 2 * pair + i;
     const int token = tile * a.tpt + row / a.group, h = hk * a.group + row % a.group;
     const bool mine = tile < a.q_tiles && row < a.group * a.tpt && token < p.q_tokens;
@@ -410,6 +468,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
       for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, r + 32 * c);
       tmem_wait_ld();
+      if constexpr (kApart) {
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(s_free + i);
+      }
       const int left = end - j * 128;
       if (__any_sync(0xffffffffu, left < 128)) {
 #pragma unroll
@@ -436,10 +499,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         sum *= f;
         grow = true;
       }
-      if (__any_sync(0xffffffffu, grow)) {
+      grow = __any_sync(0xffffffffu, grow);
+      if (it > 0 && (kApart || grow)) {  // the previous product: it reads P's place, or is about to be rescaled
         ok = wait.warp(o_full + i, (it - 1) & 1);
         if (!ok) break;
         tc_fence_after();
+      }
+      if (grow) {
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
           uint32_t o[32];
@@ -451,6 +517,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       const float shift = top == -INFINITY ? 0.0f : -top;
+      if constexpr (kApart) {
+        ok = my_turn(wait, turn, i, it, t1[i ^ 1] - t0);
+        if (!ok) break;
+      }
       const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(shift, shift);
       float2 s2[2] = {make_float2(0, 0), make_float2(0, 0)};
 #pragma unroll
@@ -461,10 +531,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c + k]), __uint_as_float(r[c + k + 1])), scale2, shift2);
           x = make_float2(ex2(x.x), ex2(x.y));
           s2[k / 2 & 1] = __fadd2_rn(s2[k / 2 & 1], x);
-          // a NaN goes missing here, and shows in the sum
-          q[k / 2] = pack2_finite(x.x, x.y);
+          q[k / 2] = pack2(x.x, x.y);
         }
-        tmem_st16(ts + c / 2, q);
+        tmem_st16(tp + c / 2, q);
+        if (kApart && c == 0) pass_turn(turn, i);
       }
       sum += (s2[0].x + s2[0].y) + (s2[1].x + s2[1].y);
       tmem_wait_st();
@@ -515,43 +585,50 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (mine) p.ws[a.splits * rows * p.head_dim + split * rows + at] = lse;
     }
   }
-  leave(tmem, warp, fail, drain, p.err);
+  leave(tmem, warp == roles.product, fail, drain, p.err);
 }
 
 // ---------------------------------------------------------------------------
 // Backward, dK and dV: one key tile (its rows are the TMEM lanes) past the
 // query tiles that see it. Per query tile: S' = K Q', dP' = V dO', and from
-// TMEM dV += P' dO, dK += dS' Q. The two warpgroups take 64 query columns
-// each, as two pipelines of their own that the product warp serves in turn:
+// TMEM dV += P' dO, dK += dS' Q. A warpgroup takes 32 query columns: the
+// arithmetic is bound by its latencies, and four warps an SM quarter cover one
+// another's where two (64 columns each) left it idle two thirds of the time.
+// The columns go to the products in halves. Where TMEM has 128 columns left
+// (head sizes up to 64), P' and dS' have places of their own, and the next S'
+// and dP' are computed as soon as all warpgroups have loaded these:
+//   P0(j): dV   S free: S(j+1)   dS0(j): dK   P1(j): dV   dP free: dP(j+1)   dS1(j): dK
+// Else they replace S' and dP', and a half of the next one follows the product
+// that reads them:
 //   P0(j): dV, S0(j+1)   dS0(j): dK, dP0(j+1)   P1(j): dV, S1(j+1)   dS1(j): dK, dP1(j+1)
-// so that they run half a tile apart: one is in its exponentials while the
-// other is in its products and differences, and a warpgroup finds its next
-// operands ready. The order of the sums is fixed.
+// The order of the sums is fixed in both.
 // ---------------------------------------------------------------------------
 
 template <int DP>
 struct BwdSmem {
   static constexpr int kBoxes = DP / 64, kStages = DP == 64 ? 3 : 2;
   static constexpr uint32_t kTile = kBoxes * kImage;
-  static constexpr uint32_t kRowSums = 8 * 128 * 4;  // a warp's copy of 64 lse and 64 delta
-  static constexpr size_t kBytes = 1024 + (2 + 2 * kStages) * kTile + kRowSums + 256;
+  static constexpr uint32_t kRowSums = (2 * 256 + 4) * 4;  // shifts and deltas of two query tiles, two flags
+  static constexpr size_t kBytes = 1024 + (2 + 2 * kStages) * kTile + kRowSums + 512;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     k_attn_dkv_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg, const AttnParams p,
                   const TcArgs a) {
   using L = BwdSmem<DP>;
+  constexpr bool kApart = DP == 64;
   extern __shared__ uint8_t raw[];
   uint8_t *base = align1024(raw);
   uint8_t *sk = base, *sv = sk + L::kTile, *sq = sv + L::kTile, *sg = sq + L::kStages * L::kTile;
   float *row_sums = reinterpret_cast<float *>(sg + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sg + L::kStages * L::kTile + L::kRowSums);
   uint64_t *kv_full = bars, *s_full = bars + 1, *g_full = bars + 3, *p_full = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *full = bars + 13, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 13 + 2 * L::kStages);
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *s_free = bars + 13, *g_free = bars + 14, *used = bars + 15, *full = bars + 17, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 17 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
+  constexpr Roles roles(kBwdGroups);
   const int warp = threadIdx.x >> 5;
 
   long long id = blockIdx.x;
@@ -567,22 +644,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 13; b++) mbar_init(b, b >= p_full && b < done ? 4 : 1);
+    for (uint64_t *b = bars; b < bars + 17; b++)
+      mbar_init(b, b >= p_full && b < done ? 8 : b == s_free || b == g_free ? 16 : b >= s_full && b < g_full ? 2 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
   // rows of the query images past group * tpt are never written by the copies
   if (a.group * a.tpt < 128)
-    for (int t = warp; t < 2 * L::kStages; t += kTcThreads / 32) clear_rows(sq + t * L::kTile, L::kBoxes, a.group * a.tpt);
-  if (warp == kMmaWarp) tmem_alloc(tmem_ptr, 512);
+    for (int t = warp; t < 2 * L::kStages; t += threads_of(kBwdGroups) / 32) clear_rows(sq + t * L::kTile, L::kBoxes, a.group * a.tpt);
+  if (warp == roles.product) tmem_alloc(tmem_ptr, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const uint32_t t_s = tmem, t_g = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
+  // P' and dS' of half w of the query columns: 32 columns from w * p_step on,
+  // or the first half of every warpgroup's own 32 columns of S' and dP'
+  const uint32_t t_p = kApart ? tmem + 384 : t_s, t_d = kApart ? tmem + 448 : t_g;
+  constexpr uint32_t p_step = kApart ? 32 : 64, p_gap = kApart ? 16 : 32;
   const Waiter wait{fail};
 
-  if (warp == kProducerWarp && (threadIdx.x & 31) == 0 && some) {
+  if (warp == roles.copy && (threadIdx.x & 31) == 0 && some) {
     mbar_expect_tx(kv_full, 2 * L::kTile);
     load_images(smem_u32(sk), &mk, L::kBoxes, a.kh * hk, key0, a.kb * n, kv_full);
     load_images(smem_u32(sv), &mv, L::kBoxes, a.vh * hk, key0, a.vb * n, kv_full);
@@ -597,18 +679,52 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     mbar_wait(kv_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
-  } else if (warp == kClearWarp && clear_at < t1 && clear_at >= t0) {
+  } else if (warp == roles.clear && clear_at < t1 && clear_at >= t0) {
     const int it = clear_at - t0, s = it % L::kStages, from = (mask.q_len - clear_at * a.tpt) * a.group;
     if (wait.warp(ask, 0) && wait.warp(full + s, (it / L::kStages) & 1)) {
       clear_rows(sq + s * L::kTile, L::kBoxes, from);
       clear_rows(sg + s * L::kTile, L::kBoxes, from);
       if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
     }
-  } else if (warp == kMmaWarp && some && elect_one()) {
+  } else if (warp == roles.sums && some) {
+    // lse and delta of every query tile's rows, half a tile ahead of their use:
+    // shift (base 2; -inf where a row has no probabilities) and -delta
+    const int lane = threadIdx.x & 31;
+    int column[4];  // token within a query tile
+    const float *lse_of[4], *delta_of[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int r = k * 32 + lane;
+      column[k] = r < a.group * a.tpt ? r / a.group : INT_MAX / 2;
+      const long long at = ((long long)n * p.heads + hk * a.group + r % a.group) * p.q_tokens;
+      lse_of[k] = p.lse + at, delta_of[k] = p.ws + at;
+    }
+    for (int j = t0; j < t1; j++) {
+      const int it = j - t0;
+      float l[4], d[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int token = j * a.tpt + column[k];
+        l[k] = -INFINITY, d[k] = 0;
+        if (token < mask.q_len) l[k] = lse_of[k][token], d[k] = delta_of[k][token];
+      }
+      // with the probabilities of tile j - 1 the warpgroups are done with
+      // tile j - 2 (a wait for that tile itself could miss its phase)
+      if (it >= 1 && !(wait.warp(p_full, (it - 1) & 1) && wait.warp(p_full + 1, (it - 1) & 1))) break;
+      float *to = row_sums + (it & 1) * 256;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        to[k * 32 + lane] = l[k] == -INFINITY ? -INFINITY : -l[k] * kLog2e;
+        to[128 + k * 32 + lane] = -d[k];
+      }
+      __syncwarp();
+      if (lane < 2) mbar_arrive(s_full + lane);
+    }
+  } else if (warp == roles.product && some && elect_one()) {
     const uint64_t dk = smem_desc(smem_u32(sk)), dv = smem_desc(smem_u32(sv)), dq = smem_desc(smem_u32(sq)),
                    dg = smem_desc(smem_u32(sg)), dq_mn = desc_mn(smem_u32(sq)), dg_mn = desc_mn(smem_u32(sg));
     constexpr uint32_t kStep = L::kTile >> 4;
-    const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
+    const uint32_t id_s = instr_desc(1, 64), id_s2 = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
     bool ok = wait(kv_full, 0) && wait(full, 0) && (t0 != clear_at || cleared(wait, ask, clean));
 #pragma unroll 1
@@ -618,18 +734,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mma_rows<DP>(t_g + w * 64, dv, dg + w * kHalfRows, nk, id_s);
       mma_commit(g_full + w);
     }
-    int s = 0, turn = 0;
+    int s = 0, use = 0;
     for (int j = t0; j < t1 && ok; j++) {
-      const int s1 = s + 1 == L::kStages ? 0 : s + 1, turn1 = s1 ? turn : turn ^ 1, parity = (j - t0) & 1;
+      const int s1 = s + 1 == L::kStages ? 0 : s + 1, use1 = s1 ? use : use ^ 1, parity = (j - t0) & 1;
       const bool more = j + 1 < t1;
 #pragma unroll 1
       for (int w = 0; w < 2; w++) {
         ok = wait(p_full + w, parity);
         if (!ok) break;
         tc_fence_after();
-        mma_tmem<64>(t_dv, t_s + w * 64, dg_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0);
-        if (more) {
-          if (w == 0) ok = wait(full + s1, turn1) && (j + 1 != clear_at || cleared(wait, ask, clean));
+        mma_tmem<64>(t_dv, t_p + w * p_step, dg_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0, p_gap);
+        if (more && kApart) {
+          if (w == 0) {
+            ok = wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean)) && wait(s_free, parity);
+            if (!ok) break;
+            tc_fence_after();
+            mma_rows<DP>(t_s, dk, dq + s1 * kStep, nk, id_s2);
+            mma_commit(s_full);
+            mma_commit(s_full + 1);
+          } else {
+            ok = wait(g_free, parity);
+            if (!ok) break;
+            tc_fence_after();
+            mma_rows<DP>(t_g, dv, dg + s1 * kStep, nk, id_s2);
+            mma_commit(g_full);
+            mma_commit(g_full + 1);
+          }
+        } else if (more) {
+          if (w == 0) ok = wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean));
           if (!ok) break;
           mma_rows<DP>(t_s + w * 64, dk, dq + s1 * kStep + w * kHalfRows, nk, id_s);
           mma_commit(s_full + w);
@@ -637,76 +769,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         ok = wait(d_full + w, parity);
         if (!ok) break;
         tc_fence_after();
-        mma_tmem<64>(t_dk, t_g + w * 64, dq_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0);
+        mma_tmem<64>(t_dk, t_d + w * p_step, dq_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0, p_gap);
+        if (kApart) mma_commit(used + w);
         if (w == 1) mma_commit(empty + s);
-        if (more) {
+        if (more && !kApart) {
           mma_rows<DP>(t_g + w * 64, dv, dg + s1 * kStep + w * kHalfRows, nk, id_s);
           mma_commit(g_full + w);
         }
       }
-      s = s1, turn = turn1;
+      s = s1, use = use1;
     }
     if (ok) mma_commit(done);
-  } else if (warp < kProducerWarp) {
-    const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
+  } else if (warp < roles.copy) {
+    const int wg = warp >> 2, half = wg >> 1, row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
-    const uint32_t ts = t_s + lane_base + wg * 64, tg = t_g + lane_base + wg * 64;
+    const uint32_t ts = t_s + lane_base + wg * 32, tg = t_g + lane_base + wg * 32;
+    const uint32_t tp = t_p + lane_base + half * p_step + (wg & 1) * p_gap, td = t_d + lane_base + half * p_step + (wg & 1) * p_gap;
     const int key = key0 + row;
     const int begin = key < mask.k_len ? mask.row_begin(key) : INT_MAX / 2;
     const float sl2 = p.scale * kLog2e;
-    float *mine_lse = row_sums + warp * 128, *mine_delta = mine_lse + 64;
     const float2 scale2 = make_float2(sl2, sl2);
-    // lse and delta of the two columns this lane fetches of query tile j, as
-    // they come: nothing waits for them until the next tile begins
-    float nl[2], nd[2];
-    int column[2];          // token within a query tile
-    const float *lse_of[2], *delta_of[2];  // of its head
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      const int r = wg * 64 + k * 32 + lane;
-      column[k] = r < a.group * a.tpt ? r / a.group : INT_MAX / 2;
-      const long long at = ((long long)n * p.heads + hk * a.group + r % a.group) * p.q_tokens;
-      lse_of[k] = p.lse + at, delta_of[k] = p.ws + at;
-    }
-    auto fetch = [&](int j) {
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const int token = j * a.tpt + column[k];
-        nl[k] = -INFINITY, nd[k] = 0;
-        if (token < mask.q_len) {
-          nl[k] = lse_of[k][token];
-          nd[k] = delta_of[k][token];
-        }
-      }
-    };
     bool ok = true;
-    if (some) fetch(t0);
     for (int j = t0; j < t1; j++) {
       const int it = j - t0;
-      __syncwarp();
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        // exponent's shift in base 2; a row without probabilities (lse -inf) gets none here either
-        mine_lse[k * 32 + lane] = nl[k] == -INFINITY ? -INFINITY : -nl[k] * kLog2e;
-        mine_delta[k * 32 + lane] = -nd[k];
-      }
-      __syncwarp();
-      // probabilities are NaN where a row's lse is, and nowhere else
-      const bool spoiled = __any_sync(0xffffffffu, nl[0] != nl[0] || nl[1] != nl[1]);
-      if (j + 1 < t1) fetch(j + 1);
+      const float *mine_shift = row_sums + (it & 1) * 256 + wg * 32, *mine_delta = mine_shift + 128;
       // columns below `skip` are queries that do not see this key
-      const int skip = min(max(min(max(begin - j * a.tpt, 0), 128) * a.group - wg * 64, 0), 64);
+      const int skip = min(max(min(max(begin - j * a.tpt, 0), 128) * a.group - wg * 32, 0), 32);
       const bool masked = __any_sync(0xffffffffu, skip > 0);
-      ok = wait.warp(s_full + wg, it & 1);
+      ok = wait.warp(s_full + half, it & 1);
       if (!ok) break;
       tc_fence_after();
-      uint32_t r[64];
+      uint32_t r[32];
       tmem_ld32(ts, r);
-      tmem_ld32(ts + 32, r + 32);
       tmem_wait_ld();
+      if constexpr (kApart) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+      }
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 l = *reinterpret_cast<const float4 *>(mine_lse + c);
+      for (int c = 0; c < 32; c += 4) {
+        const float4 l = *reinterpret_cast<const float4 *>(mine_shift + c);
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, make_float2(l.x, l.y));
         const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, make_float2(l.z, l.w));
         r[c] = __float_as_uint(ex2(x.x)), r[c + 1] = __float_as_uint(ex2(x.y));
@@ -714,83 +817,88 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (masked) {
 #pragma unroll
-        for (int c = 0; c < 64; c++)
+        for (int c = 0; c < 32; c++)
           if (c < skip) r[c] = 0;
       }
-      uint32_t q[32];
-      if (!spoiled) {
+      uint32_t q[16];
 #pragma unroll
-        for (int c = 0; c < 32; c++) q[c] = pack2_finite(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-      } else {
-#pragma unroll
-        for (int c = 0; c < 32; c++) q[c] = pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      for (int c = 0; c < 16; c++) q[c] = pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      if (kApart && it > 0) {  // the products of the last tile are done with P' and dS'
+        ok = wait.warp(used + half, (it - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
       }
-      tmem_st32(ts, q);
+      tmem_st16(tp, q);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + wg);
-      ok = wait.warp(g_full + wg, it & 1);
+      if (lane == 0) mbar_arrive(p_full + half);
+      ok = wait.warp(g_full + half, it & 1);
       if (!ok) break;
       tc_fence_after();
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        uint32_t g[32];
-        tmem_ld32(tg + 32 * half, g);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 d = *reinterpret_cast<const float4 *>(mine_delta + 32 * half + c);
-          const uint32_t *pr = r + 32 * half + c;
-          const float2 x = __fmul2_rn(make_float2(__uint_as_float(pr[0]), __uint_as_float(pr[1])),
-                                      __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), make_float2(d.x, d.y)));
-          const float2 y = __fmul2_rn(make_float2(__uint_as_float(pr[2]), __uint_as_float(pr[3])),
-                                      __fadd2_rn(make_float2(__uint_as_float(g[c + 2]), __uint_as_float(g[c + 3])), make_float2(d.z, d.w)));
-          float v[4] = {x.x, x.y, y.x, y.y};
-          if (masked) {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-              if (32 * half + c + k < skip) v[k] = 0;
-          }
-          q[16 * half + c / 2] = pack2(v[0], v[1]);
-          q[16 * half + c / 2 + 1] = pack2(v[2], v[3]);
-        }
+      uint32_t g[32];
+      tmem_ld32(tg, g);
+      tmem_wait_ld();
+      if constexpr (kApart) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(g_free);
       }
-      tmem_st32(tg, q);
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 32; c++)
+          if (c < skip) g[c] = 0;
+      }
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const float4 d = *reinterpret_cast<const float4 *>(mine_delta + c);
+        const float2 x = __fmul2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])),
+                                    __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), make_float2(d.x, d.y)));
+        const float2 y = __fmul2_rn(make_float2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])),
+                                    __fadd2_rn(make_float2(__uint_as_float(g[c + 2]), __uint_as_float(g[c + 3])), make_float2(d.z, d.w)));
+        q[c / 2] = pack2(x.x, x.y);
+        q[c / 2 + 1] = pack2(y.x, y.y);
+      }
+      tmem_st16(td, q);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(d_full + wg);
+      if (lane == 0) mbar_arrive(d_full + half);
     }
     if (some && ok) ok = wait.warp(done, 0);
     tc_fence_after();
     const bool inside = key < p.k_tokens, have = some && ok && key < mask.k_len;
-    // warpgroup 0 writes dV, warpgroup 1 dK
-    const AttnTensor &t = wg ? p.dk : p.dv;
-    bf16 *dst = (bf16 *)t.p + n * t.s[0] + (long long)key * t.s[1] + hk * t.s[2];
+    // warpgroups 0 and 1 write dV, 2 and 3 dK, half of the columns each
+    constexpr int kCols = DP / 2;
+    const AttnTensor &t = half ? p.dk : p.dv;
+    const int first = (wg & 1) * kCols;
+    bf16 *dst = (bf16 *)t.p + n * t.s[0] + (long long)key * t.s[1] + hk * t.s[2] + first;
     if (some && ok) {
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = 0; c < kCols; c += 32) {
         uint32_t o[32];
-        tmem_ld32((wg ? t_dk : t_dv) + lane_base + c, o);
+        tmem_ld32((half ? t_dk : t_dv) + lane_base + first + c, o);
         tmem_wait_ld();
-        if (inside && have) store_bf16(dst + c, o, p.head_dim - c, wg ? p.scale : 1.0f);
+        if (inside && have) store_bf16(dst + c, o, p.head_dim - first - c, half ? p.scale : 1.0f);
       }
     }
-    if (inside && !have) store_zeros(dst, p.head_dim);
+    if (inside && !have) store_zeros(dst, min(kCols, p.head_dim - first));
   }
-  leave(tmem, warp, fail, drain, p.err);
+  leave(tmem, warp == roles.product, fail, drain, p.err);
 }
 
 // ---------------------------------------------------------------------------
 // Backward, dQ: one query tile past the key tiles it sees. S = Q K' and
-// dP = dO V' are recomputed, dQ += dS K from TMEM. The warpgroups take 64 key
-// columns each, as two pipelines half a tile apart (as above); a thread's lse and delta stay in registers. This pass runs
-// first and leaves the row sums delta in the workspace for the other.
+// dP = dO V' are recomputed, dQ += dS K from TMEM. The warpgroups take 32 key
+// columns each; dS has a TMEM place of its own, and the next S and dP are
+// computed as soon as all warpgroups have loaded these:
+//   S free: S(j+1)   dS0(j): dQ   dP free: dP(j+1)   dS1(j): dQ
+// A thread's lse and delta stay in registers. This pass runs first and leaves
+// the row sums delta in the workspace for the other.
 // ---------------------------------------------------------------------------
 
 template <int DP>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     k_attn_dq_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                  const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg, const AttnParams p,
                  const TcArgs a) {
@@ -800,10 +908,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t *sq = base, *sg = sq + L::kTile, *sk = sg + L::kTile, *sv = sk + L::kStages * L::kTile;
   float *row_sums = reinterpret_cast<float *>(sv + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile + L::kRowSums);
-  uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 3, *s_free = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *full = bars + 13, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 13 + 2 * L::kStages);
+  uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 3, *s_free = bars + 5, *g_free = bars + 6, *d_full = bars + 7,
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *used = bars + 13, *full = bars + 15, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 15 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
+  constexpr Roles roles(kBwdGroups);
   const int warp = threadIdx.x >> 5;
 
   long long id = blockIdx.x;
@@ -818,19 +927,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 13; b++) mbar_init(b, b >= s_free && b < done ? 4 : 1);
+    for (uint64_t *b = bars; b < bars + 15; b++) mbar_init(b, b == s_free || b == g_free ? 16 : b == d_full || b == d_full + 1 ? 8 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
-  if (warp == kMmaWarp) tmem_alloc(tmem_ptr, 512);
+  if (warp == roles.product) tmem_alloc(tmem_ptr, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  const uint32_t t_s = tmem, t_g = tmem + 128, t_dq = tmem + 256;
+  const uint32_t t_s = tmem, t_g = tmem + 128, t_dq = tmem + 256, t_d = tmem + 384;
   const Waiter wait{fail};
 
-  if (warp == kProducerWarp && (threadIdx.x & 31) == 0 && t1 > 0) {
+  if (warp == roles.copy && (threadIdx.x & 31) == 0 && t1 > 0) {
     mbar_expect_tx(q_full, 2 * L::kBoxes * a.group * a.tpt * 128);
     load_images(smem_u32(sq), &mq, L::kBoxes, a.qh * hk * a.group, first, a.qb * n, q_full);
     load_images(smem_u32(sg), &mg, L::kBoxes, a.gh * hk * a.group, first, a.gb * n, q_full);
@@ -845,70 +954,66 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     mbar_wait(q_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
-  } else if (warp == kClearWarp && clear_at < t1) {
+  } else if (warp == roles.clear && clear_at < t1) {
     const int s = clear_at % L::kStages;
     if (wait.warp(ask, 0) && wait.warp(full + s, (clear_at / L::kStages) & 1)) {
       clear_rows(sk + s * L::kTile, L::kBoxes, mask.k_len - clear_at * 128);
       if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
     }
-  } else if (warp == kMmaWarp && t1 > 0 && elect_one()) {
+  } else if (warp == roles.product && t1 > 0 && elect_one()) {
     const uint64_t dq = smem_desc(smem_u32(sq)), dg = smem_desc(smem_u32(sg)), dk = smem_desc(smem_u32(sk)),
                    dv = smem_desc(smem_u32(sv)), dk_mn = desc_mn(smem_u32(sk));
     constexpr uint32_t kStep = L::kTile >> 4;
-    const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
+    const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
     bool ok = wait(q_full, 0) && wait(full, 0) && (clear_at != 0 || cleared(wait, ask, clean));
-#pragma unroll 1
-    for (int w = 0; w < 2 && ok; w++) {
-      mma_rows<DP>(t_s + w * 64, dq, dk + w * kHalfRows, nk, id_s);
-      mma_commit(s_full + w);
-      mma_rows<DP>(t_g + w * 64, dg, dv + w * kHalfRows, nk, id_s);
-      mma_commit(g_full + w);
+    if (ok) {
+      mma_rows<DP>(t_s, dq, dk, nk, id_s);
+      mma_commit(s_full);
+      mma_rows<DP>(t_g, dg, dv, nk, id_s);
+      mma_commit(g_full);
     }
-    int s = 0, turn = 0;
+    int s = 0, use = 0;
     for (int j = 0; j < t1 && ok; j++) {
-      const int s1 = s + 1 == L::kStages ? 0 : s + 1, turn1 = s1 ? turn : turn ^ 1, parity = j & 1;
+      const int s1 = s + 1 == L::kStages ? 0 : s + 1, use1 = s1 ? use : use ^ 1, parity = j & 1;
       const bool more = j + 1 < t1;
 #pragma unroll 1
       for (int w = 0; w < 2; w++) {
         if (more) {
-          ok = wait(s_free + w, parity);
-          if (ok && w == 0) ok = wait(full + s1, turn1) && (j + 1 != clear_at || cleared(wait, ask, clean));
+          ok = (w || (wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean)))) &&
+               wait(w ? g_free : s_free, parity);
           if (!ok) break;
           tc_fence_after();
-          mma_rows<DP>(t_s + w * 64, dq, dk + s1 * kStep + w * kHalfRows, nk, id_s);
-          mma_commit(s_full + w);
+          mma_rows<DP>(w ? t_g : t_s, w ? dg : dq, (w ? dv : dk) + s1 * kStep, nk, id_s);
+          mma_commit(w ? g_full : s_full);
         }
         ok = wait(d_full + w, parity);
         if (!ok) break;
         tc_fence_after();
-        mma_tmem<64>(t_dq, t_g + w * 64, dk_mn + s * kStep + w * kHalfRows, id_o, j == 0 && w == 0);
+        mma_tmem<64>(t_dq, t_d + w * 32, dk_mn + s * kStep + w * kHalfRows, id_o, j == 0 && w == 0);
+        mma_commit(used + w);
         if (w == 1) mma_commit(empty + s);
-        if (more) {
-          mma_rows<DP>(t_g + w * 64, dg, dv + s1 * kStep + w * kHalfRows, nk, id_s);
-          mma_commit(g_full + w);
-        }
       }
-      s = s1, turn = turn1;
+      s = s1, use = use1;
     }
     if (ok) mma_commit(done);
-  } else if (warp < kProducerWarp) {
-    const int wg = warp >> 2, row = threadIdx.x & 127, lane = threadIdx.x & 31;
+  } else if (warp < roles.copy) {
+    const int wg = warp >> 2, half = wg >> 1, row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
-    const uint32_t ts = t_s + lane_base + wg * 64, tg = t_g + lane_base + wg * 64;
+    const uint32_t ts = t_s + lane_base + wg * 32, tg = t_g + lane_base + wg * 32;
     const int token = first + row / a.group, h = hk * a.group + row % a.group;
     const bool mine = row < a.group * a.tpt && token < p.q_tokens;
     const int end = mine ? mask.key_end(token) : 0;
     const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
     const float v = end ? p.lse[at] : -INFINITY;
     const float shift = v == -INFINITY ? -INFINITY : -v * kLog2e;
-    // delta = rowsum(dO O): a warpgroup adds every second 8 columns
+    // delta = rowsum(dO O): a warpgroup adds every fourth 8 columns
     float part = 0;
     if (end > 0) {
       const bf16 *x = (const bf16 *)p.dout.p + n * p.dout.s[0] + token * p.dout.s[1] + h * p.dout.s[2];
       const bf16 *y = (const bf16 *)p.out.p + n * p.out.s[0] + token * p.out.s[1] + h * p.out.s[2];
 #pragma unroll
-      for (int c = 0; c < DP; c += 16)
+      for (int c = 0; c < DP; c += 32)
         if (c + wg * 8 < p.head_dim) {
           float u[8], w[8];
           tok::Pack<bf16, 8>::load(x + c + wg * 8, u);
@@ -918,74 +1023,77 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     }
     row_sums[wg * 128 + row] = part;
-    bar_named(1, 256);
-    const float delta = row_sums[row] + row_sums[128 + row];
+    bar_named(1, 512);
+    const float delta = (row_sums[row] + row_sums[128 + row]) + (row_sums[256 + row] + row_sums[384 + row]);
     if (wg == 0 && mine) p.ws[at] = delta;  // for the key pass
     const float sl2 = p.scale * kLog2e;
     const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(shift, shift), delta2 = make_float2(-delta, -delta);
     bool ok = true;
     for (int j = 0; j < t1; j++) {
-      const int left = end - j * 128 - wg * 64;
-      const bool masked = __any_sync(0xffffffffu, left < 64);
-      ok = wait.warp(s_full + wg, j & 1);
+      const int left = end - j * 128 - wg * 32;
+      const bool masked = __any_sync(0xffffffffu, left < 32);
+      ok = wait.warp(s_full, j & 1);
       if (!ok) break;
       tc_fence_after();
-      uint32_t r[64];
+      uint32_t r[32];
       tmem_ld32(ts, r);
-      tmem_ld32(ts + 32, r + 32);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_free + wg);
+      if (lane == 0) mbar_arrive(s_free);
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
+      for (int c = 0; c < 32; c += 2) {
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, shift2);
         r[c] = __float_as_uint(ex2(x.x)), r[c + 1] = __float_as_uint(ex2(x.y));
       }
-      ok = wait.warp(g_full + wg, j & 1);
+      ok = wait.warp(g_full, j & 1);
       if (!ok) break;
       tc_fence_after();
-      uint32_t q[32];
+      uint32_t g[32], q[16];
+      tmem_ld32(tg, g);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(g_free);
+      if (masked) {
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        uint32_t g[32];
-        tmem_ld32(tg + 32 * half, g);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float2 x = __fmul2_rn(make_float2(__uint_as_float(r[32 * half + c]), __uint_as_float(r[32 * half + c + 1])),
-                                __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), delta2));
-          if (masked) {
-            if (32 * half + c >= left) x.x = 0;
-            if (32 * half + c + 1 >= left) x.y = 0;
-          }
-          q[16 * half + c / 2] = pack2(x.x, x.y);
-        }
+        for (int c = 0; c < 32; c++)
+          if (c >= left) r[c] = 0, g[c] = 0;
       }
-      tmem_st32(tg, q);
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        float2 x = __fmul2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])),
+                              __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), delta2));
+        q[c / 2] = pack2(x.x, x.y);
+      }
+      if (j > 0) {  // the product of the last tile is done with dS
+        ok = wait.warp(used + half, (j - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      tmem_st16(t_d + lane_base + wg * 16, q);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(d_full + wg);
+      if (lane == 0) mbar_arrive(d_full + half);
     }
     if (t1 > 0 && ok) ok = wait.warp(done, 0);
     tc_fence_after();
     const bool have = t1 > 0 && ok && end > 0;
     bf16 *dst = (bf16 *)p.dq.p + n * p.dq.s[0] + token * p.dq.s[1] + h * p.dq.s[2];
-    // a warpgroup writes half of the columns
-    constexpr int kHalf = DP / 2;
+    // a warpgroup writes a quarter of the columns
+    constexpr int kCols = DP / 4;
+    const int c0 = wg * kCols;
     if (t1 > 0 && ok) {
-#pragma unroll
-      for (int c = 0; c < kHalf; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(t_dq + lane_base + wg * kHalf + c, o);
-        tmem_wait_ld();
-        if (mine && have) store_bf16(dst + wg * kHalf + c, o, p.head_dim - wg * kHalf - c, p.scale);
-      }
+      uint32_t o[32];
+      if constexpr (kCols == 32) tmem_ld32(t_dq + lane_base + c0, o);
+      else tmem_ld16(t_dq + lane_base + c0, o);
+      tmem_wait_ld();
+      if (mine && have) store_bf16(dst + c0, o, min(kCols, p.head_dim - c0), p.scale);
     }
     if (mine && !have && wg == 0) store_zeros(dst, p.head_dim);
   }
-  leave(tmem, warp, fail, drain, p.err);
+  leave(tmem, warp == roles.product, fail, drain, p.err);
 }
 
 // ---------------------------------------------------------------------------
@@ -1053,7 +1161,7 @@ cudaError_t forward_tc(const AttnParams &p, const TcArgs &a, const CUtensorMap &
   const cudaError_t e = allow_smem<k_attn_tc<DP>>(sm);
   if (e != cudaSuccess) return e;
   const long long grid = (long long)p.batch * p.kv_heads * ((a.q_tiles + 1) / 2) * a.splits;
-  k_attn_tc<DP><<<(unsigned)grid, kTcThreads, sm, st>>>(mq, mk, mv, p, a);
+  k_attn_tc<DP><<<(unsigned)grid, threads_of(kFwdGroups), sm, st>>>(mq, mk, mv, p, a);
   return cudaGetLastError();
 }
 
@@ -1065,8 +1173,8 @@ cudaError_t backward_tc(const AttnParams &p, const TcArgs &a, const CUtensorMap 
   if (e == cudaSuccess) e = allow_smem<k_attn_dkv_tc<DP>>(sm);
   if (e != cudaSuccess) return e;
   const long long heads = (long long)p.batch * p.kv_heads;
-  k_attn_dq_tc<DP><<<(unsigned)(heads * a.q_tiles), kTcThreads, sm, st>>>(mq, mk, mv, mg, p, a);
-  k_attn_dkv_tc<DP><<<(unsigned)(heads * a.k_tiles), kTcThreads, sm, st>>>(mq, mk, mv, mg, p, a);
+  k_attn_dq_tc<DP><<<(unsigned)(heads * a.q_tiles), threads_of(kBwdGroups), sm, st>>>(mq, mk, mv, mg, p, a);
+  k_attn_dkv_tc<DP><<<(unsigned)(heads * a.k_tiles), threads_of(kBwdGroups), sm, st>>>(mq, mk, mv, mg, p, a);
   return cudaGetLastError();
 }
 
