@@ -594,13 +594,15 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
 // TMEM dV += P' dO, dK += dS' Q. A warpgroup takes 32 query columns: the
 // arithmetic is bound by its latencies, and four warps an SM quarter cover one
 // another's where two (64 columns each) left it idle two thirds of the time.
-// The columns go to the products in halves. Where TMEM has 128 columns left
-// (head sizes up to 64), P' and dS' have places of their own, and the next S'
-// and dP' are computed as soon as all warpgroups have loaded these:
-//   P0(j): dV   S free: S(j+1)   dS0(j): dK   P1(j): dV   dP free: dP(j+1)   dS1(j): dK
-// Else they replace S' and dP', and a half of the next one follows the product
-// that reads them:
-//   P0(j): dV, S0(j+1)   dS0(j): dK, dP0(j+1)   P1(j): dV, S1(j+1)   dS1(j): dK, dP1(j+1)
+// The columns go to the products in halves, which the product thread serves in
+// turn. Where TMEM has 128 columns left (head sizes up to 64), P' and dS' have
+// places of their own, and a half of the next S' or dP' is computed as soon as
+// its warpgroups have loaded this one:
+//   P0(j): dV   S0 free: S0(j+1)   dS0(j): dK   dP0 free: dP0(j+1)   P1(j): ...
+// Else they replace S' and dP', whose next half follows the product that reads
+// them. (One product for both halves of S' and dP' takes the tensor cores 20 %
+// less, but holds both halves to one step, and their exponentials collide:
+// 196 us against 173 at 12 heads of 6272 causal tokens, head size 64.)
 // The order of the sums is fixed in both.
 // ---------------------------------------------------------------------------
 
@@ -625,8 +627,8 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   float *row_sums = reinterpret_cast<float *>(sg + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sg + L::kStages * L::kTile + L::kRowSums);
   uint64_t *kv_full = bars, *s_full = bars + 1, *g_full = bars + 3, *p_full = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *s_free = bars + 13, *g_free = bars + 14, *used = bars + 15, *full = bars + 17, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 17 + 2 * L::kStages);
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *s_free = bars + 13, *g_free = bars + 15, *used = bars + 17, *full = bars + 19, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 19 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   constexpr Roles roles(kBwdGroups);
   const int warp = threadIdx.x >> 5;
@@ -644,8 +646,8 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 17; b++)
-      mbar_init(b, b >= p_full && b < done ? 8 : b == s_free || b == g_free ? 16 : b >= s_full && b < g_full ? 2 : 1);
+    for (uint64_t *b = bars; b < bars + 19; b++)
+      mbar_init(b, (b >= p_full && b < done) || (b >= s_free && b < used) ? 8 : b >= s_full && b < g_full ? 2 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
@@ -724,7 +726,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     const uint64_t dk = smem_desc(smem_u32(sk)), dv = smem_desc(smem_u32(sv)), dq = smem_desc(smem_u32(sq)),
                    dg = smem_desc(smem_u32(sg)), dq_mn = desc_mn(smem_u32(sq)), dg_mn = desc_mn(smem_u32(sg));
     constexpr uint32_t kStep = L::kTile >> 4;
-    const uint32_t id_s = instr_desc(1, 64), id_s2 = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
+    const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
     bool ok = wait(kv_full, 0) && wait(full, 0) && (t0 != clear_at || cleared(wait, ask, clean));
 #pragma unroll 1
@@ -745,21 +747,11 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         tc_fence_after();
         mma_tmem<64>(t_dv, t_p + w * p_step, dg_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0, p_gap);
         if (more && kApart) {
-          if (w == 0) {
-            ok = wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean)) && wait(s_free, parity);
-            if (!ok) break;
-            tc_fence_after();
-            mma_rows<DP>(t_s, dk, dq + s1 * kStep, nk, id_s2);
-            mma_commit(s_full);
-            mma_commit(s_full + 1);
-          } else {
-            ok = wait(g_free, parity);
-            if (!ok) break;
-            tc_fence_after();
-            mma_rows<DP>(t_g, dv, dg + s1 * kStep, nk, id_s2);
-            mma_commit(g_full);
-            mma_commit(g_full + 1);
-          }
+          ok = (w || (wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean)))) && wait(s_free + w, parity);
+          if (!ok) break;
+          tc_fence_after();
+          mma_rows<DP>(t_s + w * 64, dk, dq + s1 * kStep + w * kHalfRows, nk, id_s);
+          mma_commit(s_full + w);
         } else if (more) {
           if (w == 0) ok = wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean));
           if (!ok) break;
@@ -772,7 +764,12 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         mma_tmem<64>(t_dk, t_d + w * p_step, dq_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0, p_gap);
         if (kApart) mma_commit(used + w);
         if (w == 1) mma_commit(empty + s);
-        if (more && !kApart) {
+        if (kApart && more) {
+          ok = wait(g_free + w, parity);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        if (more) {
           mma_rows<DP>(t_g + w * 64, dv, dg + s1 * kStep + w * kHalfRows, nk, id_s);
           mma_commit(g_full + w);
         }
@@ -805,7 +802,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       if constexpr (kApart) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(s_free);
+        if (lane == 0) mbar_arrive(s_free + half);
       }
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
@@ -842,7 +839,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       if constexpr (kApart) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(g_free);
+        if (lane == 0) mbar_arrive(g_free + half);
       }
       if (masked) {
 #pragma unroll
@@ -890,9 +887,9 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 // ---------------------------------------------------------------------------
 // Backward, dQ: one query tile past the key tiles it sees. S = Q K' and
 // dP = dO V' are recomputed, dQ += dS K from TMEM. The warpgroups take 32 key
-// columns each; dS has a TMEM place of its own, and the next S and dP are
-// computed as soon as all warpgroups have loaded these:
-//   S free: S(j+1)   dS0(j): dQ   dP free: dP(j+1)   dS1(j): dQ
+// columns each; dS has a TMEM place of its own, and a half of the next S or dP
+// is computed as soon as its warpgroups have loaded this one:
+//   S0 free: S0(j+1)   dS0(j): dQ   dP0 free: dP0(j+1)   S1 free: ...
 // A thread's lse and delta stay in registers. This pass runs first and leaves
 // the row sums delta in the workspace for the other.
 // ---------------------------------------------------------------------------
@@ -908,9 +905,9 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   uint8_t *sq = base, *sg = sq + L::kTile, *sk = sg + L::kTile, *sv = sk + L::kStages * L::kTile;
   float *row_sums = reinterpret_cast<float *>(sv + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile + L::kRowSums);
-  uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 3, *s_free = bars + 5, *g_free = bars + 6, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *used = bars + 13, *full = bars + 15, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 15 + 2 * L::kStages);
+  uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 3, *s_free = bars + 5, *d_full = bars + 7,
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *used = bars + 13, *g_free = bars + 15, *full = bars + 17, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 17 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   constexpr Roles roles(kBwdGroups);
   const int warp = threadIdx.x >> 5;
@@ -927,7 +924,8 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 15; b++) mbar_init(b, b == s_free || b == g_free ? 16 : b == d_full || b == d_full + 1 ? 8 : 1);
+    for (uint64_t *b = bars; b < bars + 17; b++)
+      mbar_init(b, (b >= s_free && b < done) || b >= g_free ? 8 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
@@ -964,14 +962,15 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     const uint64_t dq = smem_desc(smem_u32(sq)), dg = smem_desc(smem_u32(sg)), dk = smem_desc(smem_u32(sk)),
                    dv = smem_desc(smem_u32(sv)), dk_mn = desc_mn(smem_u32(sk));
     constexpr uint32_t kStep = L::kTile >> 4;
-    const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
+    const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
     bool ok = wait(q_full, 0) && wait(full, 0) && (clear_at != 0 || cleared(wait, ask, clean));
-    if (ok) {
-      mma_rows<DP>(t_s, dq, dk, nk, id_s);
-      mma_commit(s_full);
-      mma_rows<DP>(t_g, dg, dv, nk, id_s);
-      mma_commit(g_full);
+#pragma unroll 1
+    for (int w = 0; w < 2 && ok; w++) {
+      mma_rows<DP>(t_s + w * 64, dq, dk + w * kHalfRows, nk, id_s);
+      mma_commit(s_full + w);
+      mma_rows<DP>(t_g + w * 64, dg, dv + w * kHalfRows, nk, id_s);
+      mma_commit(g_full + w);
     }
     int s = 0, use = 0;
     for (int j = 0; j < t1 && ok; j++) {
@@ -980,12 +979,11 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 #pragma unroll 1
       for (int w = 0; w < 2; w++) {
         if (more) {
-          ok = (w || (wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean)))) &&
-               wait(w ? g_free : s_free, parity);
+          ok = (w || (wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean)))) && wait(s_free + w, parity);
           if (!ok) break;
           tc_fence_after();
-          mma_rows<DP>(w ? t_g : t_s, w ? dg : dq, (w ? dv : dk) + s1 * kStep, nk, id_s);
-          mma_commit(w ? g_full : s_full);
+          mma_rows<DP>(t_s + w * 64, dq, dk + s1 * kStep + w * kHalfRows, nk, id_s);
+          mma_commit(s_full + w);
         }
         ok = wait(d_full + w, parity);
         if (!ok) break;
@@ -993,6 +991,13 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         mma_tmem<64>(t_dq, t_d + w * 32, dk_mn + s * kStep + w * kHalfRows, id_o, j == 0 && w == 0);
         mma_commit(used + w);
         if (w == 1) mma_commit(empty + s);
+        if (more) {
+          ok = wait(g_free + w, parity);
+          if (!ok) break;
+          tc_fence_after();
+          mma_rows<DP>(t_g + w * 64, dg, dv + s1 * kStep + w * kHalfRows, nk, id_s);
+          mma_commit(g_full + w);
+        }
       }
       s = s1, use = use1;
     }
@@ -1032,7 +1037,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     for (int j = 0; j < t1; j++) {
       const int left = end - j * 128 - wg * 32;
       const bool masked = __any_sync(0xffffffffu, left < 32);
-      ok = wait.warp(s_full, j & 1);
+      ok = wait.warp(s_full + half, j & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t r[32];
@@ -1040,13 +1045,13 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_free);
+      if (lane == 0) mbar_arrive(s_free + half);
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, shift2);
         r[c] = __float_as_uint(ex2(x.x)), r[c + 1] = __float_as_uint(ex2(x.y));
       }
-      ok = wait.warp(g_full, j & 1);
+      ok = wait.warp(g_full + half, j & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t g[32], q[16];
@@ -1054,7 +1059,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(g_free);
+      if (lane == 0) mbar_arrive(g_free + half);
       if (masked) {
 #pragma unroll
         for (int c = 0; c < 32; c++)
