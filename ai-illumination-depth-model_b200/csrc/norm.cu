@@ -24,6 +24,19 @@ using namespace tok;
 
 constexpr int kThreads = 256;
 
+// VW values of w or b; vectors when they are aligned like the columns (VW 4:
+// the caller checked).
+template <int VW>
+__device__ __forceinline__ void load_params(const float *p, float (&o)[VW]) {
+  if constexpr (VW == 4) {
+    const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+    o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VW; j++) o[j] = __ldg(p + j);
+  }
+}
+
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float *red) {
   v = warp_sum(v);
@@ -39,58 +52,72 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
   return v;
 }
 
-template <typename T, int VW, int VPT, int LANES>
+// A thread group of LANES threads takes ROWS rows at once: their loads are in
+// flight together, and w and b (from the L1) are read once for all of them.
+template <typename T, int VW, int VPT, int LANES, int ROWS>
 __global__ void __launch_bounds__(kThreads) k_norm(const T *__restrict__ x, long long xs, long long rows, int c,
                                                    const float *__restrict__ w, const float *__restrict__ b, float eps,
                                                    T *__restrict__ y, long long ys, float *mean, float *rstd) {
   __shared__ float red[kThreads / 32];
   const int lane = threadIdx.x % LANES;
-  const long long row = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  if (row >= rows) return;  // uniform over the threads of a row
-  const T *xr = x + row * xs;
-  float v[VPT][VW];
-  float s = 0;
+  const long long row = ((long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES) * ROWS;
+  if (row >= rows) return;  // uniform over the threads of a group
+  float v[ROWS][VPT][VW];
 #pragma unroll
-  for (int i = 0; i < VPT; i++) {
-    const int col = (i * LANES + lane) * VW;
-    if (col < c) {
-      Pack<T, VW>::load(xr + col, v[i]);
-    } else {
+  for (int k = 0; k < ROWS; k++)
 #pragma unroll
-      for (int j = 0; j < VW; j++) v[i][j] = 0;
+    for (int i = 0; i < VPT; i++) {
+      const int col = (i * LANES + lane) * VW;
+      if (col < c && row + k < rows) {
+        Pack<T, VW>::load(x + (row + k) * xs + col, v[k][i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VW; j++) v[k][i][j] = 0;
+      }
     }
+  const float inv = 1.0f / c;
+  float r[ROWS];
 #pragma unroll
-    for (int j = 0; j < VW; j++) s += v[i][j];
-  }
-  const float mu = row_sum<LANES>(s, red) / c;
-  float q = 0;
+  for (int k = 0; k < ROWS; k++) {
+    float s = 0;
 #pragma unroll
-  for (int i = 0; i < VPT; i++) {
-    const int col = (i * LANES + lane) * VW;
+    for (int i = 0; i < VPT; i++)
 #pragma unroll
-    for (int j = 0; j < VW; j++) {
-      v[i][j] -= mu;
-      if (col < c) q += v[i][j] * v[i][j];
+      for (int j = 0; j < VW; j++) s += v[k][i][j];
+    const float mu = row_sum<LANES>(s, red) * inv;
+    float q = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+      const bool in = (i * LANES + lane) * VW < c;
+#pragma unroll
+      for (int j = 0; j < VW; j++) {
+        v[k][i][j] -= mu;
+        if (in) q += v[k][i][j] * v[k][i][j];
+      }
+    }
+    r[k] = 1.0f / sqrtf(row_sum<LANES>(q, red) * inv + eps);
+    if (lane == 0 && row + k < rows) {
+      if (mean) mean[row + k] = mu;
+      if (rstd) rstd[row + k] = r[k];
     }
   }
-  const float r = 1.0f / sqrtf(row_sum<LANES>(q, red) / c + eps);
-  if (lane == 0) {
-    if (mean) mean[row] = mu;
-    if (rstd) rstd[row] = r;
-  }
-  T *yr = y + row * ys;
 #pragma unroll
   for (int i = 0; i < VPT; i++) {
     const int col = (i * LANES + lane) * VW;
     if (col >= c) break;
-    float o[VW];
+    float wv[VW], bv[VW];
 #pragma unroll
-    for (int j = 0; j < VW; j++) {
-      o[j] = v[i][j] * r;
-      if (w) o[j] *= w[col + j];
-      if (b) o[j] += b[col + j];
+    for (int j = 0; j < VW; j++) wv[j] = 1, bv[j] = 0;
+    if (w) load_params<VW>(w + col, wv);
+    if (b) load_params<VW>(b + col, bv);
+#pragma unroll
+    for (int k = 0; k < ROWS; k++) {
+      if (row + k >= rows) break;
+      float o[VW];
+#pragma unroll
+      for (int j = 0; j < VW; j++) o[j] = fmaf(v[k][i][j] * r[k], wv[j], bv[j]);
+      Pack<T, VW>::store(y + (row + k) * ys + col, o);
     }
-    Pack<T, VW>::store(yr + col, o);
   }
 }
 
@@ -124,8 +151,10 @@ __global__ void __launch_bounds__(kThreads) k_norm_long(const T *__restrict__ x,
   }
 }
 
-// part: [gridDim.x][2][c], or null when neither dw nor db is wanted.
-template <typename T, int VW, int VPT, int LANES>
+// part: [gridDim.x][2][c], or null when neither dw nor db is wanted. PRE: the
+// next row's loads are issued before this row's sums, where the registers
+// allow it.
+template <typename T, int VW, int VPT, int LANES, bool PRE>
 __global__ void __launch_bounds__(kThreads) k_norm_bwd(const T *__restrict__ dy, long long dys,
                                                        const T *__restrict__ x, long long xs, long long rows, int c,
                                                        const float *__restrict__ w, const float *__restrict__ mean,
@@ -135,40 +164,58 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd(const T *__restrict__ dy,
   __shared__ float red[kThreads / 32];
   constexpr int kRows = kThreads / LANES;
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  typedef typename RawPack<T, VW>::type Raw;
   float aw[VPT][VW], ab[VPT][VW];
 #pragma unroll
   for (int i = 0; i < VPT; i++)
 #pragma unroll
     for (int j = 0; j < VW; j++) aw[i][j] = ab[i][j] = 0;
-  for (long long row = (long long)blockIdx.x * kRows + group; row < rows; row += (long long)gridDim.x * kRows) {
-    const T *xr = x + row * xs, *gr = dy + row * dys;
-    const float mu = mean[row], r = rstd[row];
-    float h[VPT][VW], g[VPT][VW];
-    float s0 = 0, s1 = 0;
+  Raw rx[VPT], rg[VPT];
+  float mu = 0, r = 0;
+  const float inv = 1.0f / c;
+  const long long step = (long long)gridDim.x * kRows;
+  auto fetch = [&](long long row) {
+    if (row >= rows) return;
+    mu = __ldg(mean + row), r = __ldg(rstd + row);
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
       const int col = (i * LANES + lane) * VW;
       if (col < c) {
-        Pack<T, VW>::load(xr + col, h[i]);
-        Pack<T, VW>::load(gr + col, g[i]);
+        rx[i] = *reinterpret_cast<const Raw *>(x + row * xs + col);
+        rg[i] = *reinterpret_cast<const Raw *>(dy + row * dys + col);
       }
     }
+  };
+  const long long row0 = (long long)blockIdx.x * kRows + group;
+  if (PRE) fetch(row0);
+  for (long long row = row0; row < rows; row += step) {
+    if (!PRE) fetch(row);
+    float h[VPT][VW], g[VPT][VW];
+    float s0 = 0, s1 = 0;
+    const float rs = r;
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
       const int col = (i * LANES + lane) * VW;
       if (col >= c) break;
+      RawPack<T, VW>::unpack(rx[i], h[i]);
+      RawPack<T, VW>::unpack(rg[i], g[i]);
+      float wv[VW];
+#pragma unroll
+      for (int j = 0; j < VW; j++) wv[j] = 1;
+      if (w) load_params<VW>(w + col, wv);
 #pragma unroll
       for (int j = 0; j < VW; j++) {
-        h[i][j] = (h[i][j] - mu) * r;
-        aw[i][j] += g[i][j] * h[i][j];
+        h[i][j] = (h[i][j] - mu) * rs;
+        aw[i][j] = fmaf(g[i][j], h[i][j], aw[i][j]);
         ab[i][j] += g[i][j];
-        if (w) g[i][j] *= __ldg(w + col + j);
+        g[i][j] *= wv[j];
         s0 += g[i][j];
-        s1 += g[i][j] * h[i][j];
+        s1 = fmaf(g[i][j], h[i][j], s1);
       }
     }
-    s0 = row_sum<LANES>(s0, red) / c;
-    s1 = row_sum<LANES>(s1, red) / c;
+    if (PRE) fetch(row + step);
+    s0 = row_sum<LANES>(s0, red) * inv;
+    s1 = row_sum<LANES>(s1, red) * inv;
     if (dx) {
       T *dr = dx + row * dxs;
 #pragma unroll
@@ -177,7 +224,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd(const T *__restrict__ dy,
         if (col >= c) break;
         float o[VW];
 #pragma unroll
-        for (int j = 0; j < VW; j++) o[j] = r * (g[i][j] - s0 - h[i][j] * s1);
+        for (int j = 0; j < VW; j++) o[j] = rs * (g[i][j] - s0 - h[i][j] * s1);
         Pack<T, VW>::store(dr + col, o);
       }
     }
@@ -247,21 +294,23 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd_long(const T *__restrict_
   }
 }
 
-// Column sums of part ([n][2c]) in a fixed order: 32 columns a CTA, its 32
-// warps take every 32nd row, then the warps' sums are added.
-__global__ void __launch_bounds__(1024) k_norm_reduce(const float *__restrict__ part, int n, int c, float *dw,
-                                                      float *db) {
-  __shared__ float s[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + tx;
+// Column sums of part ([n][2c]) in a fixed order: a CTA takes 8 columns, its 32
+// groups of 8 threads every 32nd row, then the groups' sums are added.
+__global__ void __launch_bounds__(256) k_norm_reduce(const float *__restrict__ part, int n, int c, float *dw,
+                                                     float *db) {
+  __shared__ float s[8][33];
+  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+  const int col = blockIdx.x * 8 + tx;
   float t = 0;
-  if (col < 2 * c)
+  if (col < 2 * c) {
+#pragma unroll 4
     for (int i = ty; i < n; i += 32) t += part[(size_t)i * 2 * c + col];
-  s[ty][tx] = t;
+  }
+  s[tx][ty] = t;
   __syncthreads();
-  t = warp_sum(s[tx][ty]);
-  const int o = blockIdx.x * 32 + ty;
-  if (tx == 0 && o < 2 * c) {
+  const int o = blockIdx.x * 8 + (threadIdx.x >> 5);
+  t = warp_sum(s[threadIdx.x >> 5][threadIdx.x & 31]);
+  if ((threadIdx.x & 31) == 0 && o < 2 * c) {
     if (o < c) {
       if (dw) dw[o] = t;
     } else if (db) {
@@ -289,37 +338,49 @@ void launch(const NormArgs &a, bool bwd) {
   constexpr int kRows = kThreads / LANES;
   const T *x = (const T *)a.x;
   if (!bwd) {
-    k_norm<T, VW, VPT, LANES><<<(unsigned)((a.rows + kRows - 1) / kRows), kThreads, 0, a.st>>>(
-        x, a.xs, a.rows, a.c, a.w, a.b, a.eps, (T *)a.y, a.ys, a.mean, a.rstd);
+    // two rows a warp once there are enough rows to fill the GPU with half the
+    // warps, and registers for both
+    constexpr int kTwo = LANES == 32 && VW * VPT <= 24 ? 2 : 1;
+    if (kTwo == 2 && a.rows >= 148 * 64 * 2)
+      k_norm<T, VW, VPT, LANES, kTwo><<<(unsigned)((a.rows + 2 * kRows - 1) / (2 * kRows)), kThreads, 0, a.st>>>(
+          x, a.xs, a.rows, a.c, a.w, a.b, a.eps, (T *)a.y, a.ys, a.mean, a.rstd);
+    else
+      k_norm<T, VW, VPT, LANES, 1><<<(unsigned)((a.rows + kRows - 1) / kRows), kThreads, 0, a.st>>>(
+          x, a.xs, a.rows, a.c, a.w, a.b, a.eps, (T *)a.y, a.ys, a.mean, a.rstd);
   } else {
+    constexpr bool kPre = VW * VPT * sizeof(T) <= 64;
     const size_t sm = LANES == kThreads || !a.part ? 0 : (size_t)kRows * a.c * sizeof(float);
-    k_norm_bwd<T, VW, VPT, LANES><<<a.blocks, kThreads, sm, a.st>>>((const T *)a.dy, a.dys, x, a.xs, a.rows, a.c, a.w,
-                                                                  a.mean, a.rstd, (T *)a.y, a.ys, a.part);
+    k_norm_bwd<T, VW, VPT, LANES, kPre><<<a.blocks, kThreads, sm, a.st>>>(
+        (const T *)a.dy, a.dys, x, a.xs, a.rows, a.c, a.w, a.mean, a.rstd, (T *)a.y, a.ys, a.part);
   }
 }
 
-// Smallest register tile that holds a row.
+// Smallest register tile that holds a row of c columns.
 template <typename T, int VW>
 bool pick(const NormArgs &a, bool bwd) {
-  constexpr int e = VW == 1 ? 4 : VW;  // elements a thread holds at least
-  constexpr int u = e / VW;
-  if (a.c <= 32 * e) launch<T, VW, u, 32>(a, bwd);
-  else if (a.c <= 64 * e) launch<T, VW, 2 * u, 32>(a, bwd);
-  else if (a.c <= 128 * e) launch<T, VW, 4 * u, 32>(a, bwd);
-  else if (a.c <= 256 * e && e <= 4) launch<T, VW, (e <= 4 ? 8 * u : u), 32>(a, bwd);
-  else if (a.c <= 256 * e) launch<T, VW, u, 256>(a, bwd);
-  else if (a.c <= 512 * e) launch<T, VW, 2 * u, 256>(a, bwd);
-  else if (a.c <= 1024 * e && e <= 4) launch<T, VW, (e <= 4 ? 4 * u : u), 256>(a, bwd);
+  constexpr int u = 4 / VW;  // a thread holds at least 4 columns
+  const int quads = (a.c + 3) / 4;  // groups of 4 columns
+  if (quads <= 32) launch<T, VW, u, 32>(a, bwd);
+  else if (quads <= 64) launch<T, VW, 2 * u, 32>(a, bwd);
+  else if (quads <= 96) launch<T, VW, 3 * u, 32>(a, bwd);
+  else if (quads <= 128) launch<T, VW, 4 * u, 32>(a, bwd);
+  else if (quads <= 192) launch<T, VW, 6 * u, 32>(a, bwd);
+  else if (quads <= 256) launch<T, VW, 8 * u, 32>(a, bwd);
+  else if (quads <= 512) launch<T, VW, 2 * u, 256>(a, bwd);
+  else if (quads <= 1024) launch<T, VW, 4 * u, 256>(a, bwd);
   else return false;
   return true;
 }
 
 template <typename T>
 void dispatch(const NormArgs &a, bool bwd) {
-  constexpr int V = 16 / sizeof(T);
-  bool vec = a.c % V == 0 && a.xs % V == 0 && a.ys % V == 0 && aligned16(a.x) && aligned16(a.y);
-  if (bwd) vec = vec && a.dys % V == 0 && aligned16(a.dy);
-  if (vec ? pick<T, V>(a, bwd) : pick<T, 1>(a, bwd)) return;
+  // four columns at a time: 8 or 16 bytes of T, 16 bytes of w and b
+  auto fits = [](const void *p, long long stride) {
+    return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && stride % 4 == 0;
+  };
+  const bool vec = a.c % 4 == 0 && fits(a.x, a.xs) && fits(a.y, a.ys) && (!bwd || fits(a.dy, a.dys)) && aligned16(a.w) &&
+                   aligned16(a.b);
+  if (vec ? pick<T, 4>(a, bwd) : pick<T, 1>(a, bwd)) return;
   if (!bwd)
     k_norm_long<T><<<(unsigned)a.rows, kThreads, 0, a.st>>>((const T *)a.x, a.xs, a.c, a.w, a.b, a.eps, (T *)a.y, a.ys,
                                                             a.mean, a.rstd);
@@ -360,7 +421,7 @@ cudaError_t layer_norm_backward(int T, const void *dy, long long dys, const void
     if (T == 0) dispatch<float>(a, true);
     else dispatch<bf16>(a, true);
   }
-  if (dw || db) k_norm_reduce<<<(2 * c + 31) / 32, 1024, 0, st>>>(ws, a.blocks, c, dw, db);
+  if (dw || db) k_norm_reduce<<<(2 * c + 7) / 8, 256, 0, st>>>(ws, a.blocks, c, dw, db);
   return cudaGetLastError();
 }
 

@@ -117,9 +117,8 @@ struct illumina_adamw {
     long long chunk0, chunk1;
   };
   std::vector<Group> groups;
-  void *memory = nullptr;  // clock, tensor table, chunk table
+  void *memory = nullptr;  // clock, chunk table
   gpu::AdamwClock *clock = nullptr;
-  gpu::AdamwTensor *table = nullptr;
   gpu::AdamwChunk *chunks = nullptr;
   gpu::AdamwState state{};
   ~illumina_adamw() {
@@ -274,30 +273,30 @@ illumina_status illumina_adamw_create(const illumina_adamw_options *o, illumina_
   opt->device = o->device, opt->tensors = o->tensors, opt->bits = o->moment_bits;
   opt->grad_precision = o->grad_precision, opt->blocks = blocks;
   opt->counts.assign(o->counts, o->counts + o->tensors);
-  std::vector<gpu::AdamwTensor> table(o->tensors);
   std::vector<gpu::AdamwChunk> chunks;
   long long first = 0;
   for (int i = 0; i < o->tensors; i++) {
     const long long n = blocks_of(o->counts[i]);
     require(n == 0 || (o->params[i] && aligned(o->params[i], 4)), "adamw: parameter pointer missing or misaligned");
-    table[i] = {o->params[i], o->counts[i], first, o->decay ? o->decay[i] != 0 : 1, 0};
-    first += n;
     if (opt->groups.empty() || i - opt->groups.back().first >= gpu::kAdamwGrads)
       opt->groups.push_back({i, i, (long long)chunks.size(), (long long)chunks.size()});
-    for (long long b = 0; b < n; b += gpu::kAdamwChunk) chunks.push_back({i, (int)b});
+    const int decay = o->decay ? o->decay[i] != 0 : 1;
+    constexpr long long most = gpu::kAdamwChunk * gpu::kAdamwBlock;
+    for (long long b = 0; b < n; b += gpu::kAdamwChunk) {
+      const long long at = b * gpu::kAdamwBlock, left = o->counts[i] - at;
+      chunks.push_back({o->params[i] + at, first + b, i, (int)b, (int)(left < most ? left : most), decay});
+    }
+    first += n;
     opt->groups.back().end = i + 1;
     opt->groups.back().chunk1 = (long long)chunks.size();
   }
   OnDevice on(o->device);
-  const size_t a = 256, tb = table.size() * sizeof(table[0]), cb = chunks.size() * sizeof(chunks[0]);
-  const size_t at_chunks = a + (tb + 255) / 256 * 256;
-  cuda_check(cudaMalloc(&opt->memory, at_chunks + cb), "adamw: cudaMalloc");
+  const size_t a = 256, cb = chunks.size() * sizeof(chunks[0]);
+  cuda_check(cudaMalloc(&opt->memory, a + cb), "adamw: cudaMalloc");
   char *base = (char *)opt->memory;
   opt->clock = (gpu::AdamwClock *)base;
-  opt->table = (gpu::AdamwTensor *)(base + a);
-  opt->chunks = (gpu::AdamwChunk *)(base + at_chunks);
+  opt->chunks = (gpu::AdamwChunk *)(base + a);
   cuda_check(cudaMemset(base, 0, a), "adamw: clear");
-  cuda_check(cudaMemcpy(opt->table, table.data(), tb, cudaMemcpyHostToDevice), "adamw: upload");
   cuda_check(cudaMemcpy(opt->chunks, chunks.data(), cb, cudaMemcpyHostToDevice), "adamw: upload");
   opt->state.m = o->m, opt->state.v = o->v, opt->state.m_scale = o->m_scale, opt->state.v_scale = o->v_scale;
   *out = opt.release();
@@ -336,7 +335,7 @@ illumina_status illumina_adamw_step(illumina_adamw *opt, const void *const *grad
     if (group.chunk1 == group.chunk0) continue;
     gpu::AdamwGrads gr{};
     for (int i = group.first; i < group.end; i++) gr.p[i - group.first] = grads[i];
-    cuda_check(gpu::adamw_step(opt->bits, opt->grad_precision, opt->table, opt->chunks + group.chunk0,
+    cuda_check(gpu::adamw_step(opt->bits, opt->grad_precision, opt->chunks + group.chunk0,
                                group.chunk1 - group.chunk0, group.first, gr, opt->state, d, h->lr_device, opt->clock,
                                g == last - 1, (cudaStream_t)stream),
                "adamw_step");

@@ -62,6 +62,28 @@ struct Pack {
   }
 };
 
+// VW consecutive elements as they lie in memory, and their values.
+template <typename T, int VW>
+struct RawPack;
+template <>
+struct RawPack<float, 4> {
+  typedef float4 type;
+  static __device__ __forceinline__ void unpack(float4 v, float (&o)[4]) { o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w; }
+};
+template <>
+struct RawPack<bf16, 4> {
+  typedef uint2 type;
+  static __device__ __forceinline__ void unpack(uint2 v, float (&o)[4]) {
+    o[0] = __uint_as_float(v.x << 16), o[1] = __uint_as_float(v.x & 0xffff0000u);
+    o[2] = __uint_as_float(v.y << 16), o[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+};
+template <typename T>
+struct RawPack<T, 1> {
+  typedef T type;
+  static __device__ __forceinline__ void unpack(T v, float (&o)[1]) { o[0] = to_f32(v); }
+};
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

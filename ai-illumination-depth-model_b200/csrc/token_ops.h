@@ -82,15 +82,12 @@ cudaError_t attention_tc(const AttnParams &p, bool backward, cudaStream_t st);
 constexpr int kAdamwBlock = 256;   // elements that share the scales of 8-bit moments
 constexpr int kAdamwChunk = 8;     // blocks one CTA updates
 constexpr int kAdamwGrads = 440;   // gradient pointers one launch carries
-struct AdamwTensor {
-  float *param;
-  long long count;
-  long long first_block;  // of the flat moments
-  int decay;
-  int pad;
-};
+// Up to kAdamwChunk blocks of one tensor.
 struct AdamwChunk {
-  int tensor, block;  // first block within the tensor
+  float *param;           // its first element
+  long long state_block;  // of the flat moments
+  int tensor, block;      // first block within the tensor
+  int elems, decay;
 };
 struct AdamwState {
   void *m, *v;             // f32 or int8 / uint8, [blocks * kAdamwBlock]
@@ -110,12 +107,12 @@ struct AdamwHyper {
 struct AdamwGrads {
   const void *p[kAdamwGrads];
 };
-// One launch over chunks [0, n_chunks) of tensors [first_tensor, ...), whose
-// gradients are grads.p[tensor - first_tensor]. `last`: the launch ends the
-// step and advances the clock.
-cudaError_t adamw_step(int bits, int grad_type, const AdamwTensor *tensors, const AdamwChunk *chunks, long long n_chunks,
-                       int first_tensor, const AdamwGrads &grads, const AdamwState &state, const AdamwHyper &h,
-                       const float *lr_device, AdamwClock *clock, bool last, cudaStream_t st);
+// One launch over `chunks` of tensors [first_tensor, ...), whose gradients are
+// grads.p[tensor - first_tensor]. `last`: the launch ends the step and advances
+// the clock.
+cudaError_t adamw_step(int bits, int grad_type, const AdamwChunk *chunks, long long n_chunks, int first_tensor,
+                       const AdamwGrads &grads, const AdamwState &state, const AdamwHyper &h, const float *lr_device,
+                       AdamwClock *clock, bool last, cudaStream_t st);
 // The f32 values of 8-bit moments.
 cudaError_t adamw_moments(const AdamwState &state, long long blocks, float *m, float *v, cudaStream_t st);
 
