@@ -253,7 +253,8 @@ cudaError_t adamw_step(int bits, int grad_type, const AdamwChunk *chunks, long l
                        const AdamwGrads &grads, const AdamwState &state, const AdamwHyper &h, const float *lr_device,
                        AdamwClock *clock, bool last, cudaStream_t st) {
   const int nc = (int)n;
-  const unsigned grid = (unsigned)(n < 3 * 148 ? n : 3 * 148);
+  const long long resident = (bits == 32 ? 2 : 3) * 148;  // by registers
+  const unsigned grid = (unsigned)(n < resident ? n : resident);
   if (bits == 32 && grad_type == 0)
     k_adamw<32, float><<<grid, kThreads, 0, st>>>(chunks, nc, first_tensor, grads, state, h, lr_device, clock, last);
   else if (bits == 32)
