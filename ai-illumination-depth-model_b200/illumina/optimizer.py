@@ -5,13 +5,11 @@ are those of weights.py or any other float32 torch CUDA tensors.
 from __future__ import annotations
 
 import ctypes as C
-from operator import attrgetter
 
-from ._lib import (INVALID_ARG, PRECISION_BF16, PRECISION_F32, AdamwHyper, AdamwOptions, IlluminaError, check, lib, ptr)
-from .ops import _On, _require, _vector
+from ._lib import PRECISION_BF16, PRECISION_F32, AdamwOptions, check, lib, ptr
+from .ops import _load, _On, _require
 
 BLOCK = 256  # ILLUMINA_ADAMW_BLOCK
-_DTYPE = attrgetter("dtype")
 
 
 class AdamW:
@@ -59,39 +57,16 @@ class AdamW:
         handle = C.c_void_p()
         check(lib().illumina_adamw_create(C.byref(options), C.byref(handle)))
         self._h = handle
-        self._counts, self._pointers = list(counts), C.c_void_p * n
+        self._stepper = _load().Stepper(handle.value, list(counts), dev.index, gradDtype == torch.bfloat16)
 
     def step(self, grads, stream=None):
         """One step; grads: one contiguous tensor of gradDtype for each parameter, of its element count."""
-        import torch
         _require(self._h is not None, "adamw: the optimizer was destroyed")
-        grads = list(grads)
-        if len(grads) != len(self._counts):
-            _require(False, "adamw: one gradient for each parameter is needed")
-        # one pass of C-level calls for each property: this runs over every tensor in every step
-        tensor = torch.Tensor
-        try:
-            fits = (set(map(_DTYPE, grads)) == {self.gradDtype} and set(map(tensor.get_device, grads)) == {self.device.index}
-                    and list(map(tensor.numel, grads)) == self._counts and all(map(tensor.is_contiguous, grads)))
-        except (TypeError, AttributeError):  # not tensors
-            fits = False
-        if not fits:
-            self._refuse(torch, grads)
-        hyper = AdamwHyper(beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, weight_decay=self.weightDecay)
-        if isinstance(self.lr, torch.Tensor):
-            hyper.lr_device = _vector(torch, "lr", self.lr, 1, self.device)
-        else:
-            hyper.lr = self.lr
-        pointers = self._pointers(*map(tensor.data_ptr, grads))
-        with _On(torch, self.device, stream) as handle:
-            check(lib().illumina_adamw_step(self._h, pointers, C.byref(hyper), handle))
-
-    def _refuse(self, torch, grads):
-        for i, (g, n) in enumerate(zip(grads, self._counts)):
-            if not (isinstance(g, torch.Tensor) and g.dtype == self.gradDtype and g.device == self.device and g.numel() == n
-                    and g.is_contiguous()):
-                raise IlluminaError(INVALID_ARG, f"adamw: gradient {i} must be {n} contiguous {str(self.gradDtype)[6:]} "
-                                                 f"values on {self.device}")
+        args = (grads, self.lr, *self.betas, self.eps, self.weightDecay)
+        if stream is None:
+            return self._stepper.step(*args)
+        with _On(self.device, stream):
+            return self._stepper.step(*args)
 
     def moments(self, stream=None):
         """The first and second moments as flat float32 tensors, every parameter from a multiple of 256 elements on.
@@ -100,7 +75,7 @@ class AdamW:
         _require(self._h is not None, "adamw: the optimizer was destroyed")
         if self.momentBits == 32:
             return self.m, self.v
-        with _On(torch, self.device, stream) as handle:
+        with _On(self.device, stream) as handle:
             m = torch.empty(self.blocks * BLOCK, dtype=torch.float32, device=self.device)
             v = torch.empty_like(m)
             check(lib().illumina_adamw_moments(self._h, m.data_ptr(), v.data_ptr(), handle))
@@ -109,10 +84,9 @@ class AdamW:
     @property
     def steps(self) -> int:
         """Steps taken (waits for the current stream)."""
-        import torch
         _require(self._h is not None, "adamw: the optimizer was destroyed")
         n = C.c_longlong(0)
-        with _On(torch, self.device, None) as handle:
+        with _On(self.device, None) as handle:
             check(lib().illumina_adamw_get_steps(self._h, C.byref(n), handle))
         return n.value
 
@@ -135,7 +109,7 @@ class AdamW:
         for name, x in mine.items():
             if x is not None:
                 x.copy_(state[name].reshape(x.shape))
-        with _On(torch, self.device, None) as handle:
+        with _On(self.device, None) as handle:
             check(lib().illumina_adamw_set_steps(self._h, int(state["step"]), handle))
 
     def destroy(self) -> None:

@@ -109,3 +109,19 @@ def test_adamw_blocks_and_refusals():
     refused(lib.illumina_adamw_step(None, None, None, None), "null")
     refused(lib.illumina_adamw_moments(None, None, None, None), "moments")
     assert lib.illumina_adamw_destroy(None) == _lib.OK
+
+
+def test_tensors_off_the_gpu_are_refused():
+    torch = pytest.importorskip("torch")
+    import illumina
+    from illumina import ops
+    x, q = torch.zeros(4, 8), torch.zeros(1, 4, 2, 8)
+    positions = torch.zeros(1, 4, dtype=torch.int32)
+    plan = illumina.createRotary(8, [4], device="cpu")
+    calls = [lambda: ops.layerNorm(x), lambda: ops.layerNormBackward(x, x, x[:, 0], x[:, 0]),
+             lambda: ops.rotary(q, positions, plan), lambda: ops.attention(q, q, q),
+             lambda: ops.attentionBackward(q, q, q, q, q, None), lambda: illumina.createOptimizer([x])]
+    for call in calls:
+        with pytest.raises(illumina.IlluminaError) as e:
+            call()
+        assert e.value.status == _lib.INVALID_ARG and "CUDA tensor" in str(e.value)
