@@ -627,8 +627,8 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   float *row_sums = reinterpret_cast<float *>(sg + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sg + L::kStages * L::kTile + L::kRowSums);
   uint64_t *kv_full = bars, *s_full = bars + 1, *g_full = bars + 3, *p_full = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *s_free = bars + 13, *g_free = bars + 15, *used = bars + 17, *full = bars + 19, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 19 + 2 * L::kStages);
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *s_free = bars + 13, *g_free = bars + 15, *full = bars + 17, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 17 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   constexpr Roles roles(kBwdGroups);
   const int warp = threadIdx.x >> 5;
@@ -646,8 +646,8 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 19; b++)
-      mbar_init(b, (b >= p_full && b < done) || (b >= s_free && b < used) ? 8 : b >= s_full && b < g_full ? 2 : 1);
+    for (uint64_t *b = bars; b < bars + 17; b++)
+      mbar_init(b, (b >= p_full && b < done) || b >= s_free ? 8 : b >= s_full && b < g_full ? 2 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
   }
@@ -762,7 +762,6 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         if (!ok) break;
         tc_fence_after();
         mma_tmem<64>(t_dk, t_d + w * p_step, dq_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0, p_gap);
-        if (kApart) mma_commit(used + w);
         if (w == 1) mma_commit(empty + s);
         if (kApart && more) {
           ok = wait(g_free + w, parity);
@@ -820,11 +819,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       uint32_t q[16];
 #pragma unroll
       for (int c = 0; c < 16; c++) q[c] = pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-      if (kApart && it > 0) {  // the products of the last tile are done with P' and dS'
-        ok = wait.warp(used + half, (it - 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-      }
+      // P's place is free: this S' was committed after the product that read it
       tmem_st16(tp, q);
       tmem_wait_st();
       tc_fence_before();
@@ -906,8 +901,8 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   float *row_sums = reinterpret_cast<float *>(sv + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile + L::kRowSums);
   uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 3, *s_free = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *used = bars + 13, *g_free = bars + 15, *full = bars + 17, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 17 + 2 * L::kStages);
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *g_free = bars + 13, *full = bars + 15, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 15 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   constexpr Roles roles(kBwdGroups);
   const int warp = threadIdx.x >> 5;
@@ -924,7 +919,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 17; b++)
+    for (uint64_t *b = bars; b < bars + 15; b++)
       mbar_init(b, (b >= s_free && b < done) || b >= g_free ? 8 : 1);
     for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     fence_barrier_init();
@@ -989,7 +984,6 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         if (!ok) break;
         tc_fence_after();
         mma_tmem<64>(t_dq, t_d + w * 32, dk_mn + s * kStep + w * kHalfRows, id_o, j == 0 && w == 0);
-        mma_commit(used + w);
         if (w == 1) mma_commit(empty + s);
         if (more) {
           ok = wait(g_free + w, parity);
@@ -1071,11 +1065,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
                               __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), delta2));
         q[c / 2] = pack2(x.x, x.y);
       }
-      if (j > 0) {  // the product of the last tile is done with dS
-        ok = wait.warp(used + half, (j - 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-      }
+      // dS's place is free: this dP was committed after the product that read it
       tmem_st16(t_d + lane_base + wg * 16, q);
       tmem_wait_st();
       tc_fence_before();
