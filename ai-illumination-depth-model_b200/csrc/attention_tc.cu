@@ -188,6 +188,13 @@ struct Waiter {
     }
     return true;
   }
+  // The same for the computing warps, whose every tile has several waits on its
+  // critical path: a thread that gives up goes on without waiting any more (its
+  // results are lost, its loops end), so that no warp has to agree on going on.
+  __device__ __forceinline__ void pass(uint64_t *bar, uint32_t parity) const {
+    if (!try_wait(bar, parity)) (*this)(bar, parity);
+    __syncwarp();
+  }
   // The same for a whole warp: all of its threads go on, or none.
   __device__ __forceinline__ bool warp(uint64_t *bar, uint32_t parity) const {
     return __all_sync(0xffffffffu, (*this)(bar, parity));
@@ -215,10 +222,9 @@ __device__ __forceinline__ void clear_rows(uint8_t *tile, int boxes, int from) {
 // share its exponential unit, and leave it idle together during everything
 // else. The turn passes after a quarter of them: one warp alone does not fill
 // the unit.
-__device__ __forceinline__ bool my_turn(const Waiter &wait, uint64_t *turn, int g, int it, int others) {
-  uint64_t *bar = turn + 4 * g + (threadIdx.x >> 5 & 3);
-  if (g == 0) return it == 0 || it > others || wait.warp(bar, (it - 1) & 1);
-  return it >= others || wait.warp(bar, it & 1);
+__device__ __forceinline__ void my_turn(const Waiter &wait, uint64_t *turn, int g, int it, int others) {
+  if (g == 0 ? it > 0 && it <= others : it < others)
+    wait.pass(turn + 4 * g + (threadIdx.x >> 5 & 3), (g == 0 ? it - 1 : it) & 1);
 }
 __device__ __forceinline__ void pass_turn(uint64_t *turn, int g) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(turn + 4 * (g ^ 1) + (threadIdx.x >> 5 & 3));
@@ -458,11 +464,9 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
     const int end = mine ? mask.key_end(token) : 0;
     const float sl2 = p.scale * kLog2e;
     float top = -INFINITY, sum = 0;  // the exponent's base (scaled logits, base 2)
-    bool ok = true;
     for (int j = t0; j < t1[i]; j++) {
       const int it = j - t0;
-      ok = wait.warp(s_full + i, it & 1);
-      if (!ok) break;
+      wait.pass(s_full + i, it & 1);
       tc_fence_after();
       uint32_t r[128];
 #pragma unroll
@@ -501,8 +505,7 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
       }
       grow = __any_sync(0xffffffffu, grow);
       if (it > 0 && (kApart || grow)) {  // the previous product: it reads P's place, or is about to be rescaled
-        ok = wait.warp(o_full + i, (it - 1) & 1);
-        if (!ok) break;
+        wait.pass(o_full + i, (it - 1) & 1);
         tc_fence_after();
       }
       if (grow) {
@@ -517,10 +520,7 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
         }
       }
       const float shift = top == -INFINITY ? 0.0f : -top;
-      if constexpr (kApart) {
-        ok = my_turn(wait, turn, i, it, t1[i ^ 1] - t0);
-        if (!ok) break;
-      }
+      if constexpr (kApart) my_turn(wait, turn, i, it, t1[i ^ 1] - t0);
       const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(shift, shift);
       float2 s2[2] = {make_float2(0, 0), make_float2(0, 0)};
 #pragma unroll
@@ -547,13 +547,13 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
     const long long at = ((long long)n * p.heads + h) * p.q_tokens + token;
     const float f = sum > 0 ? 1.0f / sum : (sum == 0 ? 0.0f : NAN);
     const float lse = sum == 0 ? -INFINITY : (top + log2f(sum)) * kLn2;
-    const bool some = ok && t0 < t1[i];
-    if (some) ok = wait.warp(o_full + i, (t1[i] - 1 - t0) & 1);
+    const bool some = t0 < t1[i];
+    if (some) wait.pass(o_full + i, (t1[i] - 1 - t0) & 1);
     tc_fence_after();
-    const bool have = some && ok && end > 0;
+    const bool have = some && end > 0;
     if (a.splits == 1) {
       bf16 *dst = (bf16 *)p.out.p + n * p.out.s[0] + token * p.out.s[1] + h * p.out.s[2];
-      if (some && ok) {
+      if (some) {
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
           uint32_t o[32];
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
       if (mine) p.lse[at] = lse;
     } else if (mine || some) {
       float *dst = p.ws + (split * rows + at) * p.head_dim;
-      if (some && ok) {
+      if (some) {
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
           uint32_t o[32];
@@ -785,15 +785,13 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     const int begin = key < mask.k_len ? mask.row_begin(key) : INT_MAX / 2;
     const float sl2 = p.scale * kLog2e;
     const float2 scale2 = make_float2(sl2, sl2);
-    bool ok = true;
     for (int j = t0; j < t1; j++) {
       const int it = j - t0;
       const float *mine_shift = row_sums + (it & 1) * 256 + wg * 32, *mine_delta = mine_shift + 128;
       // columns below `skip` are queries that do not see this key
       const int skip = min(max(min(max(begin - j * a.tpt, 0), 128) * a.group - wg * 32, 0), 32);
       const bool masked = __any_sync(0xffffffffu, skip > 0);
-      ok = wait.warp(s_full + half, it & 1);
-      if (!ok) break;
+      wait.pass(s_full + half, it & 1);
       tc_fence_after();
       uint32_t r[32];
       tmem_ld32(ts, r);
@@ -825,8 +823,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + half);
-      ok = wait.warp(g_full + half, it & 1);
-      if (!ok) break;
+      wait.pass(g_full + half, it & 1);
       tc_fence_after();
       uint32_t g[32];
       tmem_ld32(tg, g);
@@ -857,15 +854,15 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(d_full + half);
     }
-    if (some && ok) ok = wait.warp(done, 0);
+    if (some) wait.pass(done, 0);
     tc_fence_after();
-    const bool inside = key < p.k_tokens, have = some && ok && key < mask.k_len;
+    const bool inside = key < p.k_tokens, have = some && key < mask.k_len;
     // warpgroups 0 and 1 write dV, 2 and 3 dK, half of the columns each
     constexpr int kCols = DP / 2;
     const AttnTensor &t = half ? p.dk : p.dv;
     const int first = (wg & 1) * kCols;
     bf16 *dst = (bf16 *)t.p + n * t.s[0] + (long long)key * t.s[1] + hk * t.s[2] + first;
-    if (some && ok) {
+    if (some) {
 #pragma unroll
       for (int c = 0; c < kCols; c += 32) {
         uint32_t o[32];
@@ -1027,12 +1024,10 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     if (wg == 0 && mine) p.ws[at] = delta;  // for the key pass
     const float sl2 = p.scale * kLog2e;
     const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(shift, shift), delta2 = make_float2(-delta, -delta);
-    bool ok = true;
     for (int j = 0; j < t1; j++) {
       const int left = end - j * 128 - wg * 32;
       const bool masked = __any_sync(0xffffffffu, left < 32);
-      ok = wait.warp(s_full + half, j & 1);
-      if (!ok) break;
+      wait.pass(s_full + half, j & 1);
       tc_fence_after();
       uint32_t r[32];
       tmem_ld32(ts, r);
@@ -1045,8 +1040,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, shift2);
         r[c] = __float_as_uint(ex2(x.x)), r[c + 1] = __float_as_uint(ex2(x.y));
       }
-      ok = wait.warp(g_full + half, j & 1);
-      if (!ok) break;
+      wait.pass(g_full + half, j & 1);
       tc_fence_after();
       uint32_t g[32], q[16];
       tmem_ld32(tg, g);
@@ -1072,14 +1066,14 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(d_full + half);
     }
-    if (t1 > 0 && ok) ok = wait.warp(done, 0);
+    if (t1 > 0) wait.pass(done, 0);
     tc_fence_after();
-    const bool have = t1 > 0 && ok && end > 0;
+    const bool have = t1 > 0 && end > 0;
     bf16 *dst = (bf16 *)p.dq.p + n * p.dq.s[0] + token * p.dq.s[1] + h * p.dq.s[2];
     // a warpgroup writes a quarter of the columns
     constexpr int kCols = DP / 4;
     const int c0 = wg * kCols;
-    if (t1 > 0 && ok) {
+    if (t1 > 0) {
       uint32_t o[32];
       if constexpr (kCols == 32) tmem_ld32(t_dq + lane_base + c0, o);
       else tmem_ld16(t_dq + lane_base + c0, o);
