@@ -15,12 +15,12 @@
 // consecutive tokens (row r: token r / G, head r % G): key and value tiles are
 // read once for all of them, and a single token's heads fill one tile.
 //
-// Warps: two warpgroups compute (one TMEM lane, that is one row, a thread, so
-// a row's maximum and sum need no shuffles), one thread issues the copies, one
-// the products. All waits are on mbarriers and bounded. The product thread's
-// loops are kept rolled: its instructions run seldom, between the long bodies
-// of the computing warps, and every fetch that misses the instruction cache
-// delays both pipelines.
+// Warps: two or four warpgroups compute (one TMEM lane, that is one row, a
+// thread, so a row's maximum and sum need no shuffles), one thread issues the
+// copies, and one for each of the two pipelines (query tiles, or halves of the
+// streamed tile) its products: a product's issue takes as long as the tensor
+// cores take for it, and while one thread waits for its warpgroups the other's
+// products run. All waits are on mbarriers and bounded.
 //
 // Rows of padding inside the last tile may hold NaN: where such rows are a
 // contraction index (V; K in dQ; Q and dO in dK, dV), 0 * NaN would spoil the
@@ -44,14 +44,14 @@ using namespace tcx;
 using tok::allow_smem;
 using tok::bf16;
 
-// Compute warpgroups, then one of single warps: copies, products, clearing of
-// padding, row sums.
+// Compute warpgroups, then one of single warps: copies, the products of one
+// pipeline, those of the other, clearing of padding (and row sums).
 constexpr int kFwdGroups = 2, kBwdGroups = 4;
 constexpr int threads_of(int groups) { return 128 * (groups + 1); }
 struct Roles {
-  int copy, product, clear, sums;
+  int copy, product, second, clear;
   __host__ __device__ constexpr explicit Roles(int groups)
-      : copy(4 * groups), product(4 * groups + 1), clear(4 * groups + 2), sums(4 * groups + 3) {}
+      : copy(4 * groups), product(4 * groups + 1), second(4 * groups + 2), clear(4 * groups + 3) {}
 };
 constexpr uint32_t kImage = 128 * 128;  // 128 rows x 64 bf16 columns
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -94,13 +94,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t *r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Operand descriptors of an image: K-major (smem_desc, K = the 64 columns) and
-// MN-major: the 64 columns are the N index, 8-row groups of K are 1024 bytes
-// apart, the next 64 columns are in the next image.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(kImage >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Operand descriptors of an image, as the low word (address and stride of the
+// next 64 columns' image; steps within a tile are added to it) and the high
+// word, which all share (8-row groups 1024 bytes apart, version 1, 128-byte
+// swizzle). K-major: K is the 64 columns. MN-major: the columns are the N
+// index, 8-row groups are steps of K.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr >> 4) & 0x3FFF) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return ((addr >> 4) & 0x3FFF) | ((kImage >> 4) << 16); }
 constexpr uint32_t kBMnMajor = 1u << 16;
 
 // Products are issued by one thread, chosen by elect.sync: behind its answer
@@ -114,36 +115,56 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
   return r != 0;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+// ACC: 1 adds to the accumulator, 0 overwrites it, -1 as `acc` says.
+template <int ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc = 0) {
+  if constexpr (ACC >= 0)
+    asm volatile(
+        "{\n .reg .b64 da, db;\n mov.b64 da, {%1, %4};\n mov.b64 db, {%2, %4};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, %5;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh), "n"(ACC)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %4};\n mov.b64 db, {%2, %4};\n setp.ne.b32 p, %5, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh), "r"(acc)
+        : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+template <int ACC>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc = 0) {
+  if constexpr (ACC >= 0)
+    asm volatile(
+        "{\n .reg .b64 db;\n mov.b64 db, {%2, %4};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, %5;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh), "n"(ACC)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %4};\n setp.ne.b32 p, %5, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh), "r"(acc)
+        : "memory");
 }
 // d[128][n] = a(image rows)[128][nk * 16] * b(image rows)[n][nk * 16]', with
 // a and b K-major descriptors of the tiles.
 template <int DP>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, int nk, uint32_t idesc) {
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, int nk, uint32_t idesc) {
+  mma_ss<0>(d, a, b, idesc);
 #pragma unroll
-  for (int k = 0; k < DP / 16; k++) {
+  for (int k = 1; k < DP / 16; k++) {
     constexpr uint32_t image = kImage >> 4;
     const uint32_t o = (k >> 2) * image + (k & 3) * 2;
-    if (k < nk) mma_ss(d, a + o, b + o, idesc, k > 0);
+    if (k < nk) mma_ss<1>(d, a + o, b + o, idesc);
   }
 }
 // d[128][n] (+)= a(TMEM, bf16 pairs)[128][K] * b(image)[K][n], with b an
-// MN-major descriptor; every 32 of K lie `gap` columns apart.
-template <int K>
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool first, uint32_t gap = 16) {
+// MN-major descriptor; every 32 of K lie GAP columns apart.
+template <int K, uint32_t GAP = 16>
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
+  mma_ts<-1>(d, a, b, idesc, !first);
 #pragma unroll
-  for (int k = 0; k < K / 16; k++)
-    mma_ts(d, a + (k >> 1) * gap + (k & 1) * 8, b + k * 128, idesc, first && k == 0 ? 0u : 1u);
+  for (int k = 1; k < K / 16; k++) mma_ts<1>(d, a + (k >> 1) * GAP + (k & 1) * 8, b + k * 128, idesc);
 }
 constexpr uint32_t kHalfRows = 64 * 128 >> 4;  // descriptor step from row 0 to row 64 of an image
 
@@ -230,12 +251,6 @@ __device__ __forceinline__ void pass_turn(uint64_t *turn, int g) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(turn + 4 * (g ^ 1) + (threadIdx.x >> 5 & 3));
 }
 
-// The product thread has the tile that holds padding and asks for its clearing.
-__device__ __forceinline__ bool cleared(const Waiter &wait, uint64_t *ask, uint64_t *clean) {
-  mbar_arrive(ask);
-  return wait(clean, 0);
-}
-
 // Writes n (a multiple of 8, at most 32) values as bf16, times f.
 __device__ __forceinline__ void store_bf16(bf16 *dst, const uint32_t *r, int n, float f) {
 #pragma unroll
@@ -255,9 +270,10 @@ __device__ __forceinline__ void store_zeros(bf16 *dst, int n) {
 
 // The end of every kernel: copies and products of a CTA that gave up are
 // drained, then TMEM is freed.
-__device__ __forceinline__ void leave(uint32_t tmem, bool product_warp, volatile int *fail, uint64_t *drain, int *err) {
+__device__ __forceinline__ void leave(uint32_t tmem, const Roles &roles, int warp, volatile int *fail, uint64_t *drain,
+                                      int *err) {
   __syncwarp();
-  if (product_warp) {
+  if (warp == roles.product || warp == roles.second) {
     if (elect_one()) {  // the thread that issued the products
       mma_commit(drain);
       mbar_wait(drain, 0);
@@ -267,7 +283,7 @@ __device__ __forceinline__ void leave(uint32_t tmem, bool product_warp, volatile
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *fail) report_gave_up(err);
-  if (product_warp) {
+  if (warp == roles.product) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -343,12 +359,12 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
   if (threadIdx.x == 0) {
     *fail = 0;
     for (int i = 0; i < 2; i++) mbar_init(q_full + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1), mbar_init(s_free + i, 4);
-    mbar_init(drain, 1);
-    mbar_init(ask, 1);
+    mbar_init(drain, 2);
+    mbar_init(ask, 2);
     mbar_init(clean, 1);
     for (int i = 0; i < 8; i++) mbar_init(turn + i, 1);
     for (int i = 0; i < L::kStages; i++)
-      mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
+      mbar_init(k_full + i, 1), mbar_init(k_empty + i, 2), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 2);
     fence_barrier_init();
   }
   if (warp == roles.product) tmem_alloc(tmem_ptr, 512);
@@ -392,49 +408,49 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
         clear_rows(sv + s * L::kTile, L::kBoxes, mask.k_len - clear_at * 128);
         if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
       }
-    } else if (warp == roles.product && t0 < most && elect_one()) {
-      const uint64_t dq = smem_desc(smem_u32(sq)), dk = smem_desc(smem_u32(sk)), dv = desc_mn(smem_u32(sv));
+    } else if ((warp == roles.product || warp == roles.second) && t0 < most && elect_one()) {
+      const int i = warp == roles.second;  // this thread's query tile
+      const int end = i ? t1[1] : t1[0];
+      const uint32_t dq = desc_k(smem_u32(sq)), dk = desc_k(smem_u32(sk)), dv = desc_mn(smem_u32(sv));
       constexpr uint32_t kStep = L::kTile >> 4;  // descriptors of the next tile
       const uint32_t id_s = instr_desc(1, 128), id_o = instr_desc(1, a.n16) | kBMnMajor;
       const int nk = a.n16 / 16;
-      const int end0 = t1[0], end1 = t1[1];
       bool ok = wait(k_full, 0);
-#pragma unroll 1
-      for (int i = 0; i < 2; i++) {
-        if (t0 >= (i ? end1 : end0)) continue;
-        ok = ok && wait(q_full + i, 0);
-        if (!ok) break;
-        mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk, nk, id_s);
-        mma_commit(s_full + i);
+      if (ok && t0 < end) ok = wait(q_full + i, 0);
+      if (ok) {
+        if (t0 < end) {
+          mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk, nk, id_s);
+          mma_commit(s_full + i);
+        }
+        mma_commit(k_empty);
       }
-      if (ok) mma_commit(k_empty);
       int s = 0, use = 0;  // stage of tile j, parity of its use
+      // past this query tile's own keys the stages are only passed on
       for (int j = t0; j < most && ok; j++) {
         const int s1 = s + 1 == L::kStages ? 0 : s + 1, use1 = s1 ? use : use ^ 1, parity = (j - t0) & 1;
         const bool more = j + 1 < most;
-        if constexpr (kApart) {
-          if (more) {
-            ok = wait(k_full + s1, use1);
-#pragma unroll 1
-            for (int i = 0; i < 2 && ok; i++) {
-              if (j + 1 >= (i ? end1 : end0)) continue;
+        if (more) {
+          ok = wait(k_full + s1, use1);
+          if (!ok) break;
+          if (kApart) {
+            if (j + 1 < end) {
               ok = wait(s_free + i, parity);
               if (!ok) break;
               tc_fence_after();
               mma_rows<DP>(tmem + i * 128, dq + i * kStep, dk + s1 * kStep, nk, id_s);
               mma_commit(s_full + i);
             }
-            if (!ok) break;
             mma_commit(k_empty + s1);
           }
         }
-        ok = wait(v_full + s, use) && (j != clear_at || cleared(wait, ask, clean)) &&
-             (kApart || !more || wait(k_full + s1, use1));
+        ok = wait(v_full + s, use);
         if (!ok) break;
-#pragma unroll 1
-        for (int i = 0; i < 2; i++) {
-          const int end = i ? end1 : end0;
-          if (j >= end) continue;
+        if (j == clear_at) {  // asks for the clearing of padding, waits for it
+          mbar_arrive(ask);
+          ok = wait(clean, 0);
+          if (!ok) break;
+        }
+        if (j < end) {
           ok = wait(p_full + i, parity);
           if (!ok) break;
           tc_fence_after();
@@ -445,7 +461,6 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
             mma_commit(s_full + i);
           }
         }
-        if (!ok) break;
         mma_commit(v_empty + s);
         if (!kApart && more) mma_commit(k_empty + s1);
         s = s1, use = use1;
@@ -585,25 +600,20 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
       if (mine) p.ws[a.splits * rows * p.head_dim + split * rows + at] = lse;
     }
   }
-  leave(tmem, warp == roles.product, fail, drain, p.err);
+  leave(tmem, roles, warp, fail, drain, p.err);
 }
 
 // ---------------------------------------------------------------------------
 // Backward, dK and dV: one key tile (its rows are the TMEM lanes) past the
 // query tiles that see it. Per query tile: S' = K Q', dP' = V dO', and from
 // TMEM dV += P' dO, dK += dS' Q. A warpgroup takes 32 query columns: the
-// arithmetic is bound by its latencies, and four warps an SM quarter cover one
-// another's where two (64 columns each) left it idle two thirds of the time.
-// The columns go to the products in halves, which the product thread serves in
-// turn. Where TMEM has 128 columns left (head sizes up to 64), P' and dS' have
-// places of their own, and a half of the next S' or dP' is computed as soon as
-// its warpgroups have loaded this one:
-//   P0(j): dV   S0 free: S0(j+1)   dS0(j): dK   dP0 free: dP0(j+1)   P1(j): ...
-// Else they replace S' and dP', whose next half follows the product that reads
-// them. (One product for both halves of S' and dP' takes the tensor cores 20 %
-// less, but holds both halves to one step, and their exponentials collide:
-// 196 us against 173 at 12 heads of 6272 causal tokens, head size 64.)
-// The order of the sums is fixed in both.
+// arithmetic is bound by its latencies, which four warps an SM quarter cover
+// for one another. P' and dS' replace S' and dP' in TMEM. The columns go to the
+// products in halves, two pipelines of their own:
+//   P(j): dV, S'(j+1)   dS'(j): dK, dP'(j+1)
+// Up to head size 64 each has its thread and its own accumulators, which are
+// added at the end; beyond, TMEM holds one pair, and one thread serves both
+// halves in turn. The order of the sums is fixed in both.
 // ---------------------------------------------------------------------------
 
 template <int DP>
@@ -620,15 +630,15 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg, const AttnParams p,
                   const TcArgs a) {
   using L = BwdSmem<DP>;
-  constexpr bool kApart = DP == 64;
+  constexpr bool kTwin = DP == 64;
   extern __shared__ uint8_t raw[];
   uint8_t *base = align1024(raw);
   uint8_t *sk = base, *sv = sk + L::kTile, *sq = sv + L::kTile, *sg = sq + L::kStages * L::kTile;
   float *row_sums = reinterpret_cast<float *>(sg + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sg + L::kStages * L::kTile + L::kRowSums);
   uint64_t *kv_full = bars, *s_full = bars + 1, *g_full = bars + 3, *p_full = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *s_free = bars + 13, *g_free = bars + 15, *full = bars + 17, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 17 + 2 * L::kStages);
+           *done = bars + 9, *drain = bars + 10, *clean = bars + 11, *full = bars + 12, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 12 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   constexpr Roles roles(kBwdGroups);
   const int warp = threadIdx.x >> 5;
@@ -646,9 +656,10 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 17; b++)
-      mbar_init(b, (b >= p_full && b < done) || b >= s_free ? 8 : b >= s_full && b < g_full ? 2 : 1);
-    for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    mbar_init(kv_full, 1), mbar_init(done, kTwin ? 2 : 1), mbar_init(drain, 2), mbar_init(clean, 1);
+    for (int i = 0; i < 2; i++)
+      mbar_init(s_full + i, 2), mbar_init(g_full + i, 1), mbar_init(p_full + i, 8), mbar_init(d_full + i, 8);
+    for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, kTwin ? 2 : 1);
     fence_barrier_init();
   }
   // rows of the query images past group * tpt are never written by the copies
@@ -659,11 +670,10 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  const uint32_t t_s = tmem, t_g = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
-  // P' and dS' of half w of the query columns: 32 columns from w * p_step on,
-  // or the first half of every warpgroup's own 32 columns of S' and dP'
-  const uint32_t t_p = kApart ? tmem + 384 : t_s, t_d = kApart ? tmem + 448 : t_g;
-  constexpr uint32_t p_step = kApart ? 32 : 64, p_gap = kApart ? 16 : 32;
+  // S', dP' (P' and dS' in the first half of every warpgroup's 32 columns), the
+  // accumulators of the first pipeline, and t_next further those of the second
+  const uint32_t t_s = tmem, t_g = tmem + 128, t_dv = tmem + 256, t_dk = tmem + (kTwin ? 384 : 256 + DP);
+  constexpr uint32_t t_next = kTwin ? 64 : 0;
   const Waiter wait{fail};
 
   if (warp == roles.copy && (threadIdx.x & 31) == 0 && some) {
@@ -681,14 +691,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     }
     mbar_wait(kv_full, 0);
     for (int i = max(0, issued - L::kStages); i < issued; i++) mbar_wait(full + i % L::kStages, (i / L::kStages) & 1);
-  } else if (warp == roles.clear && clear_at < t1 && clear_at >= t0) {
-    const int it = clear_at - t0, s = it % L::kStages, from = (mask.q_len - clear_at * a.tpt) * a.group;
-    if (wait.warp(ask, 0) && wait.warp(full + s, (it / L::kStages) & 1)) {
-      clear_rows(sq + s * L::kTile, L::kBoxes, from);
-      clear_rows(sg + s * L::kTile, L::kBoxes, from);
-      if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
-    }
-  } else if (warp == roles.sums && some) {
+  } else if (warp == roles.clear && some) {
     // lse and delta of every query tile's rows, half a tile ahead of their use:
     // shift (base 2; -inf where a row has no probabilities) and -delta
     const int lane = threadIdx.x & 31;
@@ -713,6 +716,13 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       // with the probabilities of tile j - 1 the warpgroups are done with
       // tile j - 2 (a wait for that tile itself could miss its phase)
       if (it >= 1 && !(wait.warp(p_full, (it - 1) & 1) && wait.warp(p_full + 1, (it - 1) & 1))) break;
+      if (j == clear_at) {
+        const int s = it % L::kStages, from = (mask.q_len - j * a.tpt) * a.group;
+        if (!wait.warp(full + s, (it / L::kStages) & 1)) break;
+        clear_rows(sq + s * L::kTile, L::kBoxes, from);
+        clear_rows(sg + s * L::kTile, L::kBoxes, from);
+        if (lane == 0) mbar_arrive(clean);
+      }
       float *to = row_sums + (it & 1) * 256;
 #pragma unroll
       for (int k = 0; k < 4; k++) {
@@ -722,15 +732,16 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       __syncwarp();
       if (lane < 2) mbar_arrive(s_full + lane);
     }
-  } else if (warp == roles.product && some && elect_one()) {
-    const uint64_t dk = smem_desc(smem_u32(sk)), dv = smem_desc(smem_u32(sv)), dq = smem_desc(smem_u32(sq)),
-                   dg = smem_desc(smem_u32(sg)), dq_mn = desc_mn(smem_u32(sq)), dg_mn = desc_mn(smem_u32(sg));
+  } else if ((warp == roles.product || (kTwin && warp == roles.second)) && some && elect_one()) {
+    const int first = warp == roles.second, last = kTwin ? first : 1;  // this thread's halves
+    const uint32_t dk = desc_k(smem_u32(sk)), dv = desc_k(smem_u32(sv)), dq = desc_k(smem_u32(sq)),
+                   dg = desc_k(smem_u32(sg)), dq_mn = desc_mn(smem_u32(sq)), dg_mn = desc_mn(smem_u32(sg));
     constexpr uint32_t kStep = L::kTile >> 4;
     const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
-    bool ok = wait(kv_full, 0) && wait(full, 0) && (t0 != clear_at || cleared(wait, ask, clean));
+    bool ok = wait(kv_full, 0) && wait(full, 0) && (t0 != clear_at || wait(clean, 0));
 #pragma unroll 1
-    for (int w = 0; w < 2 && ok; w++) {
+    for (int w = first; w <= last && ok; w++) {
       mma_rows<DP>(t_s + w * 64, dk, dq + w * kHalfRows, nk, id_s);
       mma_commit(s_full + w);
       mma_rows<DP>(t_g + w * 64, dv, dg + w * kHalfRows, nk, id_s);
@@ -741,19 +752,14 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       const int s1 = s + 1 == L::kStages ? 0 : s + 1, use1 = s1 ? use : use ^ 1, parity = (j - t0) & 1;
       const bool more = j + 1 < t1;
 #pragma unroll 1
-      for (int w = 0; w < 2; w++) {
+      for (int w = first; w <= last; w++) {
         ok = wait(p_full + w, parity);
         if (!ok) break;
         tc_fence_after();
-        mma_tmem<64>(t_dv, t_p + w * p_step, dg_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0, p_gap);
-        if (more && kApart) {
-          ok = (w || (wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean)))) && wait(s_free + w, parity);
-          if (!ok) break;
-          tc_fence_after();
-          mma_rows<DP>(t_s + w * 64, dk, dq + s1 * kStep + w * kHalfRows, nk, id_s);
-          mma_commit(s_full + w);
-        } else if (more) {
-          if (w == 0) ok = wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean));
+        mma_tmem<64, 32>(t_dv + w * t_next, t_s + w * 64, dg_mn + s * kStep + w * kHalfRows, id_o,
+                         j == t0 && (kTwin || w == 0));
+        if (more) {
+          if (w == first) ok = wait(full + s1, use1) && (j + 1 != clear_at || wait(clean, 0));
           if (!ok) break;
           mma_rows<DP>(t_s + w * 64, dk, dq + s1 * kStep + w * kHalfRows, nk, id_s);
           mma_commit(s_full + w);
@@ -761,13 +767,9 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         ok = wait(d_full + w, parity);
         if (!ok) break;
         tc_fence_after();
-        mma_tmem<64>(t_dk, t_d + w * p_step, dq_mn + s * kStep + w * kHalfRows, id_o, j == t0 && w == 0, p_gap);
-        if (w == 1) mma_commit(empty + s);
-        if (kApart && more) {
-          ok = wait(g_free + w, parity);
-          if (!ok) break;
-          tc_fence_after();
-        }
+        mma_tmem<64, 32>(t_dk + w * t_next, t_g + w * 64, dq_mn + s * kStep + w * kHalfRows, id_o,
+                         j == t0 && (kTwin || w == 0));
+        if (w == last) mma_commit(empty + s);
         if (more) {
           mma_rows<DP>(t_g + w * 64, dv, dg + s1 * kStep + w * kHalfRows, nk, id_s);
           mma_commit(g_full + w);
@@ -780,7 +782,6 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     const int wg = warp >> 2, half = wg >> 1, row = threadIdx.x & 127, lane = threadIdx.x & 31;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
     const uint32_t ts = t_s + lane_base + wg * 32, tg = t_g + lane_base + wg * 32;
-    const uint32_t tp = t_p + lane_base + half * p_step + (wg & 1) * p_gap, td = t_d + lane_base + half * p_step + (wg & 1) * p_gap;
     const int key = key0 + row;
     const int begin = key < mask.k_len ? mask.row_begin(key) : INT_MAX / 2;
     const float sl2 = p.scale * kLog2e;
@@ -796,11 +797,6 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       uint32_t r[32];
       tmem_ld32(ts, r);
       tmem_wait_ld();
-      if constexpr (kApart) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free + half);
-      }
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const float4 l = *reinterpret_cast<const float4 *>(mine_shift + c);
@@ -817,8 +813,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       uint32_t q[16];
 #pragma unroll
       for (int c = 0; c < 16; c++) q[c] = pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-      // P's place is free: this S' was committed after the product that read it
-      tmem_st16(tp, q);
+      tmem_st16(ts, q);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -828,11 +823,6 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       uint32_t g[32];
       tmem_ld32(tg, g);
       tmem_wait_ld();
-      if constexpr (kApart) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(g_free + half);
-      }
       if (masked) {
 #pragma unroll
         for (int c = 0; c < 32; c++)
@@ -848,7 +838,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         q[c / 2] = pack2(x.x, x.y);
         q[c / 2 + 1] = pack2(y.x, y.y);
       }
-      tmem_st16(td, q);
+      tmem_st16(tg, q);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -868,20 +858,27 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
         uint32_t o[32];
         tmem_ld32((half ? t_dk : t_dv) + lane_base + first + c, o);
         tmem_wait_ld();
+        if constexpr (kTwin) {
+          uint32_t o2[32];
+          tmem_ld32((half ? t_dk : t_dv) + t_next + lane_base + first + c, o2);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(o2[k]));
+        }
         if (inside && have) store_bf16(dst + c, o, p.head_dim - first - c, half ? p.scale : 1.0f);
       }
     }
     if (inside && !have) store_zeros(dst, min(kCols, p.head_dim - first));
   }
-  leave(tmem, warp == roles.product, fail, drain, p.err);
+  leave(tmem, roles, warp, fail, drain, p.err);
 }
 
 // ---------------------------------------------------------------------------
 // Backward, dQ: one query tile past the key tiles it sees. S = Q K' and
-// dP = dO V' are recomputed, dQ += dS K from TMEM. The warpgroups take 32 key
-// columns each; dS has a TMEM place of its own, and a half of the next S or dP
-// is computed as soon as its warpgroups have loaded this one:
-//   S0 free: S0(j+1)   dS0(j): dQ   dP0 free: dP0(j+1)   S1 free: ...
+// dP = dO V' are recomputed, dQ += dS K from TMEM, where dS replaces dP. The
+// warpgroups take 32 key columns each; the halves of the columns are two
+// pipelines, with a product thread and an accumulator each:
+//   S free: S(j+1)   dS(j): dQ, dP(j+1)
 // A thread's lse and delta stay in registers. This pass runs first and leaves
 // the row sums delta in the workspace for the other.
 // ---------------------------------------------------------------------------
@@ -898,8 +895,8 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   float *row_sums = reinterpret_cast<float *>(sv + L::kStages * L::kTile);
   uint64_t *bars = reinterpret_cast<uint64_t *>(sv + L::kStages * L::kTile + L::kRowSums);
   uint64_t *q_full = bars, *s_full = bars + 1, *g_full = bars + 3, *s_free = bars + 5, *d_full = bars + 7,
-           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *g_free = bars + 13, *full = bars + 15, *empty = full + L::kStages;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 15 + 2 * L::kStages);
+           *done = bars + 9, *drain = bars + 10, *ask = bars + 11, *clean = bars + 12, *full = bars + 13, *empty = full + L::kStages;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + 13 + 2 * L::kStages);
   volatile int *fail = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   constexpr Roles roles(kBwdGroups);
   const int warp = threadIdx.x >> 5;
@@ -916,9 +913,10 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 
   if (threadIdx.x == 0) {
     *fail = 0;
-    for (uint64_t *b = bars; b < bars + 15; b++)
-      mbar_init(b, (b >= s_free && b < done) || b >= g_free ? 8 : 1);
-    for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    mbar_init(q_full, 1), mbar_init(done, 2), mbar_init(drain, 2), mbar_init(ask, 2), mbar_init(clean, 1);
+    for (int i = 0; i < 2; i++)
+      mbar_init(s_full + i, 1), mbar_init(g_full + i, 1), mbar_init(s_free + i, 8), mbar_init(d_full + i, 8);
+    for (int i = 0; i < L::kStages; i++) mbar_init(full + i, 1), mbar_init(empty + i, 2);
     fence_barrier_init();
   }
   if (warp == roles.product) tmem_alloc(tmem_ptr, 512);
@@ -926,7 +924,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  const uint32_t t_s = tmem, t_g = tmem + 128, t_dq = tmem + 256, t_d = tmem + 384;
+  const uint32_t t_s = tmem, t_g = tmem + 128, t_dq = tmem + 256;
   const Waiter wait{fail};
 
   if (warp == roles.copy && (threadIdx.x & 31) == 0 && t1 > 0) {
@@ -950,45 +948,47 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       clear_rows(sk + s * L::kTile, L::kBoxes, mask.k_len - clear_at * 128);
       if ((threadIdx.x & 31) == 0) mbar_arrive(clean);
     }
-  } else if (warp == roles.product && t1 > 0 && elect_one()) {
-    const uint64_t dq = smem_desc(smem_u32(sq)), dg = smem_desc(smem_u32(sg)), dk = smem_desc(smem_u32(sk)),
-                   dv = smem_desc(smem_u32(sv)), dk_mn = desc_mn(smem_u32(sk));
+  } else if ((warp == roles.product || warp == roles.second) && t1 > 0 && elect_one()) {
+    const int w = warp == roles.second;  // this thread's half
+    const uint32_t dq = desc_k(smem_u32(sq)), dg = desc_k(smem_u32(sg)), dk = desc_k(smem_u32(sk)) + w * kHalfRows,
+                   dv = desc_k(smem_u32(sv)) + w * kHalfRows, dk_mn = desc_mn(smem_u32(sk)) + w * kHalfRows;
     constexpr uint32_t kStep = L::kTile >> 4;
     const uint32_t id_s = instr_desc(1, 64), id_o = instr_desc(1, a.n16) | kBMnMajor;
     const int nk = a.n16 / 16;
-    bool ok = wait(q_full, 0) && wait(full, 0) && (clear_at != 0 || cleared(wait, ask, clean));
-#pragma unroll 1
-    for (int w = 0; w < 2 && ok; w++) {
-      mma_rows<DP>(t_s + w * 64, dq, dk + w * kHalfRows, nk, id_s);
+    const uint32_t ts = t_s + w * 64, tg = t_g + w * 64, tq = t_dq + w * DP;
+    // key tile j is there, its padding cleared
+    auto ready = [&](int j, int s, int use) {
+      if (!wait(full + s, use)) return false;
+      if (j != clear_at) return true;
+      mbar_arrive(ask);
+      return wait(clean, 0);
+    };
+    bool ok = wait(q_full, 0) && ready(0, 0, 0);
+    if (ok) {
+      mma_rows<DP>(ts, dq, dk, nk, id_s);
       mma_commit(s_full + w);
-      mma_rows<DP>(t_g + w * 64, dg, dv + w * kHalfRows, nk, id_s);
+      mma_rows<DP>(tg, dg, dv, nk, id_s);
       mma_commit(g_full + w);
     }
     int s = 0, use = 0;
     for (int j = 0; j < t1 && ok; j++) {
       const int s1 = s + 1 == L::kStages ? 0 : s + 1, use1 = s1 ? use : use ^ 1, parity = j & 1;
       const bool more = j + 1 < t1;
-#pragma unroll 1
-      for (int w = 0; w < 2; w++) {
-        if (more) {
-          ok = (w || (wait(full + s1, use1) && (j + 1 != clear_at || cleared(wait, ask, clean)))) && wait(s_free + w, parity);
-          if (!ok) break;
-          tc_fence_after();
-          mma_rows<DP>(t_s + w * 64, dq, dk + s1 * kStep + w * kHalfRows, nk, id_s);
-          mma_commit(s_full + w);
-        }
-        ok = wait(d_full + w, parity);
+      if (more) {
+        ok = ready(j + 1, s1, use1) && wait(s_free + w, parity);
         if (!ok) break;
         tc_fence_after();
-        mma_tmem<64>(t_dq, t_d + w * 32, dk_mn + s * kStep + w * kHalfRows, id_o, j == 0 && w == 0);
-        if (w == 1) mma_commit(empty + s);
-        if (more) {
-          ok = wait(g_free + w, parity);
-          if (!ok) break;
-          tc_fence_after();
-          mma_rows<DP>(t_g + w * 64, dg, dv + s1 * kStep + w * kHalfRows, nk, id_s);
-          mma_commit(g_full + w);
-        }
+        mma_rows<DP>(ts, dq, dk + s1 * kStep, nk, id_s);
+        mma_commit(s_full + w);
+      }
+      ok = wait(d_full + w, parity);
+      if (!ok) break;
+      tc_fence_after();
+      mma_tmem<64, 32>(tq, tg, dk_mn + s * kStep, id_o, j == 0);
+      mma_commit(empty + s);
+      if (more) {
+        mma_rows<DP>(tg, dg, dv + s1 * kStep, nk, id_s);
+        mma_commit(g_full + w);
       }
       s = s1, use = use1;
     }
@@ -1045,9 +1045,6 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
       uint32_t g[32], q[16];
       tmem_ld32(tg, g);
       tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(g_free + half);
       if (masked) {
 #pragma unroll
         for (int c = 0; c < 32; c++)
@@ -1059,8 +1056,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
                               __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), delta2));
         q[c / 2] = pack2(x.x, x.y);
       }
-      // dS's place is free: this dP was committed after the product that read it
-      tmem_st16(t_d + lane_base + wg * 16, q);
+      tmem_st16(tg, q);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -1074,15 +1070,22 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
     constexpr int kCols = DP / 4;
     const int c0 = wg * kCols;
     if (t1 > 0) {
-      uint32_t o[32];
-      if constexpr (kCols == 32) tmem_ld32(t_dq + lane_base + c0, o);
-      else tmem_ld16(t_dq + lane_base + c0, o);
+      uint32_t o[32], o2[32];  // of both pipelines
+      if constexpr (kCols == 32) {
+        tmem_ld32(t_dq + lane_base + c0, o);
+        tmem_ld32(t_dq + DP + lane_base + c0, o2);
+      } else {
+        tmem_ld16(t_dq + lane_base + c0, o);
+        tmem_ld16(t_dq + DP + lane_base + c0, o2);
+      }
       tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < kCols; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(o2[k]));
       if (mine && have) store_bf16(dst + c0, o, min(kCols, p.head_dim - c0), p.scale);
     }
     if (mine && !have && wg == 0) store_zeros(dst, p.head_dim);
   }
-  leave(tmem, warp == roles.product, fail, drain, p.err);
+  leave(tmem, roles, warp, fail, drain, p.err);
 }
 
 // ---------------------------------------------------------------------------
