@@ -47,9 +47,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// a / b for b = 0 or normal, within 2 steps.
+__device__ __forceinline__ float quotient(float a, float b) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(b));
+  return a * r;
 }
 
 // What a lane holds of a block as it lies in memory: elements 128 k + 4 l + j.
@@ -64,9 +70,9 @@ struct Held {
 };
 
 template <typename T>
-__device__ __forceinline__ typename RawPack<T, 4>::type load_raw(const T *p, int n) {
+__device__ __forceinline__ typename RawPack<T, 4>::type load_raw(const T *p, int n, bool whole) {
   typedef typename RawPack<T, 4>::type Raw;
-  if (n == 4 && reinterpret_cast<uintptr_t>(p) % sizeof(Raw) == 0) return *reinterpret_cast<const Raw *>(p);
+  if (whole) return *reinterpret_cast<const Raw *>(p);
   T e[4];
 #pragma unroll
   for (int j = 0; j < 4; j++) {
@@ -78,16 +84,33 @@ __device__ __forceinline__ typename RawPack<T, 4>::type load_raw(const T *p, int
   return raw;
 }
 
-// Byte j of w as a float, without the conversion unit (which the square roots
-// and reciprocals need): 2^23 + byte, minus 2^23 (and the bias of signed codes).
-__device__ __forceinline__ float byte_value(uint32_t w, int j, float bias) {
-  return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7650 + j)) - bias;
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(typename RawPack<T, 4>::type raw, float2 *to) {
+  float e[4];
+  RawPack<T, 4>::unpack(raw, e);
+  to[0] = make_float2(e[0], e[1]), to[1] = make_float2(e[2], e[3]);
 }
-// floor(x * inv + u) within [lo, hi], as 1.5 * 2^23 + the code: a sum rounded
-// down to a whole number.
-__device__ __forceinline__ uint32_t code_of(float x, float inv, float u, float lo, float hi) {
-  constexpr float kMagic = 12582912.0f;
-  const float s = __fadd_rd(__fadd_rn(__fmul_rn(x, inv), u), kMagic);
+
+// Bytes j and j + 1 of w as floats, without the conversion unit (which the square roots
+// and reciprocals need): 2^23 + byte, minus 2^23 (and the bias of signed codes).
+// A sum of products that must not be merged with them: the compiler merges
+// packed products and sums, rounding modes or not, but not across widths.
+__device__ __forceinline__ float2 add_apart(float2 a, float2 b) {
+  return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 byte_values(uint32_t w, int j, float bias) {
+  return __fadd2_rn(make_float2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7650 + j)),
+                                __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7651 + j))),
+                    both(-bias));
+}
+// floor(x * inv + u), as 1.5 * 2^23 + the code: a sum rounded down to a whole
+// number. The caller limits it.
+constexpr float kMagic = 12582912.0f;
+__device__ __forceinline__ float2 codes_of(float2 x, float2 inv, float2 u) {
+  return __fadd2_rd(add_apart(__fmul2_rn(x, inv), u), both(kMagic));
+}
+__device__ __forceinline__ uint32_t limited(float s, float lo, float hi) {
   return __float_as_uint(fminf(fmaxf(s, kMagic + lo), kMagic + hi));
 }
 // The low bytes of four codes.
@@ -113,11 +136,13 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const AdamwChunk *__restrict
     const G *gp = (const G *)grads.p[chunk.tensor - first_tensor] + ((long long)chunk.block + warp) * kAdamwBlock;
     const float *pp = chunk.param + warp * kAdamwBlock;
     const long long sb = chunk.state_block + warp;
+    const bool pw = left >= kAdamwBlock && reinterpret_cast<uintptr_t>(pp) % sizeof(float4) == 0;
+    const bool gw = left >= kAdamwBlock && reinterpret_cast<uintptr_t>(gp) % sizeof(held.g[0]) == 0;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       const int e = 128 * k + 4 * lane, n = min(max(left - e, 0), 4);
-      held.p[k] = load_raw<float>(pp + e, n);
-      held.g[k] = load_raw<G>(gp + e, n);
+      held.p[k] = load_raw<float>(pp + e, n, pw);
+      held.g[k] = load_raw<G>(gp + e, n, gw);
       const long long i = (sb * kAdamwBlock + e) / 4;
       held.m[k] = ((const typename Held<BITS, G>::RawM *)state.m)[i];
       held.v[k] = ((const typename Held<BITS, G>::RawM *)state.v)[i];
@@ -147,21 +172,22 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const AdamwChunk *__restrict
   for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
     const AdamwChunk now = chunk;
     const int left = now.elems - warp * kAdamwBlock;
-    float p[2][4], g[2][4], m[2][4], v[2][4];
+    // elements 128 k + 4 l + 2 q and the next: two operations an instruction
+    float2 p[4], g[4], m[4], v[4];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-      RawPack<float, 4>::unpack(held.p[k], p[k]);
-      RawPack<G, 4>::unpack(held.g[k], g[k]);
+      unpack_pairs<float>(held.p[k], p + 2 * k);
+      unpack_pairs<G>(held.g[k], g + 2 * k);
       if constexpr (BITS == 32) {
-        RawPack<float, 4>::unpack(held.m[k], m[k]);
-        RawPack<float, 4>::unpack(held.v[k], v[k]);
+        unpack_pairs<float>(held.m[k], m + 2 * k);
+        unpack_pairs<float>(held.v[k], v + 2 * k);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int q = 0; q < 2; q++) {
           // signed codes with their sign bit flipped are 128 too large
-          m[k][j] = __fmul_rn(byte_value(held.m[k] ^ 0x80808080u, j, 8388736.0f), held.ms);
-          const float root = __fmul_rn(byte_value(held.v[k], j, 8388608.0f), held.vs);
-          v[k][j] = __fmul_rn(root, root);
+          m[2 * k + q] = __fmul2_rn(byte_values(held.m[k] ^ 0x80808080u, 2 * q, 8388736.0f), both(held.ms));
+          const float2 root = __fmul2_rn(byte_values(held.v[k], 2 * q, 8388608.0f), both(held.vs));
+          v[2 * k + q] = __fmul2_rn(root, root);
         }
       }
     }
@@ -169,42 +195,41 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const AdamwChunk *__restrict
     if (left <= 0) continue;
     float *pp = now.param + warp * kAdamwBlock;
     const long long sb = now.state_block + warp;
-    const bool pvec = (reinterpret_cast<uintptr_t>(pp) & 15) == 0;
+    const bool whole = left >= kAdamwBlock && (reinterpret_cast<uintptr_t>(pp) & 15) == 0;
     const float keep = now.decay ? decayed : 1.0f;
     float mtop = 0, rtop = 0;
 #pragma unroll
-    for (int k = 0; k < 2; k++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float gg = g[k][j];
-        m[k][j] = __fadd_rn(__fmul_rn(m[k][j], h.beta1), __fmul_rn(gg, h.one_minus_beta1));
-        v[k][j] = __fadd_rn(__fmul_rn(v[k][j], h.beta2), __fmul_rn(__fmul_rn(gg, gg), h.one_minus_beta2));
-        const float root = __fsqrt_rn(v[k][j]);
-        // within 2 steps of the quotient: steps of the update, not of the parameter
-        p[k][j] = fmaf(p[k][j], keep, -__fdividef(c1 * m[k][j], fmaf(root, c2, h.eps)));
-        if constexpr (BITS == 8) {
-          v[k][j] = root;
-          mtop = max_nan(mtop, fabsf(m[k][j]));
-          rtop = max_nan(rtop, root);
-        }
+    for (int q = 0; q < 4; q++) {
+      m[q] = add_apart(__fmul2_rn(m[q], both(h.beta1)), __fmul2_rn(g[q], both(h.one_minus_beta1)));
+      v[q] = add_apart(__fmul2_rn(v[q], both(h.beta2)), __fmul2_rn(__fmul2_rn(g[q], g[q]), both(h.one_minus_beta2)));
+      const float2 root = make_float2(__fsqrt_rn(v[q].x), __fsqrt_rn(v[q].y));
+      // within 2 steps of the quotient: steps of the update, not of the parameter
+      const float2 up = __fmul2_rn(m[q], both(-c1)), down = __ffma2_rn(root, both(c2), both(h.eps));
+      p[q] = __ffma2_rn(p[q], both(keep), make_float2(quotient(up.x, down.x), quotient(up.y, down.y)));
+      if constexpr (BITS == 8) {
+        v[q] = root;
+        mtop = max_nan(max_nan(mtop, fabsf(m[q].x)), fabsf(m[q].y));
+        rtop = max_nan(max_nan(rtop, root.x), root.y);
       }
+    }
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       const int e = 128 * k + 4 * lane, n = min(max(left - e, 0), 4);
-      if (pvec && n == 4) {
-        Pack<float, 4>::store(pp + e, p[k]);
+      const float o[4] = {p[2 * k].x, p[2 * k].y, p[2 * k + 1].x, p[2 * k + 1].y};
+      if (whole) {
+        Pack<float, 4>::store(pp + e, o);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          if (j < n) pp[e + j] = p[k][j];
+          if (j < n) pp[e + j] = o[j];
       }
     }
     if constexpr (BITS == 32) {
 #pragma unroll
       for (int k = 0; k < 2; k++) {
         const long long i = sb * kAdamwBlock + 128 * k + 4 * lane;
-        Pack<float, 4>::store((float *)state.m + i, m[k]);
-        Pack<float, 4>::store((float *)state.v + i, v[k]);
+        *reinterpret_cast<float4 *>((float *)state.m + i) = make_float4(m[2 * k].x, m[2 * k].y, m[2 * k + 1].x, m[2 * k + 1].y);
+        *reinterpret_cast<float4 *>((float *)state.v + i) = make_float4(v[2 * k].x, v[2 * k].y, v[2 * k + 1].x, v[2 * k + 1].y);
       }
     } else {
       constexpr float kTiny = 7.888609e-31f;  // 2^-100: below it the reciprocal of a scale would overflow
@@ -213,6 +238,7 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const AdamwChunk *__restrict
       const float ms = mtop < kTiny ? 0.0f : __fmul_rn(mtop, (float)(1.0 / 127.0));
       const float rs = rtop < kTiny ? 0.0f : __fmul_rn(rtop, (float)(1.0 / 255.0));
       const float mi = ms == 0.0f ? 0.0f : __frcp_rn(ms), ri = rs == 0.0f ? 0.0f : __frcp_rn(rs);
+      const float least = rs > 0.0f ? 1.0f : 0.0f;
       if (lane == 0) state.m_scale[sb] = ms, state.v_scale[sb] = rs;
 #pragma unroll
       for (int k = 0; k < 2; k++) {
@@ -220,12 +246,14 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const AdamwChunk *__restrict
         uint32_t mc[4], vc[4];
         uint32_t place = (uint32_t)i * 0x85EBCA6Bu + sweep;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float u = (float)(place >> 8) * 0x1p-24f;
-          place += 0x85EBCA6Bu;
-          mc[j] = code_of(m[k][j], mi, u, -127.0f, 127.0f);
-          const float root = v[k][j];
-          vc[j] = code_of(root, ri, u, root > 0.0f && rs > 0.0f ? 1.0f : 0.0f, 255.0f);
+        for (int q = 0; q < 2; q++) {
+          const float2 u = __fmul2_rn(make_float2((float)(place >> 8), (float)((place + 0x85EBCA6Bu) >> 8)), both(0x1p-24f));
+          place += 2 * 0x85EBCA6Bu;
+          const float2 root = v[2 * k + q];
+          const float2 cm = codes_of(m[2 * k + q], both(mi), u), cv = codes_of(root, both(ri), u);
+          mc[2 * q] = limited(cm.x, -127.0f, 127.0f), mc[2 * q + 1] = limited(cm.y, -127.0f, 127.0f);
+          vc[2 * q] = limited(cv.x, root.x > 0.0f ? least : 0.0f, 255.0f);
+          vc[2 * q + 1] = limited(cv.y, root.y > 0.0f ? least : 0.0f, 255.0f);
         }
         ((uint32_t *)state.m)[i / 4] = pack_codes(mc);
         ((uint32_t *)state.v)[i / 4] = pack_codes(vc);

@@ -136,6 +136,7 @@ template <typename T, int DP, int STR>
 __global__ void __launch_bounds__(kThreads) k_attn(const AttnParams p, int q_tiles, int splits, Vecs vec) {
   extern __shared__ __align__(16) float sm[];
   float *sq = sm, *sk = sq + DP * kFixLd, *sp = sk + DP * (STR + 4);
+  cudaTriggerProgrammaticLaunchCompletion();  // the join of shares
   constexpr int N = STR / 16;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   long long id = blockIdx.x;
@@ -235,10 +236,11 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnParams p, int splits) {
   __shared__ float weights[8][kMostSplits];
   const long long rows = (long long)p.batch * p.heads * p.q_tokens;
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);  // warp 0 of every CTA has one
   if (row >= rows) return;
   const int lane = threadIdx.x & 31;
   float *w = weights[threadIdx.x >> 5];
+  cudaGridDependencySynchronize();
   const float *sums = p.ws + splits * rows * p.head_dim + row;
   float top = -INFINITY;
   bool nan = false;
@@ -264,12 +266,31 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnParams p, int split
   T *out = (T *)p.out.p + bh / p.heads * p.out.s[0] + i * p.out.s[1] + bh % p.heads * p.out.s[2];
   const float *part = p.ws + row * p.head_dim;
   const long long step = rows * p.head_dim;
-  for (int d = lane; d < p.head_dim; d += 32) {
-    float o = 0;
+  if (p.head_dim % 4 == 0) {
+    // half a warp takes the even shares, half the odd ones, 16 bytes a lane
+    for (int d = 0; d < p.head_dim; d += 64) {
+      const int at = d + 4 * (lane & 15);
+      float o[4] = {0, 0, 0, 0};
 #pragma unroll 8
-    for (int s = 0; s < splits; s++)  // a share without keys (weight 0) has no output
-      if (w[s] != 0) o = fmaf(w[s], __ldcg(part + s * step + d), o);
-    from_f32(out[d], o * inv);
+      for (int s = lane >> 4; s < splits; s += 2)  // a share without keys (weight 0) has no output
+        if (w[s] != 0 && at < p.head_dim) {
+          const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + s * step + at));
+          o[0] = fmaf(w[s], v.x, o[0]), o[1] = fmaf(w[s], v.y, o[1]);
+          o[2] = fmaf(w[s], v.z, o[2]), o[3] = fmaf(w[s], v.w, o[3]);
+        }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        o[k] = (o[k] + __shfl_xor_sync(0xffffffffu, o[k], 16)) * inv;
+        if (lane < 16 && at < p.head_dim) from_f32(out[at + k], o[k]);
+      }
+    }
+  } else {
+    for (int d = lane; d < p.head_dim; d += 32) {
+      float o = 0;
+      for (int s = 0; s < splits; s++)
+        if (w[s] != 0) o = fmaf(w[s], __ldcg(part + s * step + d), o);
+      from_f32(out[d], o * inv);
+    }
   }
   if (lane == 0) p.lse[row] = total == 0 ? -INFINITY : top + logf(total);
 }
@@ -456,8 +477,8 @@ cudaError_t run_simt(const AttnParams &p, bool bwd, cudaStream_t st) {
     if ((e = allow_smem<k_attn<T, DP, STR>>(sm)) != cudaSuccess) return e;
     const long long grid = (long long)p.batch * p.heads * q_tiles * splits;
     if (grid > 0) k_attn<T, DP, STR><<<(unsigned)grid, kThreads, sm, st>>>(p, q_tiles, splits, vec);
-    if (splits > 1) k_attn_join<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, splits);
-    return cudaGetLastError();
+    if ((e = cudaGetLastError()) != cudaSuccess || splits == 1) return e;
+    return launch_next(k_attn_join<T>, (rows + 7) / 8, 256, 0, st, p, splits);
   }
   if (rows > 0) {
     k_attn_delta<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
@@ -500,8 +521,7 @@ cudaError_t attention(int T, const AttnParams &p, cudaStream_t st) {
   const int splits = attention_tc_splits(p);
   if (e != cudaSuccess || splits == 1) return e;
   const long long rows = (long long)p.batch * p.heads * p.q_tokens;
-  k_attn_join<bf16><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, splits);
-  return cudaGetLastError();
+  return launch_next(k_attn_join<bf16>, (rows + 7) / 8, 256, 0, st, p, splits);
 }
 
 cudaError_t attention_backward(int T, const AttnParams &p, cudaStream_t st) {

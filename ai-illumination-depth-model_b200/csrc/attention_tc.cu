@@ -356,6 +356,7 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
   most = max(t1[0], t1[1]);
   const int clear_at = mask.k_len % 128 ? mask.k_len / 128 : INT_MAX;  // the value tile that holds padding
 
+  cudaTriggerProgrammaticLaunchCompletion();  // the join of shares
   if (threadIdx.x == 0) {
     *fail = 0;
     for (int i = 0; i < 2; i++) mbar_init(q_full + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1), mbar_init(s_free + i, 4);
@@ -669,6 +670,9 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // delta comes from the kernel of dQ, which may still be at work; all threads
+  // stop here, so that no bounded wait runs against its time
+  cudaGridDependencySynchronize();
   const uint32_t tmem = *tmem_ptr;
   // S', dP' (P' and dS' in the first half of every warpgroup's 32 columns), the
   // accumulators of the first pipeline, and t_next further those of the second
@@ -911,6 +915,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   const int t1 = first < mask.q_len ? (mask.key_end(min(first + a.tpt, mask.q_len) - 1) + 127) / 128 : 0;
   const int clear_at = mask.k_len % 128 ? mask.k_len / 128 : INT_MAX;  // the key tile that holds padding
 
+  cudaTriggerProgrammaticLaunchCompletion();  // dK and dV
   if (threadIdx.x == 0) {
     *fail = 0;
     mbar_init(q_full, 1), mbar_init(done, 2), mbar_init(drain, 2), mbar_init(ask, 2), mbar_init(clean, 1);
@@ -1166,8 +1171,8 @@ cudaError_t backward_tc(const AttnParams &p, const TcArgs &a, const CUtensorMap 
   if (e != cudaSuccess) return e;
   const long long heads = (long long)p.batch * p.kv_heads;
   k_attn_dq_tc<DP><<<(unsigned)(heads * a.q_tiles), threads_of(kBwdGroups), sm, st>>>(mq, mk, mv, mg, p, a);
-  k_attn_dkv_tc<DP><<<(unsigned)(heads * a.k_tiles), threads_of(kBwdGroups), sm, st>>>(mq, mk, mv, mg, p, a);
-  return cudaGetLastError();
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return tok::launch_next(k_attn_dkv_tc<DP>, heads * a.k_tiles, threads_of(kBwdGroups), sm, st, mq, mk, mv, mg, p, a);
 }
 
 }  // namespace

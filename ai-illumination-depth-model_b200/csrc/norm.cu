@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd(const T *__restrict__ dy,
                                                        long long dxs, float *__restrict__ part) {
   extern __shared__ float sums[];  // [rows per CTA][c] when a warp takes a row
   __shared__ float red[kThreads / 32];
+  cudaTriggerProgrammaticLaunchCompletion();  // the sum over the partial rows
   constexpr int kRows = kThreads / LANES;
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   typedef typename RawPack<T, VW>::type Raw;
@@ -268,6 +269,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd_long(const T *__restrict_
                                                             const float *__restrict__ rstd, T *__restrict__ dx,
                                                             long long dxs, float *__restrict__ part) {
   __shared__ float red[kThreads / 32];
+  cudaTriggerProgrammaticLaunchCompletion();  // the sum over the partial rows
   float *out = part ? part + (size_t)blockIdx.x * 2 * c : nullptr;
   if (out)
     for (int i = threadIdx.x; i < 2 * c; i += kThreads) out[i] = 0;  // each thread adds to its own columns only
@@ -302,6 +304,7 @@ __global__ void __launch_bounds__(256) k_norm_reduce(const float *__restrict__ p
   const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
   const int col = blockIdx.x * 8 + tx;
   float t = 0;
+  cudaGridDependencySynchronize();
   if (col < 2 * c) {
 #pragma unroll 4
     for (int i = ty; i < n; i += 32) t += part[(size_t)i * 2 * c + col];
@@ -423,8 +426,9 @@ cudaError_t layer_norm_backward(int T, const void *dy, long long dys, const void
     if (T == 0) dispatch<float>(a, true);
     else dispatch<bf16>(a, true);
   }
-  if (dw || db) k_norm_reduce<<<(2 * c + 7) / 8, 256, 0, st>>>(ws, a.blocks, c, dw, db);
-  return cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !(dw || db)) return e;
+  return launch_next(k_norm_reduce, (2 * c + 7) / 8, 256, 0, st, ws, a.blocks, c, dw, db);
 }
 
 }  // namespace gpu

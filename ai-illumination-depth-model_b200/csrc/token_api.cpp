@@ -1,5 +1,6 @@
 // C entry points of the token operators and of the AdamW step: argument
 // checks, and the optimiser's tensor table.
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <vector>
@@ -318,7 +319,8 @@ illumina_status illumina_adamw_step(illumina_adamw *opt, const void *const *grad
   ILL_TRY
   require(opt && grads && h, "adamw: null argument");
   require(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1, "adamw: betas outside [0, 1)");
-  require(h->eps >= 0 && std::isfinite(h->lr) && std::isfinite(h->weight_decay), "adamw: bad hyperparameter");
+  require(h->eps == 0 || h->eps >= FLT_MIN, "adamw: eps must be 0 or a normal float");
+  require(std::isfinite(h->lr) && std::isfinite(h->weight_decay), "adamw: bad hyperparameter");
   const size_t e = size_of(opt->grad_precision);
   for (int i = 0; i < opt->tensors; i++)
     require(opt->counts[i] == 0 || (grads[i] && aligned(grads[i], e)),

@@ -103,6 +103,22 @@ cudaError_t allow_smem(size_t bytes) {
   return e;
 }
 
+// A kernel that follows another on its stream and needs its results: it may
+// start, and set itself up, while the last CTAs of the one before are at work,
+// if that one's CTAs called cudaTriggerProgrammaticLaunchCompletion. At least
+// one thread of each of its CTAs calls cudaGridDependencySynchronize, so that
+// what follows on the stream finds both finished.
+template <typename... P, typename... A>
+cudaError_t launch_next(void (*kernel)(P...), long long grid, int threads, size_t smem, cudaStream_t st, const A &...args) {
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)grid), c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = st;
+  c.attrs = &early, c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
+
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace tok

@@ -128,6 +128,6 @@ def createOptimizer(params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weightDecay=0
                     gradDtype=None) -> AdamW:
     """AdamW over `params` (contiguous float32 CUDA tensors of one device, updated in place). decay: per tensor, whether
     weight decay applies (default: to all). momentBits 8 keeps the moments as 8-bit codes with a scale for every 256
-    elements of a tensor. gradDtype: float32 (default) or bfloat16."""
+    elements of a tensor. gradDtype: float32 (default) or bfloat16. eps is 0 or at least the smallest normal float."""
     import torch
     return AdamW(params, lr, betas, eps, weightDecay, decay, momentBits, gradDtype or torch.float32)

@@ -497,7 +497,7 @@ typedef struct illumina_adamw_options {
   float *m_scale, *v_scale;        /* device, 8 bits only */
 } illumina_adamw_options;
 typedef struct illumina_adamw_hyper {
-  double lr, beta1, beta2, eps, weight_decay;
+  double lr, beta1, beta2, eps, weight_decay; /* eps: 0 or a normal float */
   const float *lr_device;          /* nullable: a device scalar read in place of lr (a captured step's schedule) */
 } illumina_adamw_hyper;
 

@@ -287,3 +287,11 @@ def test_refusals(torch):
     opt.betas = (1.0, 0.9)
     with pytest.raises(illumina.IlluminaError):
         opt.step([torch.zeros(10, device="cuda")])
+
+
+@pytest.mark.parametrize("eps", [-1e-8, 1e-39, float("nan")])
+def test_refuses_eps_below_the_normal_floats(torch, eps):
+    import illumina
+    opt = illumina.createOptimizer([torch.zeros(10, device="cuda")], eps=eps)
+    with pytest.raises((ValueError, RuntimeError), match="eps"):
+        opt.step([torch.zeros(10, device="cuda")])
