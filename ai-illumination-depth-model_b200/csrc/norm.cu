@@ -14,7 +14,7 @@
 // per CTA goes to the workspace and a second launch adds the partials in a
 // fixed order, so that results do not depend on scheduling.
 //
-// Measured at 50176 rows of 704, bf16: forward 32 us (4.4 TB/s), backward with
+// Measured at 50176 rows of 704, bf16: forward 31 us (4.5 TB/s), backward with
 // its second launch 44 us (4.9 TB/s, 67 us with the rows in registers); at
 // 25088 rows of 1024, f32, backward 57 us (5.4 TB/s). A single frame of 196
 // rows is a launch: 4 us on the GPU, 11 us a call.
@@ -31,13 +31,16 @@ using namespace tok;
 
 constexpr int kThreads = 256, kSms = 148;
 
-// VW values of w or b; vectors when they are aligned like the columns (VW 4:
-// the caller checked).
+// VW values of w or b; vectors when they are aligned like the columns (the
+// caller checked).
 template <int VW>
 __device__ __forceinline__ void load_params(const float *p, float (&o)[VW]) {
-  if constexpr (VW == 4) {
-    const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
-    o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+  if constexpr (VW % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < VW; j += 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(p + j));
+      o[j] = v.x, o[j + 1] = v.y, o[j + 2] = v.z, o[j + 3] = v.w;
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < VW; j++) o[j] = __ldg(p + j);
@@ -527,6 +530,7 @@ void launch(NormArgs &a, bool bwd) {
     else
       k_norm<T, VW, VPT, LANES, 1><<<(unsigned)((a.rows + kRows - 1) / kRows), kThreads, 0, a.st>>>(
           x, a.xs, a.rows, a.c, a.w, a.b, a.eps, (T *)a.y, a.ys, a.mean, a.rstd);
+  } else if constexpr (VW == 8) {  // never: such rows go through the ring
   } else if constexpr (VW == 1 || sizeof(T) == 2 || VPT == 1) {  // longer aligned rows of floats go through the ring
     constexpr bool kPre = VW * VPT * sizeof(T) <= 64;
     const size_t sm = LANES == kThreads || !a.part ? 0 : (size_t)kRows * a.c * sizeof(float);
@@ -575,6 +579,15 @@ bool pick(NormArgs &a, bool bwd) {
   return true;
 }
 
+// The forward of bf16 rows in 16-byte chunks, where a warp takes two rows
+// (704 columns 31 us at 50176 rows, 36 in 8-byte chunks; one row of 1024 a
+// warp 25 us at 25088 rows, 24.6 in 8-byte chunks).
+void pick8(NormArgs &a) {
+  if (a.c <= 256) launch<bf16, 8, 1, 32>(a, false);
+  else if (a.c <= 512) launch<bf16, 8, 2, 32>(a, false);
+  else launch<bf16, 8, 3, 32>(a, false);
+}
+
 template <typename T>
 void dispatch(NormArgs &a, bool bwd) {
   // four columns at a time: 8 or 16 bytes of T, 16 bytes of w and b
@@ -587,6 +600,10 @@ void dispatch(NormArgs &a, bool bwd) {
   // half the ring's threads would idle up to 128 columns of bf16 (17 us at 50176 rows, 22 through the ring)
   if (bwd && a.c > 128 && a.c <= 4096 && a.c * sizeof(T) % 16 == 0 && chunks(a.x, a.xs) && chunks(a.y, a.ys) && chunks(a.dy, a.dys))
     return pick_ring<T>(a);
+  if constexpr (sizeof(T) == 2)
+    if (!bwd && a.c > 128 && a.c <= 768 && a.c % 8 == 0 && chunks(a.x, a.xs) && chunks(a.y, a.ys) && aligned16(a.w) &&
+        aligned16(a.b))
+      return pick8(a);
   if (vec ? pick<T, 4>(a, bwd) : pick<T, 1>(a, bwd)) return;
   if (!bwd)
     k_norm_long<T><<<(unsigned)a.rows, kThreads, 0, a.st>>>((const T *)a.x, a.xs, a.c, a.w, a.b, a.eps, (T *)a.y, a.ys,
