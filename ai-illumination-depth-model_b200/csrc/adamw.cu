@@ -23,6 +23,12 @@
 // root that is not zero never becomes code 0: the next step would divide by
 // almost nothing.
 //
+// Measured: 112 tensors of 1.4 M elements, 32-bit moments: 10 us on the GPU,
+// 20 us a call (the pointers are checked and sent each time); 8-bit moments,
+// bf16 gradients: 217 us for 78.7 M elements (5.1 TB/s, 14 bytes an element),
+// bound by instruction issue: 85 instructions an element with one value an
+// instruction took 255 us.
+//
 // The step count lives on the device, so that a captured step can be
 // replayed: every CTA reads it, the last one to finish advances it.
 #include <cstring>
