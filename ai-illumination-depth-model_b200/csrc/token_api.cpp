@@ -1,8 +1,10 @@
 // C entry points of the token operators and of the AdamW step: argument
 // checks, and the optimiser's tensor table.
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstring>
+#include <utility>
 #include <vector>
 
 #include "api.h"
@@ -270,6 +272,15 @@ illumina_status illumina_adamw_create(const illumina_adamw_options *o, illumina_
   require(blocks > 0, "adamw: every tensor is empty");
   require(o->m && o->v && aligned(o->m, 16) && aligned(o->v, 16), "adamw: moments missing or misaligned");
   require(o->moment_bits == 32 || (o->m_scale && o->v_scale), "adamw: 8-bit moments need scales");
+  std::vector<std::pair<uintptr_t, uintptr_t>> places;
+  for (int i = 0; i < o->tensors; i++)
+    if (o->counts[i] > 0) {
+      const uintptr_t p = reinterpret_cast<uintptr_t>(o->params[i]);
+      places.emplace_back(p, p + (uintptr_t)o->counts[i] * sizeof(float));
+    }
+  std::sort(places.begin(), places.end());
+  for (size_t i = 1; i < places.size(); i++)
+    require(places[i - 1].second <= places[i].first, "adamw: parameters overlap, or one is listed twice");
   std::unique_ptr<illumina_adamw> opt(new illumina_adamw);
   opt->device = o->device, opt->tensors = o->tensors, opt->bits = o->moment_bits;
   opt->grad_precision = o->grad_precision, opt->blocks = blocks;
@@ -299,6 +310,7 @@ illumina_status illumina_adamw_create(const illumina_adamw_options *o, illumina_
   opt->chunks = (gpu::AdamwChunk *)(base + a);
   cuda_check(cudaMemset(base, 0, a), "adamw: clear");
   cuda_check(cudaMemcpy(opt->chunks, chunks.data(), cb, cudaMemcpyHostToDevice), "adamw: upload");
+  cuda_check(cudaStreamSynchronize(nullptr), "adamw: upload");  // steps may run on streams that do not wait for this one
   opt->state.m = o->m, opt->state.v = o->v, opt->state.m_scale = o->m_scale, opt->state.v_scale = o->v_scale;
   *out = opt.release();
   return ILLUMINA_OK;

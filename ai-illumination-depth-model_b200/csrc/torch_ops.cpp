@@ -9,6 +9,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 
 #include <optional>
 #include <string>
@@ -103,6 +104,13 @@ void writable(const char *name, const at::Tensor &x, const at::Tensor &like) {
   for (int64_t d = 0; d < x.dim(); d++) need(x.size(d) <= 1 || x.stride(d) != 0, name, "must not be broadcast");
 }
 
+// An output may be the input whose place it takes, element for element, but
+// not another view of the same memory (as far as strides tell in short).
+void apart(const char *name, const at::Tensor &out, const at::Tensor &in, bool in_place) {
+  const auto s = at::get_overlap_status(out, in);
+  need(s != at::MemOverlapStatus::Partial && (in_place || s != at::MemOverlapStatus::Full), name, "must not overlap an input");
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor &x, const MaybeTensor &weight,
                                                           const MaybeTensor &bias, double eps, const MaybeTensor &out) {
   const int precision = storage("x", x);
@@ -116,6 +124,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor &x, c
   if (out.has_value()) {
     y = *out;
     writable("out", y, x);
+    apart("out", y, x, true);
     y_stride = Rows("out", y).stride;
   } else {
     y = at::empty(x.sizes(), x.options());
@@ -184,6 +193,7 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
     if (out.has_value()) {
       y = *out;
       writable(name, y, x);
+      apart(name, y, x, true);
     } else {
       y = at::empty(x.sizes(), x.options());
     }
@@ -193,7 +203,10 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
   };
   at::Tensor yq = fill(a.first, q, out_q, "outQ");
   MaybeTensor yk;
-  if (k.has_value()) yk = fill(a.second, *k, out_k, "outK");
+  if (k.has_value()) {
+    yk = fill(a.second, *k, out_k, "outK");
+    apart("outQ", yq, *k, false), apart("outK", *yk, q, false), apart("outQ", yq, *yk, false);
+  }
   a.positions = positions.data_ptr(), a.positions_float = fractional;
   a.position_stride[0] = positions.stride(0), a.position_stride[1] = pd == 3 ? positions.stride(1) : 0;
   a.position_stride[2] = positions.stride(-1);

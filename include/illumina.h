@@ -373,7 +373,8 @@ illumina_status illumina_op_bilateral(const float *low, int lh, int lw, int low_
  * contiguous. The calls queue their kernels on `stream` and return; they
  * allocate nothing and can be captured. A workspace belongs to the call until
  * its kernels are done: calls that may overlap (two streams, two graphs) need
- * one each. Outputs must not overlap inputs unless an entry point says so.
+ * one each. Outputs must not overlap inputs unless an entry point says that
+ * one may be the other, then with the same strides.
  * ------------------------------------------------------------------------- */
 
 /* Layer norm over the last dimension: y = (x - mean) * rstd * w + b with
@@ -433,7 +434,7 @@ typedef struct illumina_attention_tensor {
 } illumina_attention_tensor;
 
 /* out = softmax(scale q k' masked) v for `heads` query heads, `heads / kv_heads`
- * of which share a key head; head_dim at most 128.
+ * of which share a key head; head_dim at most 128, the other sizes 2^28.
  * q_lens, k_lens ([batch] int32, nullable) are the lengths of a padded batch
  * (clamped to the token counts): padding may hold anything, and the rows of
  * padding in out, dq, dk and dv are written as zeros. causal_block 0: a query
@@ -504,7 +505,7 @@ typedef struct illumina_adamw_hyper {
 /* Blocks of the flat moments of tensors with these counts. */
 illumina_status illumina_adamw_blocks(const long long *counts, int tensors, long long *blocks);
 /* Uploads the tensor table; no step has been taken. The tensors and moments
- * must outlive the optimiser. */
+ * must outlive the optimiser; no two tensors may overlap. */
 illumina_status illumina_adamw_create(const illumina_adamw_options *opts, illumina_adamw **out);
 illumina_status illumina_adamw_destroy(illumina_adamw *opt);
 /* One step: grads is a host array of device pointers, one a tensor (ignored for
