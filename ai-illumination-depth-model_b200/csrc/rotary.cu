@@ -10,7 +10,7 @@
 // a million costs no more phase error than one of ten.
 //
 // Measured: 2 clips of 32 frames of 196 tokens, 12 + 4 heads of 64, three axes,
-// bf16: 15 us (3.4 TB/s; the 51 MB partly stay in the L2); one frame 5 us on
+// bf16: 13 us (3.9 TB/s), a third of it launch and ramp; one frame 5 us on
 // the GPU, 11 us a call.
 #include "token_common.cuh"
 #include "token_ops.h"
@@ -22,20 +22,30 @@ namespace {
 using namespace tok;
 
 constexpr int kThreads = 256;
-constexpr int kTrig = 2048;  // (token, pair) angles a CTA holds
+constexpr int kTrig = 1024;  // (token, pair) angles a CTA holds
 
 // VW: elements a thread moves at once; halves: pairs are (j, j + pairs), so a
 // thread reads VW of each half, else neighbours (2j, 2j + 1).
 template <typename T, int VW, bool HALVES>
 __global__ void __launch_bounds__(kThreads) k_rotary(const RotaryParams p, int tb) {
-  __shared__ float cs[kTrig], sn[kTrig];
+  __shared__ __align__(16) float cs[kTrig], sn[kTrig];
   const long long total = p.batch * p.tokens, first = (long long)blockIdx.x * tb;
   const int nt = (int)min((long long)tb, total - first);
+  const long long b0 = first / p.tokens, n0 = first - b0 * p.tokens;
+  // batch and token of the CTA's token t; the division is for the few CTAs that pass the end of a sequence
+  auto token = [&](int t, long long &b, long long &n) {
+    b = b0, n = n0 + t;
+    if (n >= p.tokens) {
+      const long long more = n / p.tokens;
+      b += more, n -= more * p.tokens;
+    }
+  };
   for (int i = threadIdx.x; i < nt * p.pairs; i += kThreads) {
     const int t = i / p.pairs, j = i - t * p.pairs;
-    const long long bt = first + t, b = bt / p.tokens;
+    long long b, n;
+    token(t, b, n);
     const int a = min(max(p.axis[j], 0), p.axes - 1);
-    const long long at = a * p.ps[0] + b * p.ps[1] + (bt - b * p.tokens) * p.ps[2];
+    const long long at = a * p.ps[0] + b * p.ps[1] + n * p.ps[2];
     const double pos = p.pos_float ? (double)((const float *)p.pos)[at] : (double)((const int *)p.pos)[at];
     double u = pos * p.turns[j];
     u -= rint(u);
@@ -45,6 +55,10 @@ __global__ void __launch_bounds__(kThreads) k_rotary(const RotaryParams p, int t
     sn[i] = p.inverse ? -s : s;
   }
   __syncthreads();
+  constexpr int kPart = VW == 1 ? 1 : 4;  // pairs are a multiple of VW then
+  struct alignas(4 * kPart) Part {
+    float v[kPart];
+  };
   const int turned = HALVES ? p.pairs / VW : (VW == 1 ? p.pairs : 2 * p.pairs / VW);
   const int rest = (p.head_dim - 2 * p.pairs) / VW;
   const int per_head = turned + rest, heads = p.t[0].heads + p.t[1].heads, per_token = per_head * heads;
@@ -55,7 +69,8 @@ __global__ void __launch_bounds__(kThreads) k_rotary(const RotaryParams p, int t
     const bool second = h >= p.t[0].heads;
     const RotaryTensor &q = p.t[second];
     if (second) h -= p.t[0].heads;
-    const long long bt = first + t, b = bt / p.tokens, n = bt - b * p.tokens;
+    long long b, n;
+    token(t, b, n);
     const T *x = (const T *)q.x + b * q.xs[0] + n * q.xs[1] + h * q.xs[2];
     T *y = (T *)q.y + b * q.ys[0] + n * q.ys[1] + h * q.ys[2];
     const float *ct = cs + t * p.pairs, *st = sn + t * p.pairs;
@@ -69,9 +84,16 @@ __global__ void __launch_bounds__(kThreads) k_rotary(const RotaryParams p, int t
       float u[VW], v[VW];
       Pack<T, VW>::load(x + j, u);
       Pack<T, VW>::load(x + p.pairs + j, v);
+      float cj[VW], sj[VW];
+#pragma unroll
+      for (int k = 0; k < VW; k += kPart) {
+        const Part c = *reinterpret_cast<const Part *>(ct + j + k), s = *reinterpret_cast<const Part *>(st + j + k);
+#pragma unroll
+        for (int l = 0; l < kPart; l++) cj[k + l] = c.v[l], sj[k + l] = s.v[l];
+      }
 #pragma unroll
       for (int k = 0; k < VW; k++) {
-        const float c = ct[j + k], s = st[j + k], a = u[k];
+        const float c = cj[k], s = sj[k], a = u[k];
         u[k] = a * c - v[k] * s;
         v[k] = a * s + v[k] * c;
       }
@@ -110,7 +132,7 @@ void launch(const RotaryParams &p, cudaStream_t st) {
     for (int i = 0; i < 3; i++) vec = vec && t.xs[i] % V == 0 && t.ys[i] % V == 0;
   }
   const long long total = p.batch * p.tokens;
-  int tb = kTrig / p.pairs < 16 ? kTrig / p.pairs : 16;
+  int tb = kTrig / p.pairs < 8 ? kTrig / p.pairs : 8;  // 2 x 6272 tokens, 16 heads of 64: 13.2 us, with 16 tokens 15.0, with 4 16.3
   while (tb > 1 && (total + tb - 1) / tb < 2 * 148) tb = (tb + 1) / 2;
   const unsigned grid = (unsigned)((total + tb - 1) / tb);
   if (vec && p.interleaved) k_rotary<T, V, false><<<grid, kThreads, 0, st>>>(p, tb);
