@@ -50,6 +50,8 @@
 
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+
 namespace illumina {
 namespace gpu {
 
@@ -1160,13 +1162,13 @@ TcArgs shape_of(const AttnParams &p) {
 }
 
 // Shares of the keys in the forward: enough for a CTA on every SM, while a
-// share keeps at least two key tiles.
+// share keeps at least two key tiles, and none is empty.
 int tc_splits(const AttnParams &p, const TcArgs &a) {
   const long long ctas = (long long)p.batch * p.kv_heads * ((a.q_tiles + 1) / 2);
   const int sms = 148, most = a.k_tiles / 2;
   if (ctas == 0 || ctas * 2 > sms || most < 2) return 1;
-  const int want = (int)(sms / ctas);
-  return want < most ? want : most;
+  const int want = std::min((int)(sms / ctas), most), per = (a.k_tiles + want - 1) / want;
+  return (a.k_tiles + per - 1) / per;
 }
 
 template <int DP>

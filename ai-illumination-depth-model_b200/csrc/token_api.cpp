@@ -272,15 +272,6 @@ illumina_status illumina_adamw_create(const illumina_adamw_options *o, illumina_
   require(blocks > 0, "adamw: every tensor is empty");
   require(o->m && o->v && aligned(o->m, 16) && aligned(o->v, 16), "adamw: moments missing or misaligned");
   require(o->moment_bits == 32 || (o->m_scale && o->v_scale), "adamw: 8-bit moments need scales");
-  std::vector<std::pair<uintptr_t, uintptr_t>> places;
-  for (int i = 0; i < o->tensors; i++)
-    if (o->counts[i] > 0) {
-      const uintptr_t p = reinterpret_cast<uintptr_t>(o->params[i]);
-      places.emplace_back(p, p + (uintptr_t)o->counts[i] * sizeof(float));
-    }
-  std::sort(places.begin(), places.end());
-  for (size_t i = 1; i < places.size(); i++)
-    require(places[i - 1].second <= places[i].first, "adamw: parameters overlap, or one is listed twice");
   std::unique_ptr<illumina_adamw> opt(new illumina_adamw);
   opt->device = o->device, opt->tensors = o->tensors, opt->bits = o->moment_bits;
   opt->grad_precision = o->grad_precision, opt->blocks = blocks;
@@ -302,6 +293,15 @@ illumina_status illumina_adamw_create(const illumina_adamw_options *o, illumina_
     opt->groups.back().end = i + 1;
     opt->groups.back().chunk1 = (long long)chunks.size();
   }
+  std::vector<std::pair<uintptr_t, uintptr_t>> places;
+  for (int i = 0; i < o->tensors; i++)
+    if (o->counts[i] > 0) {
+      const uintptr_t p = reinterpret_cast<uintptr_t>(o->params[i]);
+      places.emplace_back(p, p + (uintptr_t)o->counts[i] * sizeof(float));
+    }
+  std::sort(places.begin(), places.end());
+  for (size_t i = 1; i < places.size(); i++)
+    require(places[i - 1].second <= places[i].first, "adamw: parameters overlap, or one is listed twice");
   OnDevice on(o->device);
   const size_t a = 256, cb = chunks.size() * sizeof(chunks[0]);
   cuda_check(cudaMalloc(&opt->memory, a + cb), "adamw: cudaMalloc");
