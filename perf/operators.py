@@ -5,7 +5,6 @@ maps, the rotation of queries and keys by the tokens' (frame, row, column), atte
 clip with its backward pass, one frame's queries against a cached clip, and an AdamW step over a model's tensors.
 `own` selects the library's calls; otherwise the same formulas run as elementary torch operations in 32 bits.
 """
-import functools
 import math
 import os
 import sys
@@ -35,9 +34,7 @@ DEPTH_OPS = (
     ("pw", 24, 32, 1), ("dwpw", 32, 32, 3), ("pw", 32, 1, 1))
 
 
-@functools.lru_cache(maxsize=None)
 def _library():
-    """The package, imported once, as a program does."""
     package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                            "ai-illumination-depth-model_b200")
     if package not in sys.path:
