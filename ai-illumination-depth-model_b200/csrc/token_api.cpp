@@ -203,7 +203,7 @@ illumina_status illumina_op_rotary(const illumina_rotary_args *a, void *stream) 
   require(a->batch >= 0 && a->tokens >= 0, "rotary: negative size");
   require(a->batch == 0 || a->tokens < kMostBlocks / a->batch, "rotary: more than 2^30 tokens");
   require(a->head_dim >= 1 && a->head_dim <= 1024, "rotary: head_dim outside [1, 1024]");
-  require(a->pairs >= 1 && 2 * a->pairs <= a->head_dim, "rotary: pairs outside [1, head_dim / 2]");
+  require(a->pairs >= 1 && a->pairs <= a->head_dim / 2, "rotary: pairs outside [1, head_dim / 2]");
   require(a->axes >= 1, "rotary: axes must be positive");
   const bool some = a->batch * a->tokens > 0 && (a->first.heads > 0 || a->second.heads > 0);
   gpu::RotaryParams p;
