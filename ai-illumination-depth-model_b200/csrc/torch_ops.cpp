@@ -72,8 +72,8 @@ template <typename T>
 T *vector_of(const char *name, const MaybeTensor &x, int64_t n, const at::Tensor &like, at::ScalarType type) {
   if (!x.has_value()) return nullptr;
   if (!(x->scalar_type() == type && x->device() == like.device() && x->numel() == n && x->is_contiguous()))
-    refuse(std::string(name) + " must be " + std::to_string(n) + " contiguous " + (type == at::kInt ? "int32" : "float32") +
-           " values on the device of the others");
+    refuse(std::string(name) + " must be " + std::to_string(n) + " contiguous " +
+           (type == at::kInt ? "int32" : type == at::kDouble ? "float64" : "float32") + " values on the device of the others");
   return static_cast<T *>(x->data_ptr());
 }
 float *floats(const char *name, const MaybeTensor &x, int64_t n, const at::Tensor &like) {
@@ -174,7 +174,10 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
   a.precision = storage("q", q, 4);
   const int64_t b = q.size(0), t = q.size(1), d = q.size(3);
   if (d != head_dim) refuse("q must have the plan's " + std::to_string(head_dim) + " elements a head");
-  need(turns.device() == q.device(), "the plan must be on the device of q");
+  const int64_t pairs = turns.numel();
+  need(pairs <= d / 2, "the plan must have at most headDim / 2 pairs");
+  a.turns = vector_of<double>("the plan's turns", turns, pairs, q, at::kDouble);
+  a.axis = vector_of<int>("the plan's axis", axis, pairs, q, at::kInt);
   const bool fractional = positions.scalar_type() == at::kFloat;
   need(positions.device() == q.device() && (fractional || positions.scalar_type() == at::kInt),
        "positions must be int32 or float32 on the device of q");
@@ -186,7 +189,7 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
     need(k->size(0) == b && k->size(1) == t && k->size(3) == d, "k must have the batch, tokens and head size of q");
   }
   On on(q);
-  a.batch = b, a.tokens = t, a.head_dim = (int)d, a.pairs = (int)turns.numel(), a.axes = (int)axes;
+  a.batch = b, a.tokens = t, a.head_dim = (int)d, a.pairs = (int)pairs, a.axes = (int)axes;
   a.interleaved = interleaved, a.inverse = inverse;
   auto fill = [](illumina_rotary_tensor &slot, const at::Tensor &x, const MaybeTensor &out, const char *name) {
     at::Tensor y;
@@ -210,7 +213,6 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
   a.positions = positions.data_ptr(), a.positions_float = fractional;
   a.position_stride[0] = positions.stride(0), a.position_stride[1] = pd == 3 ? positions.stride(1) : 0;
   a.position_stride[2] = positions.stride(-1);
-  a.turns = turns.data_ptr<double>(), a.axis = axis.data_ptr<int>();
   check(illumina_op_rotary(&a, on.stream));
   return {std::move(yq), std::move(yk)};
 }
