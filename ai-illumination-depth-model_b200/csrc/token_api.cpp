@@ -25,6 +25,11 @@ void require_precision(int precision, const char *op) {
           std::string(op) + ": unknown precision");
 }
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// Vectors of 32-bit values (weights, statistics, lengths); any may be null.
+template <typename... P>
+bool words(const P *...p) {
+  return (aligned(p, 4) && ...);
+}
 size_t size_of(int precision) { return precision == ILLUMINA_PRECISION_F32 ? 4 : 2; }
 
 void check_norm(int precision, long long rows, int c, const char *op) {
@@ -65,6 +70,7 @@ gpu::AttnParams attn_params(const illumina_attention_args *a, bool backward, boo
   const double rows = (double)a->batch * a->heads * ((double)a->q_tokens + 32) / 32;
   const double keys = (double)a->batch * a->kv_heads * ((double)a->k_tokens + 32) / 32;
   require(rows < 16e6 && keys < 1e9, "attention: too many rows for one call");
+  require(words(a->q_lens, a->k_lens, a->lse), "attention: misaligned lengths or lse");
   gpu::AttnParams p;
   p.batch = a->batch, p.heads = a->heads, p.kv_heads = a->kv_heads, p.head_dim = a->head_dim;
   p.q_tokens = a->q_tokens, p.k_tokens = a->k_tokens, p.causal_block = a->causal_block, p.scale = a->scale;
@@ -157,6 +163,7 @@ illumina_status illumina_op_layer_norm(int precision, const void *x, long long x
   check_norm(precision, rows, c, "layer_norm");
   require(rows == 0 || (x && y), "layer_norm: null pointer");
   require(aligned(x, size_of(precision)) && aligned(y, size_of(precision)), "layer_norm: misaligned tensor");
+  require(words(w, b, mean, rstd), "layer_norm: misaligned weights or statistics");
   require(eps >= 0, "layer_norm: eps must not be negative");
   cuda_check(gpu::layer_norm(precision, x, x_stride, rows, c, w, b, eps, y, y_stride, mean, rstd, (cudaStream_t)stream),
              "layer_norm");
@@ -183,6 +190,7 @@ illumina_status illumina_op_layer_norm_backward(int precision, const void *dy, l
   require(rows == 0 || (dy && x && mean && rstd), "layer_norm_backward: null pointer");
   const size_t e = size_of(precision);
   require(aligned(x, e) && aligned(dy, e) && aligned(dx, e), "layer_norm_backward: misaligned tensor");
+  require(words(w, mean, rstd, dw, db), "layer_norm_backward: misaligned weights or statistics");
   if (dw || db) {
     const size_t need = (size_t)gpu::layer_norm_blocks(rows, c) * 2 * c * sizeof(float);
     require(need == 0 || (workspace && aligned(workspace, 16)), "layer_norm_backward: workspace missing or misaligned");
@@ -211,6 +219,7 @@ illumina_status illumina_op_rotary(const illumina_rotary_args *a, void *stream) 
   p.t[1] = rotary_tensor(a->second, a->precision, some);
   require((long long)a->first.heads + a->second.heads <= 65536, "rotary: more than 65536 heads");
   require(!some || (a->positions && a->turns && a->axis), "rotary: null pointer");
+  require(aligned(a->positions, 4) && aligned(a->turns, 8) && words(a->axis), "rotary: misaligned positions or plan");
   p.batch = a->batch, p.tokens = a->tokens, p.head_dim = a->head_dim, p.pairs = a->pairs, p.axes = a->axes;
   p.interleaved = a->interleaved, p.inverse = a->inverse, p.pos = a->positions, p.pos_float = a->positions_float;
   p.turns = a->turns, p.axis = a->axis;
@@ -272,6 +281,7 @@ illumina_status illumina_adamw_create(const illumina_adamw_options *o, illumina_
   require(blocks > 0, "adamw: every tensor is empty");
   require(o->m && o->v && aligned(o->m, 16) && aligned(o->v, 16), "adamw: moments missing or misaligned");
   require(o->moment_bits == 32 || (o->m_scale && o->v_scale), "adamw: 8-bit moments need scales");
+  require(words(o->m_scale, o->v_scale), "adamw: misaligned scales");
   std::unique_ptr<illumina_adamw> opt(new illumina_adamw);
   opt->device = o->device, opt->tensors = o->tensors, opt->bits = o->moment_bits;
   opt->grad_precision = o->grad_precision, opt->blocks = blocks;
@@ -333,6 +343,7 @@ illumina_status illumina_adamw_step(illumina_adamw *opt, const void *const *grad
   require(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1, "adamw: betas outside [0, 1)");
   require(h->eps == 0 || h->eps >= FLT_MIN, "adamw: eps must be 0 or a normal float");
   require(std::isfinite(h->lr) && std::isfinite(h->weight_decay), "adamw: bad hyperparameter");
+  require(words(h->lr_device), "adamw: misaligned lr");
   const size_t e = size_of(opt->grad_precision);
   for (int i = 0; i < opt->tensors; i++)
     require(opt->counts[i] == 0 || (grads[i] && aligned(grads[i], e)),

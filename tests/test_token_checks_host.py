@@ -7,7 +7,7 @@ import pytest
 
 from illumina import _lib
 from tests.conftest import PKG_DIR
-from tests.test_tokens_host import refused
+from tests.test_tokens_host import attention_args, refused
 
 
 def rotary_args(**over):
@@ -33,3 +33,25 @@ print(_lib.lib().illumina_op_rotary(C.byref(a), None), _lib.lib().illumina_last_
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert run.returncode == 0 and run.stdout.startswith(f"{_lib.INVALID_ARG} ") and "pairs" in run.stdout
+
+
+def test_vectors_between_the_places_of_their_type():
+    lib = _lib.lib()
+    at, off = 0x1000, 0x1002
+    for n in range(4):  # w, b, mean, rstd
+        w, b, mean, rstd = (off if i == n else at for i in range(4))
+        refused(lib.illumina_op_layer_norm(0, at, 8, 4, 8, w, b, 1e-6, at, 8, mean, rstd, None), "misaligned")
+    for n in range(5):  # w, mean, rstd, dw, db
+        w, mean, rstd, dw, db = (off if i == n else at for i in range(5))
+        refused(lib.illumina_op_layer_norm_backward(0, at, 8, at, 8, 4, 8, w, mean, rstd, at, 8, dw, db, at, 1 << 20, None), "misaligned")
+    for over in (dict(positions=off), dict(turns=0x1004), dict(axis=off)):
+        refused(lib.illumina_op_rotary(C.byref(rotary_args(**over)), None), "misaligned")
+    for over in (dict(q_lens=off), dict(k_lens=off), dict(lse=off)):
+        refused(lib.illumina_op_attention(C.byref(attention_args(**over)), None), "misaligned")
+        a = attention_args(workspace=at, workspace_bytes=1 << 40, **over)
+        refused(lib.illumina_op_attention_backward(C.byref(a), None), "misaligned")
+    for name in ("m_scale", "v_scale"):
+        o = _lib.AdamwOptions(device=0, tensors=1, params=(C.c_void_p * 1)(at), counts=(C.c_longlong * 1)(5), moment_bits=8,
+                              m=at, v=at, m_scale=at, v_scale=at)
+        setattr(o, name, off)
+        refused(lib.illumina_adamw_create(C.byref(o), C.byref(C.c_void_p())), "misaligned")
