@@ -287,19 +287,35 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
   return {std::move(dq), std::move(dk), std::move(dv)};
 }
 
-// What a step of an optimiser checks its gradients against.
+// What a step of an optimiser checks its gradients against, and the tensors
+// whose places the optimiser was created with.
 struct Stepper {
   illumina_adamw *handle;
+  std::vector<at::Tensor> params, moments;
   std::vector<int64_t> counts;
-  std::vector<const void *> pointers;
+  std::vector<const void *> pointers, places;
   c10::Device device;
   bool bf16;
-  Stepper(uintptr_t h, std::vector<int64_t> n, int64_t index, bool b)
-      : handle((illumina_adamw *)h), counts(std::move(n)), device(c10::kCUDA, (c10::DeviceIndex)index), bf16(b) {
+  Stepper(uintptr_t h, std::vector<at::Tensor> p, std::vector<at::Tensor> m, int64_t index, bool b)
+      : handle((illumina_adamw *)h), params(std::move(p)), moments(std::move(m)),
+        device(c10::kCUDA, (c10::DeviceIndex)index), bf16(b) {
+    for (const at::Tensor &x : params) counts.push_back(x.numel()), places.push_back(x.data_ptr());
+    for (const at::Tensor &x : moments) places.push_back(x.data_ptr());
     pointers.resize(counts.size());
   }
 
+  // A tensor that was given other memory (p.data = ..., a module moved to another type or device) no longer lies
+  // where the optimiser writes.
+  void stay() const {
+    for (size_t i = 0; i < params.size(); i++)
+      if (params[i].data_ptr() != places[i] || params[i].numel() != counts[i])
+        refuse("adamw: parameter " + std::to_string(i) + " has moved since the optimizer was created");
+    for (size_t i = 0; i < moments.size(); i++)
+      need(moments[i].data_ptr() == places[params.size() + i], "adamw: the moments have moved since the optimizer was created");
+  }
+
   void step(const py::sequence &grads, const py::object &lr, double beta1, double beta2, double eps, double decay) {
+    stay();
     need(py::len(grads) == counts.size(), "adamw: one gradient for each parameter is needed");
     const auto type = bf16 ? at::kBFloat16 : at::kFloat;
     for (size_t i = 0; i < counts.size(); i++) {
@@ -341,6 +357,7 @@ PYBIND11_MODULE(_torch_ops, m) {
   m.def("attention", &attention);
   m.def("attention_backward", &attention_backward);
   py::class_<Stepper>(m, "Stepper")
-      .def(py::init<uintptr_t, std::vector<int64_t>, int64_t, bool>())
+      .def(py::init<uintptr_t, std::vector<at::Tensor>, std::vector<at::Tensor>, int64_t, bool>())
+      .def("stay", &Stepper::stay)
       .def("step", &Stepper::step);
 }

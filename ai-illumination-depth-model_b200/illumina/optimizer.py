@@ -57,10 +57,13 @@ class AdamW:
         handle = C.c_void_p()
         check(lib().illumina_adamw_create(C.byref(options), C.byref(handle)))
         self._h = handle
-        self._stepper = _load().Stepper(handle.value, list(counts), dev.index, gradDtype == torch.bfloat16)
+        moments = [x for x in (self.m, self.v, self.mScale, self.vScale) if x is not None]
+        self._stepper = _load().Stepper(handle.value, self.params, moments, dev.index, gradDtype == torch.bfloat16)
 
     def step(self, grads, stream=None):
-        """One step; grads: one contiguous tensor of gradDtype for each parameter, of its element count."""
+        """One step; grads: one contiguous tensor of gradDtype for each parameter, of its element count. The parameters
+        must lie where they lay at creation: a step after p.data = ... or a move of a module is refused (a captured step
+        cannot look, and must not be replayed then)."""
         _require(self._h is not None, "adamw: the optimizer was destroyed")
         args = (grads, self.lr, *self.betas, self.eps, self.weightDecay)
         if stream is None:
@@ -75,6 +78,7 @@ class AdamW:
         _require(self._h is not None, "adamw: the optimizer was destroyed")
         if self.momentBits == 32:
             return self.m, self.v
+        self._stepper.stay()
         with _On(self.device, stream) as handle:
             m = torch.empty(self.blocks * BLOCK, dtype=torch.float32, device=self.device)
             v = torch.empty_like(m)

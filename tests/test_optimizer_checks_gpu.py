@@ -1,0 +1,35 @@
+"""AdamW: what a step refuses and keeps of its arguments, and sizes that send its kernels round their loops."""
+import numpy as np
+import pytest
+
+from tests import token_reference as R
+from tests.test_optimizer_gpu import BLOCK, HYPER, codes, places, plain_8_bit, tensors, torch  # noqa: F401
+from tests.test_token_checks_gpu import refused
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_refuses_parameters_that_moved(torch, bits):  # noqa: F811
+    import illumina
+    p = [torch.nn.Parameter(torch.ones(n, device="cuda")) for n in (1000, 0, 300)]
+    g = [torch.ones(n, device="cuda") for n in (1000, 0, 300)]
+    opt = illumina.createOptimizer(p, momentBits=bits)
+    opt.step(g)
+    old, kept = p[2].data, p[2].detach().clone()
+    first = p[0].detach().clone()
+    p[2].data = torch.ones(300, device="cuda")
+    refused(lambda: opt.step(g), "parameter 2 has moved")
+    assert torch.equal(old, kept) and torch.equal(p[0], first) and opt.steps == 1
+    p[2].data = old[:200]  # the place of its first 200 elements
+    refused(lambda: opt.step(g), "parameter 2 has moved")
+    with torch.no_grad():
+        p[2].set_(torch.zeros(300, device="cuda"))
+    refused(lambda: opt.step(g), "parameter 2 has moved")
+    p[2].data = old
+    opt.step(g)
+    assert opt.steps == 2
+    opt.m.set_(opt.m.clone())
+    refused(lambda: opt.step(g), "moments have moved")
+    if bits == 8:
+        refused(opt.moments, "moments have moved")
