@@ -318,8 +318,11 @@ struct Stepper {
     stay();
     need(py::len(grads) == counts.size(), "adamw: one gradient for each parameter is needed");
     const auto type = bf16 ? at::kBFloat16 : at::kFloat;
+    std::vector<py::object> held;  // until the launch: a sequence may make its items as they are asked for
+    held.reserve(counts.size());
     for (size_t i = 0; i < counts.size(); i++) {
-      const py::object item = grads[i];
+      held.push_back(grads[i]);
+      const py::object &item = held.back();
       const at::Tensor *g = THPVariable_Check(item.ptr()) ? &THPVariable_Unpack(item.ptr()) : nullptr;
       if (!g || g->scalar_type() != type || g->device() != device || g->numel() != counts[i] || !g->is_contiguous())
         refuse("adamw: gradient " + std::to_string(i) + " must be " + std::to_string(counts[i]) + " contiguous " +

@@ -33,3 +33,27 @@ def test_refuses_parameters_that_moved(torch, bits):  # noqa: F811
     refused(lambda: opt.step(g), "moments have moved")
     if bits == 8:
         refused(opt.moments, "moments have moved")
+
+
+def test_gradients_made_as_they_are_asked_for(torch):  # noqa: F811
+    """Every gradient lives until the step is queued: here none would, and each could take the place of the one before."""
+    import illumina
+
+    class Cast:
+        def __init__(self, tensors):
+            self.tensors = tensors
+
+        def __len__(self):
+            return len(self.tensors)
+
+        def __getitem__(self, i):
+            return self.tensors[i].bfloat16()
+
+    grads = [torch.full((5000,), 0.01 * (i + 1), device="cuda") for i in range(6)]
+    runs = []
+    for given in ([g.bfloat16() for g in grads], Cast(grads)):
+        p = [torch.ones(5000, device="cuda") for _ in grads]
+        opt = illumina.createOptimizer(p, gradDtype=torch.bfloat16)
+        opt.step(given)
+        runs.append((*p, opt.m.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
