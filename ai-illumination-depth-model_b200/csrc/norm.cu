@@ -477,9 +477,10 @@ __global__ void __launch_bounds__(kThreads) k_norm_bwd_long(const T *__restrict_
 }
 
 // Column sums of part ([n][2c]) in a fixed order: a CTA takes 8 columns, its 32
-// groups of 8 threads every 32nd row, then the groups' sums are added.
-__global__ void __launch_bounds__(256) k_norm_reduce(const float *__restrict__ part, int n, int c, float *dw,
-                                                     float *db) {
+// groups of 8 threads every 32nd row, then the groups' sums are added. The rows
+// are still being written when the kernel starts: not read-only memory, and
+// read past the L1.
+__global__ void __launch_bounds__(256) k_norm_reduce(const float *part, int n, int c, float *dw, float *db) {
   __shared__ float s[8][33];
   const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
   const int col = blockIdx.x * 8 + tx;
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(256) k_norm_reduce(const float *__restrict__ p
   cudaGridDependencySynchronize();
   if (col < 2 * c) {
 #pragma unroll 4
-    for (int i = ty; i < n; i += 32) t += part[(size_t)i * 2 * c + col];
+    for (int i = ty; i < n; i += 32) t += __ldcg(part + (size_t)i * 2 * c + col);
   }
   s[tx][ty] = t;
   __syncthreads();

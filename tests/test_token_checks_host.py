@@ -1,5 +1,8 @@
 """Refusals of the token and AdamW entry points at the borders of their arguments' types; no GPU."""
 import ctypes as C
+import glob
+import os
+import re
 import subprocess
 import sys
 
@@ -55,3 +58,15 @@ def test_vectors_between_the_places_of_their_type():
                               m=at, v=at, m_scale=at, v_scale=at)
         setattr(o, name, off)
         refused(lib.illumina_adamw_create(C.byref(o), C.byref(C.c_void_p())), "misaligned")
+
+
+def test_kernels_that_start_early_promise_nothing_about_memory():
+    """A kernel launched to start while the one before it still writes must not declare what that one writes read-only for
+    its own life (const __restrict__ lets the compiler load it early, or through a cache that is not kept coherent)."""
+    sources = {f: open(f).read() for f in glob.glob(os.path.join(PKG_DIR, "csrc", "*.cu"))}
+    started = {(f, name) for f, text in sources.items() for name in re.findall(r"launch_next\((k_\w+)", text)}
+    assert {name for _, name in started} >= {"k_norm_reduce", "k_attn_join", "k_attn_dkv", "k_attn_dkv_join", "k_attn_dkv_tc"}
+    for f, name in started:
+        head, body = re.search(r"__global__[^;{]*?\b" + name + r"\((.*?)\)\s*\{(.*?)\n\}", sources[f], re.S).groups()
+        assert "__restrict__" not in head, name
+        assert "cudaGridDependencySynchronize();" in body, name
