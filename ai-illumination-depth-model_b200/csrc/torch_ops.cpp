@@ -9,7 +9,6 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 
 #include <optional>
 #include <string>
@@ -97,18 +96,69 @@ struct Rows {
   }
 };
 
-// An output that the caller gives: no element may lie under another.
+// Bytes from the first element of x to the end of its last.
+int64_t span_of(const at::Tensor &x) {
+  int64_t n = 1;
+  for (int64_t d = 0; d < x.dim(); d++) n += (x.size(d) - 1) * x.stride(d);
+  return n * (int64_t)x.element_size();
+}
+
+// An output that the caller gives: no element may lie under another, which is
+// sure where every dimension steps over all those with smaller strides.
 void writable(const char *name, const at::Tensor &x, const at::Tensor &like) {
   storage_like(name, x, like);
   need(x.sizes() == like.sizes(), name, "must have the shape of its input");
-  for (int64_t d = 0; d < x.dim(); d++) need(x.size(d) <= 1 || x.stride(d) != 0, name, "must not be broadcast");
+  if (x.numel() == 0) return;
+  for (int64_t d = 0; d < x.dim(); d++) {
+    if (x.size(d) <= 1) continue;
+    int64_t below = 1;
+    for (int64_t e = 0; e < x.dim(); e++)
+      if (x.size(e) > 1 && e != d && (x.stride(e) < x.stride(d) || (x.stride(e) == x.stride(d) && e < d)))
+        below += (x.size(e) - 1) * x.stride(e);
+    need(x.stride(d) >= below, name, "must not be broadcast or lie under itself");
+  }
+}
+
+// Whether x repeats with a pitch of `pitch` bytes: every stride is a multiple
+// of it, or belongs to the `width` bytes that x takes of each.
+bool repeats(const at::Tensor &x, int64_t pitch, int64_t &width) {
+  width = (int64_t)x.element_size();
+  for (int64_t d = 0; d < x.dim(); d++) {
+    if (x.size(d) <= 1) continue;
+    const int64_t step = x.stride(d) * (int64_t)x.element_size();
+    if (step < pitch) width += (x.size(d) - 1) * step;
+    else if (step % pitch) return false;
+  }
+  return width <= pitch;
+}
+
+// Whether no byte belongs to both: their ranges of addresses are apart, or they
+// take different parts of one pitch (the heads of a packed projection, columns
+// of the same rows).
+bool separate(const at::Tensor &x, const at::Tensor &y) {
+  if (x.numel() == 0 || y.numel() == 0) return true;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x.const_data_ptr()), b = reinterpret_cast<uintptr_t>(y.const_data_ptr());
+  if (a + span_of(x) <= b || b + span_of(y) <= a) return true;
+  for (const at::Tensor *t : {&x, &y})
+    for (int64_t d = 0; d < t->dim(); d++) {
+      const int64_t pitch = t->stride(d) * (int64_t)t->element_size();
+      int64_t wx, wy;
+      if (t->size(d) <= 1 || pitch <= 0 || !repeats(x, pitch, wx) || !repeats(y, pitch, wy)) continue;
+      const int64_t at = (int64_t)((b % pitch + pitch - a % pitch) % pitch);  // y's part, from the start of x's
+      if (at >= wx && at + wy <= pitch) return true;
+    }
+  return false;
 }
 
 // An output may be the input whose place it takes, element for element, but
-// not another view of the same memory (as far as strides tell in short).
+// must not share memory with it, or with another input, in any other way.
 void apart(const char *name, const at::Tensor &out, const at::Tensor &in, bool in_place) {
-  const auto s = at::get_overlap_status(out, in);
-  need(s != at::MemOverlapStatus::Partial && (in_place || s != at::MemOverlapStatus::Full), name, "must not overlap an input");
+  if (in_place && out.const_data_ptr() == in.const_data_ptr() && out.sizes() == in.sizes()) {
+    bool same = true;
+    for (int64_t d = 0; d < out.dim(); d++) same = same && (out.size(d) <= 1 || out.stride(d) == in.stride(d));
+    if (same) return;
+  }
+  need(separate(out, in), name, "must not overlap an input");
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor &x, const MaybeTensor &weight,
@@ -125,6 +175,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor &x, c
     y = *out;
     writable("out", y, x);
     apart("out", y, x, true);
+    if (weight.has_value()) apart("out", y, *weight, false);
+    if (bias.has_value()) apart("out", y, *bias, false);
     y_stride = Rows("out", y).stride;
   } else {
     y = at::empty(x.sizes(), x.options());
@@ -191,12 +243,13 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
   On on(q);
   a.batch = b, a.tokens = t, a.head_dim = (int)d, a.pairs = (int)pairs, a.axes = (int)axes;
   a.interleaved = interleaved, a.inverse = inverse;
-  auto fill = [](illumina_rotary_tensor &slot, const at::Tensor &x, const MaybeTensor &out, const char *name) {
+  auto fill = [&](illumina_rotary_tensor &slot, const at::Tensor &x, const MaybeTensor &out, const char *name) {
     at::Tensor y;
     if (out.has_value()) {
       y = *out;
       writable(name, y, x);
       apart(name, y, x, true);
+      for (const at::Tensor *t : {&positions, &turns, &axis}) apart(name, y, *t, false);
     } else {
       y = at::empty(x.sizes(), x.options());
     }
@@ -208,7 +261,9 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
   MaybeTensor yk;
   if (k.has_value()) {
     yk = fill(a.second, *k, out_k, "outK");
-    apart("outQ", yq, *k, false), apart("outK", *yk, q, false), apart("outQ", yq, *yk, false);
+    if (out_q.has_value()) apart("outQ", yq, *k, false);
+    if (out_k.has_value()) apart("outK", *yk, q, false);
+    if (out_q.has_value() && out_k.has_value()) apart("outQ", yq, *yk, false);
   }
   a.positions = positions.data_ptr(), a.positions_float = fractional;
   a.position_stride[0] = positions.stride(0), a.position_stride[1] = pd == 3 ? positions.stride(1) : 0;

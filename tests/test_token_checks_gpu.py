@@ -29,3 +29,60 @@ def test_rotary_plans_made_by_hand(torch, ops):  # noqa: F811
         refused(lambda: ops.rotary(q, pos, replace(plan, **over)), word)
     few = replace(plan, turns=plan.turns[:8].clone(), axis=plan.axis[:8].clone())
     assert torch.equal(ops.rotary(q, pos, few)[..., 16:], q[..., 16:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_outputs_that_share_memory_in_views_with_gaps(torch, ops, dtype):  # noqa: F811
+    import illumina
+    plan = illumina.createRotary(32, [16])
+    pos = torch.arange(10, dtype=torch.int32, device="cuda")[None]
+    packed = randn(torch, 2, 10, 8, 32, dtype=dtype)
+    kept = packed.clone()
+    q, k = packed[:, :, :4], packed[:, :, 4:6]
+    wide = randn(torch, 20, 3, 208, dtype=dtype)
+    x = wide[:, 1, 8:184]
+    heads_first = randn(torch, 2, 8, 10, 32, dtype=dtype).transpose(1, 2)
+    rows = randn(torch, 40, 64, dtype=dtype)
+    flat = randn(torch, 4000, dtype=dtype)
+    for call in (lambda: ops.rotary(q, pos, plan, outQ=packed[:, :, 1:5]), lambda: ops.rotary(q, pos, plan, k=k, outK=packed[:, :, 3:5]),
+                 lambda: ops.rotary(q, pos, plan, k=k, outQ=packed[:, :, 2:6]), lambda: ops.rotary(q[:, :9], pos[:, :9], plan, outQ=q[:, 1:]),
+                 lambda: ops.rotary(q, pos, plan, k=k, outQ=packed[:, :, 4:8]),
+                 lambda: ops.rotary(q, pos, plan, outQ=packed.view(-1)[1:].as_strided(q.shape, q.stride())),
+                 lambda: ops.rotary(heads_first[:, :, :4], pos, plan, outQ=heads_first[:, :, 1:5]),
+                 lambda: ops.layerNorm(x, out=wide[:, 1, 9:185]), lambda: ops.layerNorm(x[:19], out=x[1:]),
+                 lambda: ops.layerNorm(x[:10], out=wide.view(-1)[624 + 208 + 8:].as_strided((10, 176), (312, 1))),
+                 lambda: ops.layerNorm(rows[:20], out=rows.view(-1).as_strided((20, 64), (128, 1)))):
+        refused(call, "overlap an input")
+    # results that lie under themselves
+    refused(lambda: ops.layerNorm(randn(torch, 20, 64, dtype=dtype), out=flat.as_strided((20, 64), (32, 1))), "under itself")
+    refused(lambda: ops.rotary(q, pos, plan, outQ=flat.as_strided(q.shape, (640, 64, 16, 1))), "under itself")
+    assert torch.equal(packed, kept)
+    # parts of the same rows that do not meet, and results in place
+    want = ops.rotary(q, pos, plan, k=k)
+    got = ops.rotary(q, pos, plan, k=k, outK=packed[:, :, 6:])
+    assert torch.equal(got[1], want[1]) and torch.equal(packed[:, :, :6], kept[:, :, :6])
+    got = ops.rotary(q, pos, plan, k=k, outQ=q, outK=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    half = ops.rotary(heads_first[:, :, :4], pos, plan)
+    ops.rotary(heads_first[:, :, :4], pos, plan, outQ=heads_first[:, :, 4:])
+    assert torch.equal(half, heads_first[:, :, 4:])
+    y = ops.layerNorm(x)[0]
+    ops.layerNorm(x, out=wide[:, 0, 8:184])
+    assert torch.equal(y, wide[:, 0, 8:184])
+    y = ops.layerNorm(rows[::2])[0]
+    ops.layerNorm(rows[::2], out=rows[1::2])
+    assert torch.equal(y, rows[1::2])
+    one = randn(torch, 1, 64, dtype=dtype)  # the stride of a single row says nothing
+    y = ops.layerNorm(one)[0]
+    ops.layerNorm(one, out=one.as_strided((1, 64), (7, 1)))
+    assert torch.equal(y, one)
+
+
+def test_outputs_that_share_memory_with_weights_or_positions(torch, ops):  # noqa: F811
+    import illumina
+    w, x = randn(torch, 64), randn(torch, 1, 64)
+    refused(lambda: ops.layerNorm(x, w, out=w[None]), "overlap an input")
+    refused(lambda: ops.layerNorm(x, None, w, out=w[None]), "overlap an input")
+    plan = illumina.createRotary(32, [16])
+    place = torch.zeros(1, 10, 4, 32, device="cuda")
+    refused(lambda: ops.rotary(randn(torch, 1, 10, 4, 32), place.view(-1)[100:110][None], plan, outQ=place), "overlap an input")
