@@ -5,6 +5,7 @@
 // as long.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -49,6 +50,21 @@ struct On {
     stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
   }
 };
+
+// The calls record nothing for autograd: a tensor whose gradient or tangent
+// would be lost is refused.
+inline void no_gradient(const at::Tensor &x) {
+  need(!(c10::GradMode::is_enabled() && x.requires_grad()),
+       "a tensor requires a gradient, which these calls do not record: detach it, or call under torch.no_grad()");
+  need(!x._fw_grad(0).defined(), "a tensor carries a tangent, which these calls do not pass on");
+}
+inline void no_gradient(const MaybeTensor &x) {
+  if (x.has_value()) no_gradient(*x);
+}
+template <typename... X>
+void no_gradients(const X &...x) {
+  (no_gradient(x), ...);
+}
 
 // A storage tensor: on a CUDA device, float32 or bfloat16, contiguous in its
 // last dimension; returns its precision.
@@ -163,6 +179,7 @@ void apart(const char *name, const at::Tensor &out, const at::Tensor &in, bool i
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor &x, const MaybeTensor &weight,
                                                           const MaybeTensor &bias, double eps, const MaybeTensor &out) {
+  no_gradients(x, weight, bias, out);
   const int precision = storage("x", x);
   const Rows r("x", x);
   need(r.width > 0, "x must not have a width of zero");
@@ -191,6 +208,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor &x, c
 std::tuple<at::Tensor, MaybeTensor, MaybeTensor> layer_norm_backward(const at::Tensor &dy, const at::Tensor &x,
                                                                      const MaybeTensor &mean, const MaybeTensor &rstd,
                                                                      const MaybeTensor &weight, bool need_weight) {
+  no_gradients(dy, x, mean, rstd, weight);
   const int precision = storage("x", x);
   storage_like("dy", dy, x);
   need(dy.sizes() == x.sizes(), "dy must have the shape of x");
@@ -222,6 +240,7 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
                                            const at::Tensor &turns, const at::Tensor &axis, int64_t axes, int64_t head_dim,
                                            bool interleaved, bool inverse, const MaybeTensor &out_q,
                                            const MaybeTensor &out_k) {
+  no_gradients(q, k, positions, turns, out_q, out_k);
   illumina_rotary_args a{};
   a.precision = storage("q", q, 4);
   const int64_t b = q.size(0), t = q.size(1), d = q.size(3);
@@ -311,6 +330,7 @@ at::Tensor attention_workspace(illumina_attention_args &a, int backward, const a
 std::tuple<at::Tensor, at::Tensor> attention(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
                                              std::optional<double> scale, int64_t causal_block, const MaybeTensor &q_lens,
                                              const MaybeTensor &k_lens) {
+  no_gradients(q, k, v);
   illumina_attention_args a = attention_args(q, k, v, scale, causal_block, q_lens, k_lens);
   On on(q);
   at::Tensor out = at::empty(q.sizes(), q.options());
@@ -327,6 +347,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
                                                                   const at::Tensor &out, const MaybeTensor &lse,
                                                                   std::optional<double> scale, int64_t causal_block,
                                                                   const MaybeTensor &q_lens, const MaybeTensor &k_lens) {
+  no_gradients(dout, q, k, v, out, lse);
   illumina_attention_args a = attention_args(q, k, v, scale, causal_block, q_lens, k_lens);
   storage_like("dOut", dout, q, 4);
   storage_like("out", out, q, 4);

@@ -10,8 +10,11 @@ network's feature maps, or over the frames of a clip. They take shaped torch
 CUDA tensors of one device, float32 or bfloat16, with any strides over a
 contiguous last dimension, and run on `stream` (a torch stream or handle; by
 default torch's current stream of that device), where their results are
-allocated too. Inputs must stay alive until the work is done. Errors are
-IlluminaError with status INVALID_ARG.
+allocated too. Inputs must stay alive until the work is done. Autograd is not
+part of them: a tensor that requires a gradient is refused (unless under
+torch.no_grad()), and so is one with a forward-mode tangent; the backward
+passes are calls of their own. Errors are IlluminaError with status
+INVALID_ARG.
 """
 from __future__ import annotations
 

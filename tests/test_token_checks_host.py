@@ -70,3 +70,28 @@ def test_kernels_that_start_early_promise_nothing_about_memory():
         head, body = re.search(r"__global__[^;{]*?\b" + name + r"\((.*?)\)\s*\{(.*?)\n\}", sources[f], re.S).groups()
         assert "__restrict__" not in head, name
         assert "cudaGridDependencySynchronize();" in body, name
+
+
+def test_gradients_are_not_lost_in_silence():
+    torch = pytest.importorskip("torch")
+    import illumina
+    from illumina import ops
+    x, q, w = torch.zeros(4, 8), torch.zeros(1, 4, 2, 8), torch.zeros(8, requires_grad=True)
+    g, qg = x.clone().requires_grad_(), q.clone().requires_grad_()
+    lse, stats, positions = torch.zeros(1, 2, 4), torch.zeros(4), torch.zeros(1, 4, dtype=torch.int32)
+    plan = illumina.createRotary(8, [4], device="cpu")
+    calls = [lambda: ops.layerNorm(g), lambda: ops.layerNorm(x, w), lambda: ops.layerNorm(x, None, w), lambda: ops.layerNorm(x, out=g),
+             lambda: ops.layerNormBackward(g, x, stats, stats), lambda: ops.layerNormBackward(x, g, stats, stats),
+             lambda: ops.layerNormBackward(x, x, stats, stats, w), lambda: ops.rotary(qg, positions, plan),
+             lambda: ops.rotary(q, positions, plan, k=qg), lambda: ops.rotary(q, positions, plan, outQ=qg),
+             lambda: ops.attention(qg, q, q), lambda: ops.attention(q, qg, q), lambda: ops.attention(q, q, qg),
+             lambda: ops.attentionBackward(qg, q, q, q, q, lse), lambda: ops.attentionBackward(q, q, q, q, qg, lse)]
+    for i, call in enumerate(calls):
+        with pytest.raises(illumina.IlluminaError, match="requires a gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(illumina.IlluminaError, match="CUDA tensor"):
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(illumina.IlluminaError, match="tangent"):
+            ops.layerNorm(dual)
