@@ -177,6 +177,14 @@ void apart(const char *name, const at::Tensor &out, const at::Tensor &in, bool i
   need(separate(out, in), name, "must not overlap an input");
 }
 
+// x was written in place: autograd finds it changed if it had saved it.
+void written(const at::Tensor &x) {
+  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+void written(const MaybeTensor &x) {
+  if (x.has_value()) written(*x);
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor &x, const MaybeTensor &weight,
                                                           const MaybeTensor &bias, double eps, const MaybeTensor &out) {
   no_gradients(x, weight, bias, out);
@@ -202,6 +210,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor &x, c
   at::Tensor mean = at::empty({r.rows}, f32), rstd = at::empty({r.rows}, f32);
   check(illumina_op_layer_norm(precision, x.data_ptr(), r.stride, r.rows, (int)r.width, w, b, (float)eps, y.data_ptr(),
                                y_stride, mean.data_ptr<float>(), rstd.data_ptr<float>(), on.stream));
+  written(out);
   return {std::move(y), std::move(mean), std::move(rstd)};
 }
 
@@ -288,6 +297,7 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
   a.position_stride[0] = positions.stride(0), a.position_stride[1] = pd == 3 ? positions.stride(1) : 0;
   a.position_stride[2] = positions.stride(-1);
   check(illumina_op_rotary(&a, on.stream));
+  written(out_q), written(out_k);
   return {std::move(yq), std::move(yk)};
 }
 
@@ -416,6 +426,7 @@ struct Stepper {
     }
     h.beta1 = beta1, h.beta2 = beta2, h.eps = eps, h.weight_decay = decay;
     check(illumina_adamw_step(handle, pointers.data(), &h, c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+    for (const at::Tensor &x : params) written(x);
   }
 };
 

@@ -86,3 +86,41 @@ def test_outputs_that_share_memory_with_weights_or_positions(torch, ops):  # noq
     plan = illumina.createRotary(32, [16])
     place = torch.zeros(1, 10, 4, 32, device="cuda")
     refused(lambda: ops.rotary(randn(torch, 1, 10, 4, 32), place.view(-1)[100:110][None], plan, outQ=place), "overlap an input")
+
+
+def test_autograd_sees_what_the_calls_overwrite(torch, ops):  # noqa: F811
+    import illumina
+    plan, pos = illumina.createRotary(32, [16]), torch.arange(10, dtype=torch.int32, device="cuda")[None]
+    leaf = torch.ones(1, 10, 4, 32, device="cuda", requires_grad=True)
+    flat = torch.ones(40, 32, device="cuda", requires_grad=True)
+    for call in (lambda x: ops.rotary(x, pos, plan, outQ=x), lambda x: ops.rotary(x.clone(), pos, plan, k=x, outK=x)):
+        x = randn(torch, 1, 10, 4, 32)
+        loss = (leaf * x).sum()  # saves x
+        call(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    x = randn(torch, 40, 32)
+    loss = (flat * x).sum()
+    ops.layerNorm(x, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    p = [torch.nn.Parameter(torch.ones(8, 8, device="cuda")), torch.nn.Parameter(torch.ones(0, device="cuda"))]
+    opt = illumina.createOptimizer(p)
+    a = torch.ones(8, 8, device="cuda", requires_grad=True)
+    loss = (a @ p[0]).sum()  # saves p[0]
+    opt.step([torch.ones(8, 8, device="cuda"), torch.ones(0, device="cuda")])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        x = randn(torch, 40, 32)
+        want = ops.layerNorm(x)[0]
+        ops.layerNorm(x, out=x)
+        assert torch.equal(x, want)
+
+
+def test_parameters_are_taken_without_a_graph(torch, ops):  # noqa: F811
+    x, w = randn(torch, 40, 32), torch.nn.Parameter(torch.ones(32, device="cuda"))
+    refused(lambda: ops.layerNorm(x, w), "requires a gradient")
+    want = ops.layerNorm(x, w.detach())[0]
+    with torch.no_grad():
+        assert torch.equal(ops.layerNorm(x, w)[0], want)
