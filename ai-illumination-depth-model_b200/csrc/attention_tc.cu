@@ -80,6 +80,7 @@ struct TcArgs {
   int q_tiles, k_tiles;  // per (batch, key head)
   int splits;
   int n16;               // head_dim rounded up to the MMA's 16 columns
+  long long wait;        // cycles a wait may take
   int qh, qb, kh, kb, vh, vb, gh, gb;  // 0: that dimension of the tensor is broadcast (stride 0)
 };
 
@@ -217,11 +218,12 @@ __device__ __forceinline__ bool try_wait(uint64_t *bar, uint32_t parity) {
 // A wait that ends when another role of the CTA has given up, too.
 struct Waiter {
   volatile int *fail;
+  long long limit;
   __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity) const {
     if (try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     while (!try_wait(bar, parity)) {
-      if (*fail || clock64() - t0 > kWaitCycles) {
+      if (*fail || clock64() - t0 > limit) {
         *fail = 1;
         return false;
       }
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  const Waiter wait{fail};
+  const Waiter wait{fail, a.wait};
 
   if (warp >= roles.copy) {
     reg_dealloc<88>();
@@ -698,7 +700,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   // accumulators of the first pipeline, and t_next further those of the second
   const uint32_t t_s = tmem, t_g = tmem + 128, t_dv = tmem + 256, t_dk = tmem + (kTwin ? 384 : 256 + DP);
   constexpr uint32_t t_next = kTwin ? 64 : 0;
-  const Waiter wait{fail};
+  const Waiter wait{fail, a.wait};
 
   if (warp == roles.copy && (threadIdx.x & 31) == 0 && some) {
     mbar_expect_tx(kv_full, 2 * L::kTile);
@@ -950,7 +952,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const uint32_t t_s = tmem, t_g = tmem + 128, t_dq = tmem + 256;
-  const Waiter wait{fail};
+  const Waiter wait{fail, a.wait};
 
   if (warp == roles.copy && (threadIdx.x & 31) == 0 && t1 > 0) {
     mbar_expect_tx(q_full, 2 * L::kBoxes * a.group * a.tpt * 128);
@@ -1158,6 +1160,7 @@ TcArgs shape_of(const AttnParams &p) {
   a.k_tiles = (p.k_tokens + 127) / 128;
   a.n16 = (p.head_dim + 15) / 16 * 16;
   a.splits = 1;
+  a.wait = p.wait > 0 ? p.wait : kWaitCycles;
   return a;
 }
 

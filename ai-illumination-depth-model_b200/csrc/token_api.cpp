@@ -93,26 +93,34 @@ gpu::AttnParams attn_params(const illumina_attention_args *a, bool backward, boo
   return p;
 }
 
-// The word that attention kernels set when they give up a bounded wait: host
-// memory that every device can write, allocated on first use (a call that is
-// being captured included). A later call reports and clears it.
-int *attention_error() {
-  static int *const word = [] {
+// The words that attention kernels set when they give up a bounded wait, one a
+// device: host memory that every device can write, allocated on first use (a
+// call that is being captured included).
+constexpr int kMostDevices = 64;
+int *attention_words() {
+  static int *const words = [] {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "attention: capture mode");
     void *p = nullptr;
-    const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    const cudaError_t e = cudaHostAlloc(&p, kMostDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
     cudaThreadExchangeStreamCaptureMode(&mode);
     cuda_check(e, "attention: cudaHostAlloc");
-    *(int *)p = 0;
+    std::memset(p, 0, kMostDevices * sizeof(int));
     return (int *)p;
   }();
-  if (*(volatile int *)word) {
-    *(volatile int *)word = 0;
-    throw Error(ILLUMINA_TIMEOUT, "attention: a kernel of an earlier call gave up a bounded wait");
-  }
+  return words;
+}
+// The current device's word; whoever finds it set clears it and reports it.
+int *attention_error() {
+  int device = 0;
+  cuda_check(cudaGetDevice(&device), "attention: cudaGetDevice");
+  require(device < kMostDevices, "attention: more devices than expected");
+  int *word = attention_words() + device;
+  if (__atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL))
+    throw Error(ILLUMINA_TIMEOUT, "attention: a kernel of an earlier call on this device gave up a bounded wait");
   return word;
 }
+thread_local long long g_attention_wait = 0;
 
 }  // namespace
 
@@ -240,7 +248,7 @@ illumina_status illumina_op_attention_workspace(const illumina_attention_args *a
 illumina_status illumina_op_attention(const illumina_attention_args *a, void *stream) {
   ILL_TRY
   gpu::AttnParams p = attn_params(a, false, true);
-  p.err = attention_error();
+  p.err = attention_error(), p.wait = g_attention_wait;
   cuda_check(gpu::attention(a->precision, p, (cudaStream_t)stream), "attention");
   return ILLUMINA_OK;
   ILL_CATCH
@@ -249,8 +257,23 @@ illumina_status illumina_op_attention(const illumina_attention_args *a, void *st
 illumina_status illumina_op_attention_backward(const illumina_attention_args *a, void *stream) {
   ILL_TRY
   gpu::AttnParams p = attn_params(a, true, true);
-  p.err = attention_error();
+  p.err = attention_error(), p.wait = g_attention_wait;
   cuda_check(gpu::attention_backward(a->precision, p, (cudaStream_t)stream), "attention_backward");
+  return ILLUMINA_OK;
+  ILL_CATCH
+}
+
+illumina_status illumina_op_attention_status(void) {
+  ILL_TRY
+  attention_error();
+  return ILLUMINA_OK;
+  ILL_CATCH
+}
+
+illumina_status illumina_op_attention_set_wait_limit(long long cycles) {
+  ILL_TRY
+  require(cycles >= 0, "attention: negative wait limit");
+  g_attention_wait = cycles;
   return ILLUMINA_OK;
   ILL_CATCH
 }

@@ -64,6 +64,7 @@ struct AttnParams {
   // sums of dout * out
   float *ws = nullptr;
   int *err = nullptr;  // host-mapped word: a tensor-core kernel gave up a bounded wait
+  long long wait = 0;  // cycles such a wait may take; 0: the default
 };
 // Bytes of workspace of the forward / backward.
 size_t attention_workspace(int T, const AttnParams &p, bool backward);

@@ -178,6 +178,8 @@ SIGNATURES = {
     "illumina_op_attention_workspace": (_S, [_V, C.c_int, C.POINTER(C.c_size_t)]),
     "illumina_op_attention": (_S, [_V, _V]),
     "illumina_op_attention_backward": (_S, [_V, _V]),
+    "illumina_op_attention_status": (_S, []),
+    "illumina_op_attention_set_wait_limit": (_S, [C.c_longlong]),
     "illumina_adamw_blocks": (_S, [C.POINTER(C.c_longlong), C.c_int, C.POINTER(C.c_longlong)]),
     "illumina_adamw_create": (_S, [C.POINTER(AdamwOptions), C.POINTER(C.c_void_p)]),
     "illumina_adamw_destroy": (_S, [_V]),

@@ -215,3 +215,19 @@ def attention(q, k, v, scale=None, causalBlock=0, qLens=None, kLens=None, stream
 def attentionBackward(dOut, q, k, v, out, lse, scale=None, causalBlock=0, qLens=None, kLens=None, stream=None):
     """Gradients (dq, dk, dv) of attention, from its results out and lse and the same masks."""
     return _call("attention_backward", stream, dOut, q, k, v, out, lse, scale, causalBlock, qLens, kLens)
+
+
+def checkAttention(device=None) -> None:
+    """Raises IlluminaError with status TIMEOUT if a tensor-core kernel of an attention call on the device (the current
+    one) gave up a bounded wait since this was last reported: the results of that call are undefined. Does not wait for
+    the device: ask after the work, a replayed graph's too, has been synchronised. The next attention call on the device
+    asks as well, and is not queued when it raises."""
+    import torch
+    with torch.cuda.device(device):
+        check(lib().illumina_op_attention_status())
+
+
+def setAttentionWaitLimit(cycles: int) -> None:
+    """Cycles such a wait may take in the attention calls of this thread from now on; 0 restores the default (about a
+    second). Captured calls keep the limit they were captured with."""
+    check(lib().illumina_op_attention_set_wait_limit(int(cycles)))

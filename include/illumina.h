@@ -460,10 +460,18 @@ typedef struct illumina_attention_args {
 illumina_status illumina_op_attention_workspace(const illumina_attention_args *args, int backward, size_t *bytes);
 illumina_status illumina_op_attention(const illumina_attention_args *args, void *stream);
 /* Recomputes the probabilities from lse. Every sum has a fixed order, over the
- * query heads that share a key head too: the same inputs give the same bits.
- * ILLUMINA_TIMEOUT from either call: a tensor-core kernel of an earlier call
- * gave up a bounded wait (that call's outputs are undefined). */
+ * query heads that share a key head too: the same inputs give the same bits. */
 illumina_status illumina_op_attention_backward(const illumina_attention_args *args, void *stream);
+/* ILLUMINA_TIMEOUT, once, if a tensor-core kernel of an attention call on the
+ * current device gave up a bounded wait since this was last reported: that
+ * call's outputs are undefined. Does not wait: ask after the work, a replayed
+ * graph's too, has been synchronised. The next attention call on the device
+ * asks as well, and is not queued when it reports. */
+illumina_status illumina_op_attention_status(void);
+/* Cycles such a wait may take in the attention calls of this thread from now
+ * on (0 = the default, ~1 s); captured calls keep theirs. A small limit makes
+ * the waits give up, so that the error path can be exercised. */
+illumina_status illumina_op_attention_set_wait_limit(long long cycles);
 
 /* ---------------------------------------------------------------------------
  * AdamW over many tensors (the weights of a model, illumina_weights_* order or

@@ -95,3 +95,8 @@ def test_gradients_are_not_lost_in_silence():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises(illumina.IlluminaError, match="tangent"):
             ops.layerNorm(dual)
+
+
+def test_attention_wait_limit_refusal():
+    refused(_lib.lib().illumina_op_attention_set_wait_limit(-1), "negative")
+    assert _lib.lib().illumina_op_attention_set_wait_limit(0) == _lib.OK
