@@ -535,15 +535,17 @@ bool vec_rows(const AttnTensor &t) {
 
 int ceil_div(long long a, int b) { return (int)((a + b - 1) / b); }
 
-// Shares of the keys in the forward: as many as give every SM a CTA, while a
+// `want` shares of `tiles`, without those that would be left empty.
+int even_shares(int tiles, int want) { return ceil_div(tiles, ceil_div(tiles, want)); }
+
+// Shares of the keys in the forward: as many as give every SM two CTAs, while a
 // share keeps at least four key tiles (joining costs another launch).
 template <int STR>
 int simt_splits(const AttnParams &p) {
   const long long ctas = (long long)p.batch * p.heads * ceil_div(p.q_tokens, kFix);
   const int tiles = ceil_div(p.k_tokens, STR);
   if (ctas == 0 || ctas >= 148 || tiles < 8) return 1;
-  const int want = (int)(kMostSplits / ctas), most = tiles / 4;
-  return want < most ? want : most;
+  return even_shares(tiles, (int)std::min<long long>(kMostSplits / ctas, tiles / 4));
 }
 
 // Shares of the query tiles that the keys of one CTA of dK and dV see: the same
@@ -553,8 +555,9 @@ template <int STR>
 int dkv_splits(const AttnParams &p) {
   const long long ctas = (long long)p.batch * p.kv_heads * ceil_div(p.k_tokens, kFix);
   if (ctas == 0 || ctas >= 148) return 1;
-  const long long want = 2 * 148 / ctas, most = (long long)ceil_div(p.q_tokens, STR) * (p.heads / p.kv_heads) / 2;
-  return (int)std::max(1ll, std::min(want, most));
+  const int tiles = ceil_div(p.q_tokens, STR) * (p.heads / p.kv_heads);
+  const long long want = std::min<long long>(kMostSplits / ctas, tiles / 2);
+  return want <= 1 ? 1 : even_shares(tiles, (int)want);
 }
 
 template <typename T, int DP, int STR>

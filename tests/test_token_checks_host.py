@@ -100,3 +100,27 @@ def test_gradients_are_not_lost_in_silence():
 def test_attention_wait_limit_refusal():
     refused(_lib.lib().illumina_op_attention_set_wait_limit(-1), "negative")
     assert _lib.lib().illumina_op_attention_set_wait_limit(0) == _lib.OK
+
+
+def shares(backward, **over):
+    """Shares that the workspace has room for: of the keys (forward), of the query tiles (backward)."""
+    a, n = attention_args(precision=0, **over), C.c_size_t(0)
+    assert _lib.lib().illumina_op_attention_workspace(C.byref(a), backward, C.byref(n)) == _lib.OK
+    rows = a.batch * a.heads * a.q_tokens
+    if not backward:
+        return n.value // (4 * rows * (a.head_dim + 1)) or 1
+    return (n.value - 4 * ((rows + 3) // 4 * 4)) // (8 * a.batch * a.kv_heads * a.k_tokens * a.head_dim) or 1
+
+
+@pytest.mark.parametrize("tokens", [25000, 3000, 513, 512, 511, 200, 64, 1])
+@pytest.mark.parametrize("heads", [(1, 1), (4, 1), (12, 4)])
+@pytest.mark.parametrize("d", [32, 104])
+def test_no_share_of_the_cuda_core_kernels_is_planned_empty(tokens, heads, d):
+    wide = 64 if d <= 64 else 32
+    h, hk = heads
+    for backward in (0, 1):
+        n = shares(backward, batch=1, heads=h, kv_heads=hk, head_dim=d, q_tokens=tokens if backward else 30,
+                   k_tokens=30 if backward else tokens)
+        tiles = -(-tokens // wide) * (h // hk if backward else 1)
+        per = -(-tiles // n)
+        assert n == 1 or (n - 1) * per < tiles, (backward, n, tiles)
