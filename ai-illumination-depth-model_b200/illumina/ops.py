@@ -124,8 +124,11 @@ class _On:
 
     def __init__(self, device, stream):
         import torch
+        _require(device.type == "cuda", "the tensors of a call must be CUDA tensors")
         if isinstance(stream, int):
             stream = torch.cuda.ExternalStream(stream, device=device)
+        # a stream of another device would leave the call on the current stream of this one
+        _require(stream is None or stream.device == device, f"stream must be a stream of {device}")
         self._scopes = [torch.cuda.device(device)] + ([] if stream is None else [torch.cuda.stream(stream)])
         self._handle = (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
 

@@ -124,3 +124,20 @@ def test_no_share_of_the_cuda_core_kernels_is_planned_empty(tokens, heads, d):
         tiles = -(-tokens // wide) * (h // hk if backward else 1)
         per = -(-tiles // n)
         assert n == 1 or (n - 1) * per < tiles, (backward, n, tiles)
+
+
+def test_streams_of_another_device_are_refused():
+    torch = pytest.importorskip("torch")
+    import illumina
+    from illumina import ops
+
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 0
+
+    with pytest.raises(illumina.IlluminaError, match="stream of cuda:0") as e:
+        ops._On(torch.device("cuda", 0), Stream())
+    assert e.value.status == _lib.INVALID_ARG
+    x = torch.zeros(4, 8)
+    for stream in (0, Stream()):
+        with pytest.raises(illumina.IlluminaError, match="CUDA tensor"):
+            ops.layerNorm(x, stream=stream)
