@@ -93,18 +93,26 @@ gpu::AttnParams attn_params(const illumina_attention_args *a, bool backward, boo
   return p;
 }
 
+// Allows a scope calls that a capture, on whichever thread, would otherwise be
+// ended by: allocating and freeing memory that the capture does not know.
+struct Uncaptured {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  const bool set = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+  ~Uncaptured() {
+    if (set) cudaThreadExchangeStreamCaptureMode(&mode);
+  }
+};
+
 // The words that attention kernels set when they give up a bounded wait, one a
 // device: host memory that every device can write, allocated on first use (a
 // call that is being captured included).
 constexpr int kMostDevices = 64;
 int *attention_words() {
   static int *const words = [] {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "attention: capture mode");
+    const Uncaptured scope;
     void *p = nullptr;
-    const cudaError_t e = cudaHostAlloc(&p, kMostDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    cuda_check(e, "attention: cudaHostAlloc");
+    cuda_check(cudaHostAlloc(&p, kMostDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped),
+               "attention: cudaHostAlloc");
     std::memset(p, 0, kMostDevices * sizeof(int));
     return (int *)p;
   }();
@@ -138,7 +146,8 @@ struct illumina_adamw {
   gpu::AdamwClock *clock = nullptr;
   gpu::AdamwChunk *chunks = nullptr;
   gpu::AdamwState state{};
-  ~illumina_adamw() {
+  ~illumina_adamw() {  // at any time, if an interpreter collects it
+    const Uncaptured scope;
     if (memory) cudaFree(memory);
   }
 };

@@ -57,3 +57,24 @@ def test_gradients_made_as_they_are_asked_for(torch):  # noqa: F811
         opt.step(given)
         runs.append((*p, opt.m.clone()))
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_an_optimizer_released_during_a_capture(torch):  # noqa: F811
+    """Python may collect an optimizer at any time, while a graph is being captured too: the capture goes on."""
+    import illumina
+    p, g = torch.ones(5000, device="cuda"), torch.ones(5000, device="cuda")
+    want = [torch.ones(5000, device="cuda") for _ in range(2)]
+    for x in want:
+        illumina.createOptimizer([x]).step([g])
+    opt = illumina.createOptimizer([p])
+    gone = [illumina.createOptimizer([torch.ones(300, device="cuda")]) for _ in range(2)]
+    gone[1].step([g[:300]])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gone[0].destroy()  # reports what goes wrong
+        gone.pop()         # collected
+        opt.step([g])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert opt.steps == 1 and torch.equal(p, want[0])
