@@ -1,9 +1,8 @@
 """AdamW: what a step refuses and keeps of its arguments, and sizes that send its kernels round their loops."""
-import numpy as np
 import pytest
 
-from tests import token_reference as R
-from tests.test_optimizer_gpu import BLOCK, HYPER, codes, places, plain_8_bit, tensors, torch  # noqa: F401
+from tests import test_optimizer_gpu as G
+from tests.test_optimizer_gpu import torch  # noqa: F401
 from tests.test_token_checks_gpu import refused
 
 pytestmark = pytest.mark.gpu
@@ -78,3 +77,28 @@ def test_an_optimizer_released_during_a_capture(torch):  # noqa: F811
     graph.replay()
     torch.cuda.synchronize()
     assert opt.steps == 1 and torch.equal(p, want[0])
+
+
+# chunks of 2048 elements: more than the CTAs of a launch (296 with 32-bit moments, 444 with 8-bit ones) take at once
+LARGE = [1, 255, 0, 600001, 256, 700000, 33, 500003, 4097, 700001]
+MANY = [(7 * i) % 600 + (5000 if i % 3 == 0 else 0) for i in range(1000)]  # three launches a step, over 700 chunks each
+
+
+@pytest.mark.parametrize("grad", ["float32", "bfloat16"])
+@pytest.mark.parametrize("gap", [0, 1])
+def test_32_bit_moments_round_the_loop(torch, monkeypatch, grad, gap):  # noqa: F811
+    monkeypatch.setattr(G, "COUNTS", LARGE)
+    G.test_32_bit_moments(torch, grad, gap)
+
+
+@pytest.mark.parametrize("grad", ["float32", "bfloat16"])
+@pytest.mark.parametrize("counts", [LARGE, MANY], ids=["large", "many"])
+def test_8_bit_moments_round_the_loop_bit_for_bit(torch, monkeypatch, grad, counts):  # noqa: F811
+    monkeypatch.setattr(G, "COUNTS", counts)
+    G.test_8_bit_moments_bit_for_bit(torch, grad)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_captured_steps_round_the_loop(torch, monkeypatch, bits):  # noqa: F811
+    monkeypatch.setattr(G, "COUNTS", MANY)
+    G.test_captured_steps_count_on(torch, bits)

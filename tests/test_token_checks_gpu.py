@@ -124,3 +124,47 @@ def test_parameters_are_taken_without_a_graph(torch, ops):  # noqa: F811
     want = ops.layerNorm(x, w.detach())[0]
     with torch.no_grad():
         assert torch.equal(ops.layerNorm(x, w)[0], want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,c", [(500, 96), (700, 264), (301, 257), (40, 2048), (20, 1033), (5, 5000)])
+def test_norm_entry_points_without_some_results(torch, ops, dtype, rows, c):  # noqa: F811
+    """Through the C entry points: statistics not kept, dx not wanted or in dy's place, one of dw and db alone."""
+    import ctypes as C
+
+    from illumina import _lib
+    lib, precision, stream = _lib.lib(), dtype == "bfloat16", torch.cuda.current_stream().cuda_stream
+    x, dy = randn(torch, rows, c, dtype=dtype), randn(torch, rows, c, dtype=dtype, seed=1)
+    w, b = 1 + randn(torch, c, seed=2) * 0.3, randn(torch, c, seed=3)
+    y, mean, rstd = ops.layerNorm(x, w, b)
+    dx, dw, db = ops.layerNormBackward(dy, x, mean, rstd, w)
+    got = torch.empty_like(x)
+    _lib.check(lib.illumina_op_layer_norm(precision, x.data_ptr(), c, rows, c, w.data_ptr(), b.data_ptr(), 1e-6, got.data_ptr(), c,
+                                          None, None, stream))
+    assert torch.equal(got, y)
+    size = C.c_size_t(0)
+    _lib.check(lib.illumina_op_layer_norm_workspace(rows, c, C.byref(size)))
+    work = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+
+    def backward(dy, dx, dw, db):
+        at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        space = (work.data_ptr(), size.value) if dw is not None or db is not None else (None, 0)
+        _lib.check(lib.illumina_op_layer_norm_backward(precision, dy.data_ptr(), c, x.data_ptr(), c, rows, c, w.data_ptr(),
+                                                       mean.data_ptr(), rstd.data_ptr(), at(dx), c, at(dw), at(db), *space, stream))
+
+    new = lambda: (torch.empty_like(x), torch.empty_like(w), torch.empty_like(w))  # noqa: E731
+    x1, w1, b1 = new()
+    backward(dy, None, w1, b1)
+    assert torch.equal(w1, dw) and torch.equal(b1, db)
+    x1, w1, b1 = new()
+    backward(dy, x1, w1, None)
+    assert torch.equal(x1, dx) and torch.equal(w1, dw)
+    x1, w1, b1 = new()
+    backward(dy, x1, None, b1)
+    assert torch.equal(x1, dx) and torch.equal(b1, db)
+    x1 = dy.clone()
+    backward(x1, x1, w1, b1)
+    assert torch.equal(x1, dx) and torch.equal(w1, dw) and torch.equal(b1, db)
+    x1, _, _ = new()
+    backward(dy, x1, None, None)
+    assert torch.equal(x1, dx)
