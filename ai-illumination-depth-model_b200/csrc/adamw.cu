@@ -21,7 +21,9 @@
 // no random state. Every operation on the way to a code is rounded on its
 // own (no contraction), so that a code does not depend on the compiler. A
 // root that is not zero never becomes code 0: the next step would divide by
-// almost nothing.
+// almost nothing. It stays at code 1 then, above its own value, while the
+// largest of its block is 255 times as large: its element's steps are too
+// small on average, by as much as the root is too large.
 //
 // Measured: 112 tensors of 1.4 M elements, 32-bit moments: 10 us on the GPU,
 // 14 us a call (the pointers are checked and sent each time); 8-bit moments,

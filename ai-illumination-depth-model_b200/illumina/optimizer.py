@@ -14,7 +14,8 @@ BLOCK = 256  # ILLUMINA_ADAMW_BLOCK
 
 class AdamW:
     """Create with createOptimizer. lr, betas, eps and weightDecay may be changed between steps (a captured step keeps
-    the values it was captured with; give lr as a float32 CUDA scalar to change it under a captured step)."""
+    the values it was captured with; give lr as a float32 CUDA scalar to change it under a captured step). The optimizer
+    must outlive the graphs that captured its steps."""
 
     def __init__(self, params, lr, betas, eps, weightDecay, decay, momentBits, gradDtype):
         import torch
@@ -132,6 +133,8 @@ def createOptimizer(params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weightDecay=0
                     gradDtype=None) -> AdamW:
     """AdamW over `params` (contiguous float32 CUDA tensors of one device, updated in place). decay: per tensor, whether
     weight decay applies (default: to all). momentBits 8 keeps the moments as 8-bit codes with a scale for every 256
-    elements of a tensor. gradDtype: float32 (default) or bfloat16. eps is 0 or at least the smallest normal float."""
+    elements of a tensor; the second moment's root is held at 1/255 of its block's largest at least, so elements whose
+    gradients stay below that are stepped by less than with 32 bits on average. gradDtype: float32 (default) or
+    bfloat16. eps is 0 or at least the smallest normal float."""
     import torch
     return AdamW(params, lr, betas, eps, weightDecay, decay, momentBits, gradDtype or torch.float32)

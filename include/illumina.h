@@ -487,8 +487,11 @@ illumina_status illumina_op_attention_set_wait_limit(long long cycles);
  * the second moment's root, with one float32 scale a block in m_scale and
  * v_scale: m = code * scale, v = (code * scale)^2; codes are rounded up where
  * their fraction passes a threshold that sweeps [0, 1) evenly from step to
- * step. A gradient that is not finite spoils its element, and with 8 bits its
- * block.
+ * step. A root that is not zero is held at one code at least: elements whose
+ * gradients stay below 1/255 of their block's largest are stepped as if their
+ * root were that 1/255, on average by less than with 32-bit moments, for as
+ * long as the largest lasts. A gradient that is not finite spoils its element,
+ * and with 8 bits its block.
  * ------------------------------------------------------------------------- */
 
 #define ILLUMINA_ADAMW_BLOCK 256
@@ -513,7 +516,8 @@ typedef struct illumina_adamw_hyper {
 /* Blocks of the flat moments of tensors with these counts. */
 illumina_status illumina_adamw_blocks(const long long *counts, int tensors, long long *blocks);
 /* Uploads the tensor table; no step has been taken. The tensors and moments
- * must outlive the optimiser; no two tensors may overlap. */
+ * must outlive the optimiser, and it the graphs that captured its steps; no
+ * two tensors may overlap. */
 illumina_status illumina_adamw_create(const illumina_adamw_options *opts, illumina_adamw **out);
 illumina_status illumina_adamw_destroy(illumina_adamw *opt);
 /* One step: grads is a host array of device pointers, one a tensor (ignored for

@@ -102,3 +102,29 @@ def test_8_bit_moments_round_the_loop_bit_for_bit(torch, monkeypatch, grad, coun
 def test_captured_steps_round_the_loop(torch, monkeypatch, bits):  # noqa: F811
     monkeypatch.setattr(G, "COUNTS", MANY)
     G.test_captured_steps_count_on(torch, bits)
+
+
+def test_8_bit_roots_are_held_at_one_code(torch):  # noqa: F811
+    """What is promised of elements whose gradients stay far below their block's largest: their root is one code, their
+    steps are smaller than with 32-bit moments."""
+    import illumina
+    g = torch.full((512,), 1e-3, device="cuda")
+    g[::64] = 1.0
+    small = g < 1
+    moved = {}
+    for bits in (8, 32):
+        p = torch.zeros(512, device="cuda")
+        opt = illumina.createOptimizer([p], lr=1e-2, weightDecay=0.0, momentBits=bits)
+        for _ in range(60):
+            opt.step([g])
+        moved[bits] = -p
+    assert bool((opt.moments()[1][small] < 1.1 * 1e-6).all())  # 32 bits: the gradient's square, at most
+    opt = illumina.createOptimizer([torch.zeros(512, device="cuda")], momentBits=8)
+    for _ in range(60):
+        opt.step([g])
+    assert bool((opt.v.view(-1)[small] == 1).all()) and bool((opt.v.view(-1)[~small] >= 254).all())
+    # the first step is exact; a later one divides by the root's code instead of the root, m's code being right on average
+    mean = float(moved[8][small].mean()) / float(moved[32][small].mean())
+    assert 1 / 60 < mean < 0.6
+    # the largest elements' codes are a whole scale: they move as with 32 bits, but for the codes' roundings (1/255 a step)
+    assert float((moved[8][~small] / moved[32][~small] - 1).abs().max()) < 0.02
