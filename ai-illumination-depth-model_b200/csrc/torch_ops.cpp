@@ -66,10 +66,17 @@ void no_gradients(const X &...x) {
   (no_gradient(x), ...);
 }
 
+// A view whose negation is still to be done (z.conj().imag) has other values in
+// memory than it stands for.
+inline void as_stored(const char *name, const at::Tensor &x) {
+  need(!x.is_neg(), name, "is a view with a lazy negation: call resolve_neg() on it");
+}
+
 // A storage tensor: on a CUDA device, float32 or bfloat16, contiguous in its
 // last dimension; returns its precision.
 int storage(const char *name, const at::Tensor &x, int dims = -1) {
   need(x.is_cuda(), name, "must be a CUDA tensor");
+  as_stored(name, x);
   if (dims >= 0 && x.dim() != dims) refuse(std::string(name) + " must have " + std::to_string(dims) + " dimensions");
   need(x.dim() > 0 && (x.size(-1) <= 1 || x.stride(-1) == 1), name, "must be contiguous in its last dimension");
   const auto t = x.scalar_type();
@@ -89,6 +96,7 @@ T *vector_of(const char *name, const MaybeTensor &x, int64_t n, const at::Tensor
   if (!(x->scalar_type() == type && x->device() == like.device() && x->numel() == n && x->is_contiguous()))
     refuse(std::string(name) + " must be " + std::to_string(n) + " contiguous " +
            (type == at::kInt ? "int32" : type == at::kDouble ? "float64" : "float32") + " values on the device of the others");
+  as_stored(name, *x);
   return static_cast<T *>(x->data_ptr());
 }
 float *floats(const char *name, const MaybeTensor &x, int64_t n, const at::Tensor &like) {
@@ -261,6 +269,7 @@ std::tuple<at::Tensor, MaybeTensor> rotary(const at::Tensor &q, const MaybeTenso
   const bool fractional = positions.scalar_type() == at::kFloat;
   need(positions.device() == q.device() && (fractional || positions.scalar_type() == at::kInt),
        "positions must be int32 or float32 on the device of q");
+  as_stored("positions", positions);
   const int64_t pd = positions.dim();
   need((pd == 2 || pd == 3) && positions.size(0) == axes && positions.size(-1) == t && (pd == 2 || positions.size(1) == b),
        "positions must be [axes, tokens] or [axes, batch, tokens]");
@@ -413,6 +422,7 @@ struct Stepper {
       if (!g || g->scalar_type() != type || g->device() != device || g->numel() != counts[i] || !g->is_contiguous())
         refuse("adamw: gradient " + std::to_string(i) + " must be " + std::to_string(counts[i]) + " contiguous " +
                (bf16 ? "bfloat16" : "float32") + " values on " + device.str());
+      as_stored("adamw: a gradient", *g);
       pointers[i] = g->data_ptr();
     }
     illumina_adamw_hyper h{};
@@ -420,6 +430,7 @@ struct Stepper {
       const at::Tensor &t = THPVariable_Unpack(lr.ptr());
       need(t.scalar_type() == at::kFloat && t.device() == device && t.numel() == 1,
            "lr must be a number or one float32 value on the device of the others");
+      as_stored("adamw: lr", t);
       h.lr_device = t.data_ptr<float>();
     } else {
       h.lr = lr.cast<double>();

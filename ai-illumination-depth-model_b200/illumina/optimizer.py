@@ -23,7 +23,7 @@ class AdamW:
         self.params = list(params)
         _require(len(self.params) > 0, "adamw: no tensors")
         for i, p in enumerate(self.params):
-            _require(isinstance(p, torch.Tensor) and p.is_cuda and p.dtype == torch.float32 and p.is_contiguous(),
+            _require(isinstance(p, torch.Tensor) and p.is_cuda and p.dtype == torch.float32 and p.is_contiguous() and not p.is_neg(),
                      f"adamw: parameter {i} must be a contiguous float32 CUDA tensor")
             _require(p.device == self.params[0].device, "adamw: the parameters must be on one device")
         self.device = self.params[0].device

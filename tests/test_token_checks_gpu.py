@@ -168,3 +168,21 @@ def test_norm_entry_points_without_some_results(torch, ops, dtype, rows, c):  # 
     x1, _, _ = new()
     backward(dy, x1, None, None)
     assert torch.equal(x1, dx)
+
+
+def test_views_with_a_lazy_negation(torch, ops):  # noqa: F811
+    import illumina
+    z = torch.view_as_complex(randn(torch, 10, 1, 2)).conj()
+    column = z.imag  # [10, 1]: rows of one element, whose values are not those in memory
+    assert column.is_neg()
+    refused(lambda: ops.layerNorm(column), "lazy negation")
+    assert ops.layerNorm(column.resolve_neg())[0].shape == (10, 1)
+    plan, q = illumina.createRotary(32, [16]), randn(torch, 1, 10, 4, 32)
+    refused(lambda: ops.rotary(q, column.t(), plan), "lazy negation")
+    one = z[:1, 0].imag
+    refused(lambda: ops.layerNorm(randn(torch, 4, 1), one), "lazy negation")
+    opt = illumina.createOptimizer([torch.ones(1, device="cuda")])
+    refused(lambda: opt.step([one]), "lazy negation")
+    opt.lr = one
+    refused(lambda: opt.step([torch.ones(1, device="cuda")]), "lazy negation")
+    refused(lambda: illumina.createOptimizer([one]), "contiguous float32")
