@@ -403,28 +403,13 @@ struct Stepper {
   // where the optimiser writes.
   void stay() const {
     for (size_t i = 0; i < params.size(); i++)
-      if (params[i].data_ptr() != places[i] || params[i].numel() != counts[i])
+      if (params[i].const_data_ptr() != places[i] || params[i].numel() != counts[i])
         refuse("adamw: parameter " + std::to_string(i) + " has moved since the optimizer was created");
     for (size_t i = 0; i < moments.size(); i++)
-      need(moments[i].data_ptr() == places[params.size() + i], "adamw: the moments have moved since the optimizer was created");
+      need(moments[i].const_data_ptr() == places[params.size() + i], "adamw: the moments have moved since the optimizer was created");
   }
 
   void step(const py::sequence &grads, const py::object &lr, double beta1, double beta2, double eps, double decay) {
-    stay();
-    need(py::len(grads) == counts.size(), "adamw: one gradient for each parameter is needed");
-    const auto type = bf16 ? at::kBFloat16 : at::kFloat;
-    std::vector<py::object> held;  // until the launch: a sequence may make its items as they are asked for
-    held.reserve(counts.size());
-    for (size_t i = 0; i < counts.size(); i++) {
-      held.push_back(grads[i]);
-      const py::object &item = held.back();
-      const at::Tensor *g = THPVariable_Check(item.ptr()) ? &THPVariable_Unpack(item.ptr()) : nullptr;
-      if (!g || g->scalar_type() != type || g->device() != device || g->numel() != counts[i] || !g->is_contiguous())
-        refuse("adamw: gradient " + std::to_string(i) + " must be " + std::to_string(counts[i]) + " contiguous " +
-               (bf16 ? "bfloat16" : "float32") + " values on " + device.str());
-      as_stored("adamw: a gradient", *g);
-      pointers[i] = g->data_ptr();
-    }
     illumina_adamw_hyper h{};
     if (THPVariable_Check(lr.ptr())) {
       const at::Tensor &t = THPVariable_Unpack(lr.ptr());
@@ -434,6 +419,25 @@ struct Stepper {
       h.lr_device = t.data_ptr<float>();
     } else {
       h.lr = lr.cast<double>();
+    }
+    need(py::len(grads) == counts.size(), "adamw: one gradient for each parameter is needed");
+    const auto type = bf16 ? at::kBFloat16 : at::kFloat;
+    // a list or tuple holds its items; one that may make them as they are asked for is kept as a list until the launch
+    py::object held = grads;
+    if (!PyList_CheckExact(grads.ptr()) && !PyTuple_CheckExact(grads.ptr())) {
+      py::list made;
+      for (size_t i = 0; i < counts.size(); i++) made.append(grads[i]);
+      held = std::move(made);
+    }
+    stay();  // after the last call into the interpreter
+    PyObject *const *items = PySequence_Fast_ITEMS(held.ptr());
+    for (size_t i = 0; i < counts.size(); i++) {
+      const at::Tensor *g = THPVariable_Check(items[i]) ? &THPVariable_Unpack(items[i]) : nullptr;
+      if (!g || g->scalar_type() != type || g->device() != device || g->numel() != counts[i] || !g->is_contiguous())
+        refuse("adamw: gradient " + std::to_string(i) + " must be " + std::to_string(counts[i]) + " contiguous " +
+               (bf16 ? "bfloat16" : "float32") + " values on " + device.str());
+      as_stored("adamw: a gradient", *g);
+      pointers[i] = g->const_data_ptr();
     }
     h.beta1 = beta1, h.beta2 = beta2, h.eps = eps, h.weight_decay = decay;
     check(illumina_adamw_step(handle, pointers.data(), &h, c10::cuda::getCurrentCUDAStream(device.index()).stream()));
