@@ -217,13 +217,16 @@ __device__ __forceinline__ bool try_wait(uint64_t *bar, uint32_t parity) {
 
 // A wait that ends when another role of the CTA has given up, too.
 struct Waiter {
-  volatile int *fail;
-  long long limit;
+  volatile int *fail;  // in shared memory; the cycles a wait may take follow it
+  static __device__ __forceinline__ void init(volatile int *fail, long long limit) {
+    *fail = 0;
+    *reinterpret_cast<volatile long long *>(fail + 1) = limit;
+  }
   __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity) const {
     if (try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     while (!try_wait(bar, parity)) {
-      if (*fail || clock64() - t0 > limit) {
+      if (*fail || clock64() - t0 > *reinterpret_cast<volatile long long *>(fail + 1)) {
         *fail = 1;
         return false;
       }
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
 
   cudaTriggerProgrammaticLaunchCompletion();  // the join of shares
   if (threadIdx.x == 0) {
-    *fail = 0;
+    Waiter::init(fail, a.wait);
     for (int i = 0; i < 2; i++) mbar_init(q_full + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1), mbar_init(s_free + i, 4);
     mbar_init(drain, 2);
     mbar_init(ask, 2);
@@ -395,7 +398,7 @@ __global__ void __launch_bounds__(threads_of(kFwdGroups), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  const Waiter wait{fail, a.wait};
+  const Waiter wait{fail};
 
   if (warp >= roles.copy) {
     reg_dealloc<88>();
@@ -678,7 +681,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   const int clear_at = mask.q_len % a.tpt ? mask.q_len / a.tpt : INT_MAX;  // the query tile that holds padding
 
   if (threadIdx.x == 0) {
-    *fail = 0;
+    Waiter::init(fail, a.wait);
     mbar_init(kv_full, 1), mbar_init(done, kTwin ? 2 : 1), mbar_init(drain, 2), mbar_init(clean, 1);
     for (int i = 0; i < 2; i++)
       mbar_init(s_full + i, 2), mbar_init(g_full + i, 1), mbar_init(p_full + i, 8), mbar_init(d_full + i, 8);
@@ -700,7 +703,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   // accumulators of the first pipeline, and t_next further those of the second
   const uint32_t t_s = tmem, t_g = tmem + 128, t_dv = tmem + 256, t_dk = tmem + (kTwin ? 384 : 256 + DP);
   constexpr uint32_t t_next = kTwin ? 64 : 0;
-  const Waiter wait{fail, a.wait};
+  const Waiter wait{fail};
 
   if (warp == roles.copy && (threadIdx.x & 31) == 0 && some) {
     mbar_expect_tx(kv_full, 2 * L::kTile);
@@ -939,7 +942,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
 
   cudaTriggerProgrammaticLaunchCompletion();  // dK and dV
   if (threadIdx.x == 0) {
-    *fail = 0;
+    Waiter::init(fail, a.wait);
     mbar_init(q_full, 1), mbar_init(done, 2), mbar_init(drain, 2), mbar_init(ask, 2), mbar_init(clean, 1);
     for (int i = 0; i < 2; i++)
       mbar_init(s_full + i, 1), mbar_init(g_full + i, 1), mbar_init(s_free + i, 8), mbar_init(d_full + i, 8);
@@ -952,7 +955,7 @@ __global__ void __launch_bounds__(threads_of(kBwdGroups), 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const uint32_t t_s = tmem, t_g = tmem + 128, t_dq = tmem + 256;
-  const Waiter wait{fail, a.wait};
+  const Waiter wait{fail};
 
   if (warp == roles.copy && (threadIdx.x & 31) == 0 && t1 > 0) {
     mbar_expect_tx(q_full, 2 * L::kBoxes * a.group * a.tpt * 128);
