@@ -26,7 +26,7 @@
 // small on average, by as much as the root is too large.
 //
 // Measured: 112 tensors of 1.4 M elements, 32-bit moments: 10 us on the GPU,
-// 14 us a call (the pointers are checked and sent each time); 8-bit moments,
+// 12 us a call (the pointers are checked and sent each time); 8-bit moments,
 // bf16 gradients: 213 us for 81.9 M elements (5.4 TB/s, 14 bytes an element),
 // bound by instruction issue: 64 instructions an element, where one value an
 // instruction took 82 and 255 us. The moments as floats: 135 us (6.1 TB/s).
@@ -99,14 +99,14 @@ __device__ __forceinline__ void unpack_pairs(typename RawPack<T, 4>::type raw, f
   to[0] = make_float2(e[0], e[1]), to[1] = make_float2(e[2], e[3]);
 }
 
-// Bytes j and j + 1 of w as floats, without the conversion unit (which the square roots
-// and reciprocals need): 2^23 + byte, minus 2^23 (and the bias of signed codes).
 // A sum of products that must not be merged with them: the compiler merges
 // packed products and sums, rounding modes or not, but not across widths.
 __device__ __forceinline__ float2 add_apart(float2 a, float2 b) {
   return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// Bytes j and j + 1 of w as floats, without the conversion unit (which the square roots
+// and reciprocals need): 2^23 + byte, minus 2^23 (and the bias of signed codes).
 __device__ __forceinline__ float2 byte_values(uint32_t w, int j, float bias) {
   return __fadd2_rn(make_float2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7650 + j)),
                                 __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7651 + j))),

@@ -17,7 +17,7 @@
 // Measured at 50176 rows of 704, bf16: forward 31 us (4.5 TB/s), backward with
 // its second launch 44 us (4.9 TB/s, 67 us with the rows in registers); at
 // 25088 rows of 1024, f32, backward 57 us (5.4 TB/s). A single frame of 196
-// rows is a launch: 4 us on the GPU, 11 us a call.
+// rows is a launch: 4 us on the GPU, 10 us a call.
 #include <algorithm>
 
 #include "token_common.cuh"

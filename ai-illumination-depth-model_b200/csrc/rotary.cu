@@ -11,7 +11,7 @@
 //
 // Measured: 2 clips of 32 frames of 196 tokens, 12 + 4 heads of 64, three axes,
 // bf16: 13 us (3.9 TB/s), a third of it launch and ramp; one frame 5 us on
-// the GPU, 11 us a call.
+// the GPU, 10 us a call.
 #include "token_common.cuh"
 #include "token_ops.h"
 

@@ -211,12 +211,14 @@ def attention(q, k, v, scale=None, causalBlock=0, qLens=None, kLens=None, stream
     most 128; scale defaults to headDim**-0.5. qLens, kLens (int32 [batch]): lengths of a padded batch; padding may
     hold anything and its rows come back as zeros. causalBlock n: the last query stands at the last key, and a query
     sees its own block of n keys and those before it (1: causal tokens; the tokens of a frame: causal frames). Rows
-    that see no key are zeros with lse -inf."""
+    that see no key are zeros with lse -inf. In bfloat16 the probabilities are rounded to bfloat16 before their product
+    with v (sums, maxima and lse are not): out is about 2.5e-3 of its norm off, where rounding out alone makes 1.7e-3."""
     return _call("attention", stream, q, k, v, scale, causalBlock, qLens, kLens)
 
 
 def attentionBackward(dOut, q, k, v, out, lse, scale=None, causalBlock=0, qLens=None, kLens=None, stream=None):
-    """Gradients (dq, dk, dv) of attention, from its results out and lse and the same masks."""
+    """Gradients (dq, dk, dv) of attention, from its results out and lse and the same masks. In bfloat16 the
+    probabilities and their gradients are rounded to bfloat16 before their products, as in attention."""
     return _call("attention_backward", stream, dOut, q, k, v, out, lse, scale, causalBlock, qLens, kLens)
 
 

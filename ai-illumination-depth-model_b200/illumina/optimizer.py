@@ -96,7 +96,7 @@ class AdamW:
         return n.value
 
     def state(self) -> dict:
-        """What loadState takes: the step count and copies of the moments as they are held."""
+        """What loadState takes: the step count and copies of the moments as they are held (on the current stream)."""
         copy = lambda x: None if x is None else x.clone()  # noqa: E731
         return {"step": self.steps, "m": copy(self.m), "v": copy(self.v), "mScale": copy(self.mScale),
                 "vScale": copy(self.vScale)}

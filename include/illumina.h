@@ -367,8 +367,9 @@ illumina_status illumina_op_bilateral(const float *low, int lh, int lw, int low_
  * token is a pixel of a channels-last map) or over the frames of a clip,
  * forward and backward. No counterpart in the reference.
  *
- * Storage is ILLUMINA_PRECISION_F32 or ILLUMINA_PRECISION_BF16; sums,
- * statistics and softmax are held in 32 bits. All pointers are device pointers
+ * Storage is ILLUMINA_PRECISION_F32 or ILLUMINA_PRECISION_BF16; sums and
+ * statistics are held in 32 bits, those of a softmax too (what attention rounds
+ * to bf16 on the way is said there). All pointers are device pointers
  * of the current device, strides are in elements, the last dimension is
  * contiguous. The calls queue their kernels on `stream` and return; they
  * allocate nothing and can be captured. A workspace belongs to the call until
@@ -441,7 +442,13 @@ typedef struct illumina_attention_tensor {
  * sees every key. causal_block n > 0: the last query stands at the last key, a
  * query sees its own block of n keys and those before it (1: causal tokens; the
  * tokens of a frame: causal frames). A row that sees no key gives zeros and lse
- * -inf. Keys that only the causal mask hides must be finite.
+ * -inf. Keys and, in the backward, queries and their dout that only the causal
+ * mask hides from one another must be finite.
+ * With bf16 storage the tensor cores take the products (head_dim a multiple of
+ * 8, tensors at 16-byte boundaries, a positive scale): probabilities and their
+ * gradients are rounded to bf16 before the product that takes them, and the
+ * backward reads the rounded out. Results are about 2.5e-3 of their norm off,
+ * where rounding them alone makes 1.7e-3. Store in F32 where that is too much.
  * lse: [batch][heads][q_tokens] log of the softmax's sum, for the backward. */
 typedef struct illumina_attention_args {
   int precision;
@@ -521,7 +528,7 @@ illumina_status illumina_adamw_blocks(const long long *counts, int tensors, long
 illumina_status illumina_adamw_create(const illumina_adamw_options *opts, illumina_adamw **out);
 illumina_status illumina_adamw_destroy(illumina_adamw *opt);
 /* One step: grads is a host array of device pointers, one a tensor (ignored for
- * empty tensors). The step count is kept on the device, so that a captured
+ * empty tensors), which lie apart from the parameters and moments. The step count is kept on the device, so that a captured
  * step counts on when it is replayed. Steps of one optimiser must not overlap. */
 illumina_status illumina_adamw_step(illumina_adamw *opt, const void *const *grads, const illumina_adamw_hyper *hyper,
                                     void *stream);
